@@ -322,6 +322,96 @@ int omni_attn_bwd_noalloc_gfx950(const void* q, const void* k, const void* v, co
                                  int seqlen_orig, int dtype, float softcap, void* stream);
 
 /*
+ * Norm and rotation of query and key heads in one pass (no counterpart in the reference, whose attention takes them
+ * ready).  For every head of every token
+ *   n = x * rsqrt(mean(x^2) + eps) * weight          (without a weight: n = x)
+ *   y_a = n_a cos - n_b sin,   y_b = n_b cos + n_a sin
+ * for the pairs (a, b) = (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`, of the first rotary_dim
+ * dimensions; the others stay n.  Everything in 32 bits, rounded once.
+ *
+ *   q, k       [B, Hq | Hk, S, D] at their strides, multiples of 4 elements, on 8-byte boundaries (16 and 8: wider
+ *              loads); q_out, k_out likewise (written completely; another layout than q's is fine).
+ *   table      [table_rows, rotary_dim] fp32, 16-byte aligned: the cosines of a position's rotary_dim / 2 angles,
+ *              then the sines.
+ *   positions  [B, S] rows of the table, int32 or (positions_64) int64, positions_batch entries from batch element
+ *              to batch element (0: shared).  One outside the table reads its first or last row.
+ *   q_weight, k_weight  [D], of the operands' type or (weights_f32) fp32, 16-byte aligned, or NULL.
+ * D is a multiple of 8 up to 256, rotary_dim a multiple of 8 up to D.
+ *
+ * Backward: dq, dk from dq_out, dk_out (g = R^T dy, r = rsqrt(mean(x^2) + eps): dx = r (g w - x r^2 mean(g w x))) and,
+ * where asked for, dq_weight, dk_weight = the sum of g x r over tokens and heads, of the weights' type.  q and k are
+ * needed for the sides that have a weight.  The workspace is needed where a weight's gradient is asked for.
+ */
+int omni_attn_qk_rotary_gfx950(const void* q, const void* k, omni_attn_strides q_at, omni_attn_strides k_at,
+                               void* q_out, void* k_out, omni_attn_strides q_out_at, omni_attn_strides k_out_at,
+                               const float* table, const void* positions, int64_t positions_batch, int positions_64,
+                               const void* q_weight_or_null, const void* k_weight_or_null, int weights_f32,
+                               int B, int S, int Hq, int Hk, int D, int rotary_dim, int table_rows, float eps,
+                               int interleaved, int dtype, void* stream);
+size_t omni_attn_qk_rotary_bwd_workspace_bytes(int B, int S, int D);
+int omni_attn_qk_rotary_bwd_gfx950(const void* dq_out, const void* dk_out, const void* q, const void* k,
+                                   omni_attn_strides dq_out_at, omni_attn_strides dk_out_at, omni_attn_strides q_at,
+                                   omni_attn_strides k_at, void* dq, void* dk, omni_attn_strides dq_at,
+                                   omni_attn_strides dk_at, void* dq_weight_or_null, void* dk_weight_or_null,
+                                   const float* table, const void* positions, int64_t positions_batch, int positions_64,
+                                   const void* q_weight_or_null, const void* k_weight_or_null, int weights_f32,
+                                   void* workspace, size_t workspace_bytes, int B, int S, int Hq, int Hk, int D,
+                                   int rotary_dim, int table_rows, float eps, int interleaved, int dtype, void* stream);
+
+/*
+ * New tokens of a batch of sequences enter a paged cache.  Sequence b has the tokens cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 (cu_seqlens [sequences + 1] int32) and kv_lens[b] keys with them: token i of it is at position
+ * pos = kv_lens[b] - cu_seqlens[b + 1] + i, in row pos % page_size of page page_table[b, pos / page_size].
+ *
+ *   k, v       [tokens, Hk, D] at (head, row) strides as above.  k is normed and rotated as above on the way, v goes
+ *              through bit for bit.
+ *   q, q_out   [tokens, Hq, D], or NULL with Hq = 0: the tokens' queries, normed and rotated beside them.
+ *   positions  [tokens]: table rows to rotate by, or NULL: the token's position in its sequence.
+ *   k_pages, v_pages  [num_pages, Hk, page_size, D] contiguous; page_size a power of two.
+ *   page_table [sequences, max_pages] int32.
+ * A token whose page number is outside [0, num_pages), or whose position is negative or behind the page table, is not
+ * written; nor is anything but the new tokens' rows.  Two new tokens must not name one row.  q_out rows of tokens behind
+ * the last sequence are zeros.  rotary_dim 0 (and table NULL): no rotation.
+ */
+int omni_attn_cache_append_gfx950(const void* q_or_null, const void* k, const void* v, omni_attn_strides q_at,
+                                  omni_attn_strides k_at, omni_attn_strides v_at, void* q_out_or_null,
+                                  omni_attn_strides q_out_at, void* k_pages, void* v_pages, const int32_t* page_table,
+                                  const int32_t* kv_lens, const int32_t* cu_seqlens, const float* table_or_null,
+                                  const void* positions_or_null, int positions_64, const void* q_weight_or_null,
+                                  const void* k_weight_or_null, int weights_f32, int tokens, int sequences, int Hq, int Hk,
+                                  int D, int num_pages, int page_size, int max_pages, int rotary_dim, int table_rows,
+                                  float eps, int interleaved, int dtype, void* stream);
+
+/*
+ * Attention of packed sequences with grouped heads:
+ *   o[t, h, :] = softmax_j( cap(q[t, h, :] . k[j, h / (Hq / Hk), :] / sqrt(D)) ) v[j, h / (Hq / Hk), :]
+ * over the keys j of token t's sequence, with `causal` those up to its own position.  Sequences as in
+ * omni_attn_cache_append_gfx950.
+ *
+ * omni_attn_packed_gfx950: whole prompts; k and v are [tokens, Hk, D] beside q [tokens, Hq, D], all at (head, row)
+ * strides that are multiples of 8 elements up to 2^24, on 16-byte boundaries.
+ * omni_attn_paged_gfx950: the tokens of q (one per sequence, a few, a chunk of a prompt) over the kv_lens[b] keys that
+ * pages hold, theirs included; the last token is at position kv_lens[b] - 1.  page_size from 16.  Page numbers outside
+ * [0, num_pages) are cut to it; keys at or behind kv_lens[b] are never read.
+ *   o          [tokens, Hq, D] contiguous, written completely; lse [tokens, Hq] fp32 (natural logarithm) or NULL.
+ *              Rows without a key, and rows of tokens behind the last sequence, are zeros (lse -inf).
+ *   workspace  omni_attn_packed_workspace_bytes, omni_attn_paged_workspace_bytes of the current device (may be 0),
+ *              16-byte aligned; its contents before and after the call are meaningless.
+ * D is 32, 64 or 128; softcap as in omni_attn_fwd_gfx950.  Two calls that may run at the same time need two workspaces.
+ */
+size_t omni_attn_packed_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D);
+int omni_attn_packed_gfx950(const void* q, const void* k, const void* v, omni_attn_strides q_at, omni_attn_strides k_at,
+                            omni_attn_strides v_at, void* o, float* lse_or_null, const int32_t* cu_seqlens,
+                            void* workspace, size_t workspace_bytes, int tokens, int sequences, int Hq, int Hk, int D,
+                            int causal, int dtype, float softcap, void* stream);
+size_t omni_attn_paged_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D);
+int omni_attn_paged_gfx950(const void* q, omni_attn_strides q_at, const void* k_pages, const void* v_pages, void* o,
+                           float* lse_or_null, const int32_t* page_table, const int32_t* kv_lens,
+                           const int32_t* cu_seqlens, void* workspace, size_t workspace_bytes, int tokens,
+                           int sequences, int Hq, int Hk, int D, int num_pages, int page_size, int max_pages, int causal,
+                           int dtype, float softcap, void* stream);
+
+/*
  * Measurement aid (no counterpart in the reference): enqueue a kernel that issues nothing but
  * 32x32x16 matrix instructions of `dtype` from registers -- two workgroups of four waves per
  * compute unit, `iters` x 8 instructions per wave -- so that a caller timing the launch can

@@ -52,8 +52,9 @@ RESOURCES_JSON = os.path.join(OBJ, "kernel_resources.json")
 # The backward kernels and the forward with split lists keep scalar values in spare vector lanes here
 # and there (SGPR spills, no memory behind them): for them only scratch memory and spilled vector registers fail the build.
 MIN_WAVES_PER_SIMD = {"fwd_kernel": 2, "fwd_ksplit": 2, "bwd_dq_kernel": 2, "bwd_dq_short": 2, "bwd_dq_ksplit": 2,
-                      "bwd_dkdv_kernel": 2, "bwd_dkdv_split": 2, "fwd_generic_": 2}
-SGPR_SPILLS_ALLOWED = ("bwd_dq_", "bwd_dkdv_", "fwd_ksplit", "fwd_generic_")
+                      "bwd_dkdv_kernel": 2, "bwd_dkdv_split": 2, "fwd_generic_": 2, "serve_tile": 2, "serve_few": 2,
+                      "qk_rotary_kernel": 3, "cache_append_kernel": 3, "qk_rotary_bwd": 2}
+SGPR_SPILLS_ALLOWED = ("bwd_dq_", "bwd_dkdv_", "fwd_ksplit", "fwd_generic_", "serve_tile", "qk_rotary_bwd")
 # For the generic kernel scratch memory is what counts.  Forms that read rows at any alignment (E1E) have some: up to 32 columns
 # and 97 - 128 in fp16 (two registers' worth; at B=1 H=8 S=2048 D=125 48.5 us, 52.9 without, where the addresses of the
 # loads are worked out anew in every step) and 225 - 256 (half a tile's rows in flight in registers; with four waves, which
@@ -148,7 +149,14 @@ def build_capi(jobs):
         cmds.append([HIPCC] + DEVICE_FLAGS + [
             "-DOMNI_INST_BF16=%d" % bf, "-DOMNI_INST_D=%d" % d,
             "-c", os.path.join(CSRC, "omni_attn_bwd_inst.hip"), "-o", obj])
-    for src in ("omni_attn_capi", "omni_attn_probe", "omni_attn_mask_pack", "omni_attn_mask_build", "omni_attn_fwd_generic"):
+    for bf, d in INSTANCES:
+        obj = os.path.join(OBJ, "serving_inst_%s_d%d.o" % ("bf16" if bf else "f16", d))
+        objs.append(obj)
+        cmds.append([HIPCC] + DEVICE_FLAGS + [
+            "-DOMNI_INST_BF16=%d" % bf, "-DOMNI_INST_D=%d" % d,
+            "-c", os.path.join(CSRC, "omni_attn_serving_inst.hip"), "-o", obj])
+    for src in ("omni_attn_capi", "omni_attn_probe", "omni_attn_mask_pack", "omni_attn_mask_build", "omni_attn_fwd_generic",
+                "omni_attn_rotary", "omni_attn_serving"):
         obj = os.path.join(OBJ, src + ".o")
         objs.append(obj)
         cmds.append([HIPCC] + DEVICE_FLAGS + ["-c", os.path.join(CSRC, src + ".hip"), "-o", obj])
@@ -182,7 +190,7 @@ def build_ext():
     for inc in includes:
         cmd += ["-isystem", inc]
     cmd += ["-I", os.path.join(ROOT, "include"),
-            os.path.join(CSRC, "omni_attn_pybind.cpp"), "-o", out,
+            os.path.join(CSRC, "omni_attn_pybind.cpp"), os.path.join(CSRC, "omni_attn_pybind_serving.cpp"), "-o", out,
             "-L", HERE, "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN",
             "-L", torch_lib, "-Wl,-rpath," + torch_lib,
             "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python"]

@@ -85,6 +85,17 @@ int query_topology(DeviceTopology* out) {
 }
 }  // namespace
 
+// XCDs and compute units of the current device, for the other entry points.
+namespace omni_attn {
+int device_units(int* n_xcd, int* cus) {
+  DeviceTopology t;
+  if (const int e = query_topology(&t)) return e;
+  *n_xcd = t.n_xcd;
+  *cus = t.n_xcd * t.cus_per_xcd;
+  return 0;
+}
+}  // namespace omni_attn
+
 namespace {
 // [B, H, S, D] contiguous.
 omni_attn_strides contiguous(int H, int S, int D) {

@@ -625,6 +625,8 @@ pybind11::tuple omni_attn_build_prefix_mask(torch::Tensor source, bool spans, in
 
 }  // namespace
 
+void bind_serving(pybind11::module& m);  // rotation, the paged cache and its attention
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "gfx950 block-sparse FlashAttention-2 forward (omni-attention operator surface)";
   m.def("omni_attn_mma_stages_split_q_shared_kv", &omni_attn_op,
@@ -658,5 +660,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("omni_attn_attend_autograd", &omni_attn_attend_autograd, "omni_attn_attend_autograd (differentiable)");
   m.def("omni_attn_build_prefix_mask", &omni_attn_build_prefix_mask,
         "omni_attn_build_prefix_mask (block mask of spans or prefix lengths)");
+  bind_serving(m);
   m.def("abi_version", []() { return omni_attn_abi_version(); });
 }

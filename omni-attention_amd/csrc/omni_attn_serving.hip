@@ -1,0 +1,169 @@
+// C ABI of the attention of packed sequences: checks, the plan of the launch, instance dispatch.
+#include "../../include/omni_attn_gfx950.h"
+#include "omni_attn_serving_kernel.hpp"
+#include "omni_attn_serving_plan.hpp"
+
+#include <cmath>
+
+namespace omni_attn {
+
+// (beside the forward's entry points)
+int device_units(int* n_xcd, int* cus);
+
+template <bool BF16, int D>
+int launch_serve(const ServeParams& p, bool tiles, unsigned blocks, hipStream_t stream);
+template <> int launch_serve<false, 32>(const ServeParams&, bool, unsigned, hipStream_t);
+template <> int launch_serve<false, 64>(const ServeParams&, bool, unsigned, hipStream_t);
+template <> int launch_serve<false, 128>(const ServeParams&, bool, unsigned, hipStream_t);
+template <> int launch_serve<true, 32>(const ServeParams&, bool, unsigned, hipStream_t);
+template <> int launch_serve<true, 64>(const ServeParams&, bool, unsigned, hipStream_t);
+template <> int launch_serve<true, 128>(const ServeParams&, bool, unsigned, hipStream_t);
+
+namespace {
+
+bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+
+// Rows of 16-byte pieces; a step of 64 rows lies within 4 GiB.
+int check_rows(const omni_attn_strides& at) {
+  if (at.head % 8 != 0 || at.row % 8 != 0) return OMNI_ATTN_ERR_MISALIGNED;
+  if (at.head < 0 || at.row < 0) return OMNI_ATTN_ERR_BAD_SHAPE;
+  if (at.row > (1LL << 24)) return OMNI_ATTN_ERR_TOO_LARGE;
+  return OMNI_ATTN_OK;
+}
+
+int check_sizes(int T, int B, int Hq, int Hk, int D) {
+  if (D != 32 && D != 64 && D != 128) return OMNI_ATTN_ERR_UNSUPPORTED_HEAD_DIM;
+  if (T <= 0 || B <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk != 0) return OMNI_ATTN_ERR_BAD_SHAPE;
+  // (rows of a key head, and rows in all, are numbered with an int)
+  if ((long long)T * Hq > 0x3fffffffLL || (long long)B * Hk > 0x3fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
+  return OMNI_ATTN_OK;
+}
+
+int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes, int dtype, float softcap, void* stream) {
+  if (!(softcap >= 0.f) || std::isinf(softcap)) return OMNI_ATTN_ERR_BAD_SHAPE;
+  if (dtype != OMNI_ATTN_DTYPE_F16 && dtype != OMNI_ATTN_DTYPE_BF16) return OMNI_ATTN_ERR_UNSUPPORTED_DTYPE;
+  int cus = 0;
+  if (const int e = device_units(&p.n_xcd, &cus)) {
+    record_hip_error(e);
+    return OMNI_ATTN_ERR_LAUNCH;
+  }
+  p.G = Hq / p.Hk;
+  p.group = fast_div(uint32_t(p.G));
+  p.heads = fast_div(uint32_t(p.Hk));
+  const ServePlan plan = plan_serve(p.T, p.B, p.Hk, p.G, p.page_table != nullptr, cus);
+  const int64_t blocks = serve_blocks(plan.units, p.Hk, p.n_xcd);
+  if (blocks > 0x7fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
+  p.share = plan.share;
+  p.units = int(plan.units);
+  if (plan.share != 0.f) {
+    if (!workspace || workspace_bytes < plan.workspace_bytes(p.Hk, D)) return OMNI_ATTN_ERR_WORKSPACE;
+    if (misaligned(workspace, 16)) return OMNI_ATTN_ERR_MISALIGNED;
+    p.sums = static_cast<float*>(workspace);
+    p.stats = p.sums + plan.units * p.Hk * plan.rows() * D;
+  }
+  p.softcap = softcap;
+  p.cap_c2 = softcap > 0.f ? float(2.0 * 1.4426950408889634 / (std::sqrt(double(D)) * double(softcap))) : 0.f;
+  p.sl2 = softcap > 0.f ? float(1.4426950408889634) : float(1.4426950408889634 / std::sqrt(double(D)));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool bf = dtype == OMNI_ATTN_DTYPE_BF16;
+  const unsigned n = unsigned(blocks);
+  int e;
+  switch (D) {
+    case 32: e = bf ? launch_serve<true, 32>(p, plan.tiles, n, s) : launch_serve<false, 32>(p, plan.tiles, n, s); break;
+    case 64: e = bf ? launch_serve<true, 64>(p, plan.tiles, n, s) : launch_serve<false, 64>(p, plan.tiles, n, s); break;
+    default: e = bf ? launch_serve<true, 128>(p, plan.tiles, n, s) : launch_serve<false, 128>(p, plan.tiles, n, s); break;
+  }
+  if (e != 0) {
+    record_hip_error(e);
+    return OMNI_ATTN_ERR_LAUNCH;
+  }
+  return OMNI_ATTN_OK;
+}
+
+size_t workspace_of(int T, int B, int Hq, int Hk, int D, bool paged) {
+  int xcds = 0, cus = 0;
+  if (check_sizes(T, B, Hq, Hk, D) != OMNI_ATTN_OK) return 0;
+  if (const int e = device_units(&xcds, &cus)) {
+    record_hip_error(e);
+    return 0;
+  }
+  return plan_serve(T, B, Hk, Hq / Hk, paged, cus).workspace_bytes(Hk, D);
+}
+
+}  // namespace
+}  // namespace omni_attn
+
+extern "C" size_t omni_attn_packed_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D) {
+  return omni_attn::workspace_of(tokens, sequences, Hq, Hk, D, false);
+}
+extern "C" size_t omni_attn_paged_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D) {
+  return omni_attn::workspace_of(tokens, sequences, Hq, Hk, D, true);
+}
+
+extern "C" int omni_attn_packed_gfx950(const void* q, const void* k, const void* v, omni_attn_strides q_at,
+                                       omni_attn_strides k_at, omni_attn_strides v_at, void* o, float* lse_or_null,
+                                       const int32_t* cu_seqlens, void* workspace, size_t workspace_bytes, int tokens,
+                                       int sequences, int Hq, int Hk, int D, int causal, int dtype, float softcap,
+                                       void* stream) {
+  using namespace omni_attn;
+  if (!q || !k || !v || !o || !cu_seqlens) return OMNI_ATTN_ERR_NULL_POINTER;
+  if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(o, 16) || misaligned(lse_or_null, 4) ||
+      misaligned(cu_seqlens, 4))
+    return OMNI_ATTN_ERR_MISALIGNED;
+  if (const int rc = check_sizes(tokens, sequences, Hq, Hk, D)) return rc;
+  for (const omni_attn_strides* at : {&q_at, &k_at, &v_at})
+    if (const int rc = check_rows(*at)) return rc;
+  ServeParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.q_row = q_at.row;
+  p.q_head = q_at.head;
+  p.k_at = {0, k_at.head, uint32_t(k_at.row)};
+  p.v_at = {0, v_at.head, uint32_t(v_at.row)};
+  p.o = static_cast<uint16_t*>(o);
+  p.lse = lse_or_null;
+  p.cu = cu_seqlens;
+  p.T = tokens;
+  p.B = sequences;
+  p.Hk = Hk;
+  p.causal = causal != 0;
+  return serve(p, Hq, D, workspace, workspace_bytes, dtype, softcap, stream);
+}
+
+extern "C" int omni_attn_paged_gfx950(const void* q, omni_attn_strides q_at, const void* k_pages, const void* v_pages,
+                                      void* o, float* lse_or_null, const int32_t* page_table, const int32_t* kv_lens,
+                                      const int32_t* cu_seqlens, void* workspace, size_t workspace_bytes, int tokens,
+                                      int sequences, int Hq, int Hk, int D, int num_pages, int page_size, int max_pages,
+                                      int causal, int dtype, float softcap, void* stream) {
+  using namespace omni_attn;
+  if (!q || !k_pages || !v_pages || !o || !page_table || !kv_lens || !cu_seqlens) return OMNI_ATTN_ERR_NULL_POINTER;
+  if (misaligned(q, 16) || misaligned(k_pages, 16) || misaligned(v_pages, 16) || misaligned(o, 16) ||
+      misaligned(lse_or_null, 4) || misaligned(page_table, 4) || misaligned(kv_lens, 4) || misaligned(cu_seqlens, 4))
+    return OMNI_ATTN_ERR_MISALIGNED;
+  if (const int rc = check_sizes(tokens, sequences, Hq, Hk, D)) return rc;
+  if (const int rc = check_rows(q_at)) return rc;
+  // (a wave's load fills up to 16 rows, of one page)
+  if (num_pages <= 0 || max_pages <= 0 || page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)) != 0)
+    return OMNI_ATTN_ERR_BAD_SHAPE;
+  if ((long long)max_pages * page_size > 0x3fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
+  ServeParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k_pages);
+  p.v = static_cast<const uint16_t*>(v_pages);
+  p.q_row = q_at.row;
+  p.q_head = q_at.head;
+  p.o = static_cast<uint16_t*>(o);
+  p.lse = lse_or_null;
+  p.cu = cu_seqlens;
+  p.kv_lens = kv_lens;
+  p.page_table = page_table;
+  p.num_pages = num_pages;
+  p.max_pages = max_pages;
+  p.page_shift = __builtin_ctz(unsigned(page_size));
+  p.T = tokens;
+  p.B = sequences;
+  p.Hk = Hk;
+  p.causal = causal != 0;
+  return serve(p, Hq, D, workspace, workspace_bytes, dtype, softcap, stream);
+}

@@ -1,0 +1,57 @@
+// Attention of packed sequences, one translation unit per (element type, head_dim): compiled several times with
+// -DOMNI_INST_BF16={0,1} -DOMNI_INST_D={32,64,128}; each object defines the kernels of that pair, for packed and paged
+// keys, behind one C++ symbol.
+#include "omni_attn_serving_kernel.hpp"
+
+#ifndef OMNI_INST_BF16
+#error "compile with -DOMNI_INST_BF16=0|1"
+#endif
+#ifndef OMNI_INST_D
+#error "compile with -DOMNI_INST_D=32|64|128"
+#endif
+
+namespace omni_attn {
+namespace {
+
+template <auto Kernel>
+int launch(const ServeParams& p, unsigned blocks, unsigned threads, size_t lds, hipStream_t stream) {
+  static std::atomic<bool> lds_limit_set[kMaxDevices];
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return int(e);
+  const bool cached = dev >= 0 && dev < kMaxDevices;
+  if (lds != 0 && (!cached || !lds_limit_set[dev].load(std::memory_order_acquire))) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+    if (e != hipSuccess) return int(e);
+    if (cached) lds_limit_set[dev].store(true, std::memory_order_release);
+  }
+  ServeParams params = p;
+  void* args[] = {&params};
+  return int(hipLaunchKernel(reinterpret_cast<const void*>(Kernel), dim3(blocks), dim3(threads), args, lds, stream));
+}
+
+}  // namespace
+
+template <bool BF16, int D>
+int launch_serve(const ServeParams& p, bool tiles, unsigned blocks, hipStream_t stream);
+
+template <>
+int launch_serve<OMNI_INST_BF16 != 0, OMNI_INST_D>(const ServeParams& p, bool tiles, unsigned blocks, hipStream_t stream) {
+  constexpr bool BF = OMNI_INST_BF16 != 0;
+  constexpr int D = OMNI_INST_D;
+  const bool paged = p.page_table != nullptr;
+  int e;
+  if (tiles) {
+    e = paged ? launch<serve_tile_kernel<BF, D, true>>(p, blocks, 256, kTileLdsBytes<D>, stream)
+              : launch<serve_tile_kernel<BF, D, false>>(p, blocks, 256, kTileLdsBytes<D>, stream);
+  } else {
+    e = paged ? launch<serve_few_kernel<BF, D, true>>(p, blocks, 64, kFewLdsBytes<D>, stream)
+              : launch<serve_few_kernel<BF, D, false>>(p, blocks, 64, kFewLdsBytes<D>, stream);
+  }
+  if (e != 0 || p.share == 0.f) return e;
+  const unsigned join_blocks = unsigned((int64_t(p.T) * p.Hk * p.G + 3) / 4);
+  return tiles ? launch<serve_join_kernel<BF, D, 128>>(p, join_blocks, 256, 0, stream)
+               : launch<serve_join_kernel<BF, D, 32>>(p, join_blocks, 256, 0, stream);
+}
+
+}  // namespace omni_attn

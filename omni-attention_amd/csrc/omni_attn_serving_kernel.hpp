@@ -1,0 +1,918 @@
+// Attention of packed sequences: new tokens of many sequences, one behind the other, over their own keys and
+// values, which lie packed the same way or in the pages of a cache.  Query heads come in groups of G that share a
+// key head.
+//   O[t, h, :] = softmax_j( cap(Q[t, h, :] . K[j, h / G, :] / sqrt(D)) ) V[j, h / G, :]
+// over the keys j of the token's sequence: those up to the token's own position, or all of them.  Sequence b has
+// the tokens cu[b] .. cu[b + 1] - 1 and kv keys; its last token is at position kv - 1.
+//
+// As in the block-sparse forward everything is computed transposed, so that a lane owns one query row: S^T = K Q^T
+// and O^T = V^T P^T with 32x32x16 matrix instructions, P in registers throughout.  A row here is a token and one of
+// the G heads of a group: the rows of a tile share one key head, so K and V are read once for all of them, a single
+// token fills G rows, and a tile of a prompt has few tokens, so little of its last steps is masked.
+//
+// Work is dealt on the device, because lengths are there: every workgroup reads the lengths (64 sequences per wave at
+// a time) and finds the unit with its number.  A unit is a tile of rows and a range of keys (all of them, or where
+// there are fewer units than the card holds, parts that are equal over the whole batch).  Parts leave their sums
+// and maxima in a workspace, and a second kernel joins them.
+#pragma once
+
+#include "omni_attn_fwd_kernel.hpp"
+
+namespace omni_attn {
+
+struct ServeParams {
+  const uint16_t* q;  // [T, Hk * G, D] at q_row, q_head
+  const uint16_t* k;  // packed [T, Hk, D] at their strides, or pages [num_pages, Hk, page, D]
+  const uint16_t* v;
+  int64_t q_row, q_head;
+  RowStrides k_at, v_at;  // (h, row) of packed keys and values
+  uint16_t* o;            // [T, Hk * G, D]
+  float* lse;             // [T, Hk * G] or null
+  const int32_t* cu;      // [B + 1]
+  const int32_t* kv_lens;     // [B]; null: packed
+  const int32_t* page_table;  // [B, max_pages]
+  int num_pages, max_pages, page_shift;
+  int B, T, Hk, G;
+  FastDiv group;       // by G
+  FastDiv heads;       // by Hk
+  int n_xcd;
+  int causal;
+  float share;         // units per key head that the batch's steps are shared over; 0: whole tiles
+  int units;           // units per key head that there is a place for
+  float* sums;         // [units, Hk, M, D] unscaled O of parts
+  float* stats;        // [units, Hk, M, 2] their reference points (log2 domain) and sums of weights
+  float sl2, softcap, cap_c2;
+};
+
+constexpr int kStepKeys = 64;  // lengths are counted in steps of as many keys
+
+// Inclusive sum over the lanes before this one, and this one.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
+}
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+__device__ __forceinline__ float wave_sum(float x) {
+  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
+  return x;
+}
+__device__ __forceinline__ int wave_max(int x) {
+  for (int m = 1; m < 64; m <<= 1) {
+    const int y = __shfl_xor(x, m);
+    x = x > y ? x : y;
+  }
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+struct Sequence {
+  int first, n, kv;  // first token, tokens, keys
+};
+// (offsets that run backwards or beyond the tokens, and lengths beyond the page table, are cut)
+__device__ __forceinline__ Sequence sequence_of(const ServeParams& p, int b) {
+  Sequence s = {0, 0, 0};
+  if (b < p.B) {
+    int from = p.cu[b], to = p.cu[b + 1];
+    from = from < 0 ? 0 : (from > p.T ? p.T : from);
+    to = to < from ? from : (to > p.T ? p.T : to);
+    s.first = from;
+    s.n = to - from;
+    s.kv = s.n;
+    if (p.kv_lens != nullptr) {
+      const int64_t most = int64_t(p.max_pages) << p.page_shift;
+      const int kv = p.kv_lens[b];
+      s.kv = kv < 0 ? 0 : (kv > most ? int(most) : kv);
+    }
+  }
+  return s;
+}
+template <int M>
+__device__ __forceinline__ int tiles_of(const ServeParams& p, const Sequence& s) {
+  return int((uint32_t(s.n) * uint32_t(p.G) + uint32_t(M - 1)) / uint32_t(M));
+}
+__device__ __forceinline__ int steps_of(int keys) { return (keys + kStepKeys - 1) / kStepKeys; }
+
+// Steps of a part: the batch's steps over the units they are shared by (the same number in every wave of both
+// kernels: the same sums in the same order), at least two.
+template <int M>
+__device__ __forceinline__ int part_steps(const ServeParams& p, int lane) {
+  float all = 0.f;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const Sequence s = sequence_of(p, b0 + lane);
+    all += wave_sum(float(tiles_of<M>(p, s)) * float(steps_of(s.kv)));
+  }
+  const float steps = ceilf(all / p.share);
+  const int part = steps < 1e9f ? int(steps) : 1000000000;
+  return __builtin_amdgcn_readfirstlane(part < 2 ? 2 : part);
+}
+__device__ __forceinline__ int parts_of(int kv, int part) {
+  const int steps = steps_of(kv);
+  return steps <= part ? 1 : (steps + part - 1) / part;
+}
+
+struct Unit {
+  Sequence seq;
+  int b, tile;
+  int step0, steps;  // range of steps (all that the tile has may be fewer)
+  bool part;         // one of several: its sums are joined later
+  bool found;
+};
+__device__ __forceinline__ Sequence pick(const Sequence& s, int lane) {
+  return {__builtin_amdgcn_readlane(s.first, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.kv, lane)};
+}
+
+// Unit number `rank` of tiles that are shared by parts: sequences in order, tiles in order, parts in order.
+template <int M>
+__device__ __forceinline__ Unit find_part(const ServeParams& p, int rank, int lane) {
+  const int part = part_steps<M>(p, lane);
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const Sequence s = sequence_of(p, b0 + lane);
+    const int tiles = tiles_of<M>(p, s), parts = parts_of(s.kv, part);
+    const int end = wave_scan(tiles * parts);
+    const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
+    if (beyond != 0) {
+      const int at = __builtin_ctzll(beyond);
+      Unit u;
+      u.seq = pick(s, at);
+      u.b = b0 + at;
+      const int n = __builtin_amdgcn_readlane(parts, at);
+      const int in = rank - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(tiles, at) * n);
+      u.tile = int(uint32_t(in) / uint32_t(n));
+      u.step0 = (in - u.tile * n) * part;
+      u.steps = part;
+      u.part = n > 1;
+      u.found = true;
+      return u;
+    }
+    rank -= __builtin_amdgcn_readlane(end, 63);
+  }
+  return Unit{{}, 0, 0, 0, 0, false, false};
+}
+
+// Unit number `rank` of whole tiles, those with most steps first: a launch then ends with short ones.  Steps are
+// compared in sixteen levels, which four rounds of counting find.
+template <int M>
+__device__ __forceinline__ Unit find_tile(const ServeParams& p, int rank, int lane) {
+  constexpr int kLog = M == 128 ? 7 : 5;
+  static_assert(M == 1 << kLog, "rows of a tile");
+  Unit u{{}, 0, 0, 0, 0x7fffffff, false, false};
+  int most = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const Sequence s = sequence_of(p, b0 + lane);
+    most = wave_max(s.n > 0 && steps_of(s.kv) > most ? steps_of(s.kv) : most);
+  }
+  int unit = 0;  // log2 of the steps of a level
+  while ((most >> unit) > 15) ++unit;
+  // tiles of a sequence with at least `steps` steps (its last ones)
+  auto long_tiles = [&](const Sequence& s, int steps) {
+    const int tiles = tiles_of<M>(p, s);
+    if (steps <= 0) return tiles;
+    if (!p.causal) return steps_of(s.kv) >= steps ? tiles : 0;
+    const int64_t token = int64_t(kStepKeys) * (steps - 1) - (s.kv - s.n);  // first token whose keys reach so far
+    if (token >= s.n) return 0;
+    return token <= 0 ? tiles : tiles - int((token * p.G) >> kLog);
+  };
+  auto count = [&](int level) {
+    int n = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) n += wave_sum(long_tiles(sequence_of(p, b0 + lane), level << unit));
+    return n;
+  };
+  const int all = count(0);
+  if (all <= rank) {
+    u.step0 = all;  // (what the caller needs to know where no unit is left)
+    return u;
+  }
+  int level = 0;
+  for (int bit = 8; bit != 0; bit >>= 1)
+    if (count(level | bit) > rank) level |= bit;
+  rank -= level == 15 ? 0 : count(level + 1);
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const Sequence s = sequence_of(p, b0 + lane);
+    const int from = long_tiles(s, level << unit);
+    const int mine = from - (level == 15 ? 0 : long_tiles(s, (level + 1) << unit));
+    const int end = wave_scan(mine);
+    const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
+    if (beyond != 0) {
+      const int at = __builtin_ctzll(beyond);
+      u.seq = pick(s, at);
+      u.b = b0 + at;
+      const int in = rank - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(mine, at));
+      u.tile = tiles_of<M>(p, u.seq) - __builtin_amdgcn_readlane(from, at) + __builtin_amdgcn_readlane(mine, at) - 1 - in;
+      u.found = true;
+      return u;
+    }
+    rank -= __builtin_amdgcn_readlane(end, 63);
+  }
+  return u;
+}
+
+// Workgroup -> (key head, rank).  Ids go round-robin over the XCDs: the heads are dealt to the XCDs, so that the
+// tiles that read one head's keys share an L2.
+__device__ __forceinline__ void deal_head(const ServeParams& p, int id, int& head, int& rank) {
+  const int X = p.n_xcd;
+  if (p.Hk % X == 0) {
+    const int per = p.Hk / X, xcd = id % X, slot = id / X;
+    head = xcd * per + slot % per;
+    rank = slot / per;
+  } else if (X % p.Hk == 0) {
+    const int per = X / p.Hk, xcd = id % X;
+    head = xcd % p.Hk;
+    rank = id / X * per + xcd / p.Hk;
+  } else {
+    rank = int(divide(uint32_t(id), p.heads));
+    head = id - rank * p.Hk;
+  }
+}
+
+// Rows of tokens behind the last sequence are zeros: their workgroups are those without a unit, the first of which is
+// number `units`.
+template <int D>
+__device__ void clear_rows(const ServeParams& p, int head, int rank, int units, int ranks, int tid, int threads) {
+  int used = p.cu[p.B];
+  used = used < 0 ? 0 : used;
+  for (int64_t t = int64_t(used) + (rank - units); t < p.T; t += ranks - units) {
+    const int64_t row = (t * p.Hk + head) * p.G;
+    for (int i = tid; i < p.G * (D / 8); i += threads) *reinterpret_cast<u32x4_t*>(p.o + row * D + i * 8) = u32x4_t{0u, 0u, 0u, 0u};
+    if (p.lse != nullptr)
+      for (int i = tid; i < p.G; i += threads) p.lse[row + i] = -INFINITY;
+  }
+}
+
+// Keys or values of one head of one sequence: resources of the rows from `row` on that end with the sequence, so that
+// rows behind it arrive as zeros whatever lies there.
+struct PackedRows {
+  const uint16_t* base;
+  uint32_t pitch;  // bytes from row to row
+  int kv;
+  template <int D>
+  __device__ __forceinline__ i32x4_t rows(int row) const {
+    const int left = kv - row;
+    const uint64_t bytes = left > 0 ? uint64_t(left - 1) * pitch + uint64_t(D * 2) : 0u;
+    return make_buffer_resource(reinterpret_cast<const uint8_t*>(base) + int64_t(row) * pitch,
+                                bytes > 0xffffffffu ? 0xffffffffu : uint32_t(bytes));
+  }
+};
+
+// The page numbers of a sequence, 64 at a time in the lanes of a wave.
+struct PageWindow {
+  int32_t pages;  // of the entries 64 * at .. 64 * at + 63
+  int at;
+  __device__ __forceinline__ void load(const ServeParams& p, int b, int window, int lane) {
+    at = window;
+    const int64_t i = int64_t(window) * 64 + lane;
+    int32_t page = i < p.max_pages ? p.page_table[int64_t(b) * p.max_pages + i] : 0;
+    page = page < 0 ? 0 : (page >= p.num_pages ? p.num_pages - 1 : page);  // (never a fault)
+    pages = page;
+  }
+};
+
+// O of a lane's row over the steps of a unit, and what its softmax needs.
+template <int DT>
+struct RowSums {
+  f32x16_t ot[DT];
+  float m_run, l_run;
+};
+
+// Weights of one step for a tile of 32 rows, written for a wave that has the step's scores of a row in a lane pair.
+template <int NTL>
+__device__ __forceinline__ void cap_scores(f32x16_t (&st)[NTL], float cap, float c2) {
+  static_for<16 * NTL>([&](auto ec) {
+    constexpr int e = decltype(ec)::value;
+    const float ex = __builtin_amdgcn_exp2f(st[e / 16][e % 16] * c2);
+    st[e / 16][e % 16] = __builtin_fmaf(__builtin_amdgcn_rcpf(ex + 1.f), -2.f * cap, cap);
+  });
+}
+// Scores of keys behind `limit` (the row's last key, counted from the step's first) become -inf.  Register r of tile t
+// holds key 32 t + 8 (r / 4) + 4 g + r % 4.
+template <int NTL>
+__device__ __forceinline__ void mask_scores(f32x16_t (&st)[NTL], int limit, int g) {
+  static_for<16 * NTL>([&](auto ec) {
+    constexpr int e = decltype(ec)::value, t = e / 16, r = e % 16;
+    constexpr int key = 32 * t + 8 * (r >> 2) + (r & 3);
+    if (key + 4 * g > limit) st[t][r] = -INFINITY;
+  });
+}
+template <int NTL>
+__device__ __forceinline__ float max_of(const f32x16_t (&st)[NTL], float sl2) {
+  float a = vmax(st[0][0], st[0][1]), b = vmax(st[0][2], st[0][3]);
+  static_for<8 * NTL - 2>([&](auto ic) {
+    constexpr int e = 2 * decltype(ic)::value + 4;
+    float& m = e & 2 ? b : a;
+    m = vmax3(m, st[e / 16][e % 16], st[e / 16][e % 16 + 1]);
+  });
+  return pair_max(vmax(a, b)) * sl2;
+}
+
+// Where a unit's results go.
+template <bool BF16, int D, int M>
+__device__ __forceinline__ void store_rows(const ServeParams& p, const Unit& u, int head, int slot, int row0, int rows_all,
+                                           f32x16_t (&ot)[D / 32], float m_run, float l_run, uint16_t* stage, int lane) {
+  // row0: first row of the wave in the sequence; slot: number of the unit
+  const int c = lane & 31, g = lane >> 5;
+  const float l = pair_sum(l_run);
+  if (u.part) {
+    const int in_tile = (row0 & (M - 1)) + c;
+    if (row0 + c < rows_all) {
+      float* at = p.sums + ((int64_t(slot) * p.Hk + head) * M + in_tile) * D;
+      typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4)
+          *reinterpret_cast<f32x4_t*>(at + 32 * dt + 8 * r4 + 4 * g) =
+              f32x4_t{ot[dt][4 * r4], ot[dt][4 * r4 + 1], ot[dt][4 * r4 + 2], ot[dt][4 * r4 + 3]};
+      if (g == 0) {
+        float* st = p.stats + ((int64_t(slot) * p.Hk + head) * M + in_tile) * 2;
+        st[0] = m_run;
+        st[1] = l;
+      }
+    }
+    return;
+  }
+  const bool live = l > 0.f || l != l;  // (sums that are no number stay so)
+  const float inv = live ? 1.f / l : 0.f;
+  // whole rows through LDS, so that a store instruction writes whole lines
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      u32x2_t ov;
+      ov[0] = pack2<BF16>(live ? ot[dt][4 * r4 + 0] * inv : 0.f, live ? ot[dt][4 * r4 + 1] * inv : 0.f);
+      ov[1] = pack2<BF16>(live ? ot[dt][4 * r4 + 2] * inv : 0.f, live ? ot[dt][4 * r4 + 3] * inv : 0.f);
+      *reinterpret_cast<u32x2_t*>(stage + c * D + ((4 * dt + r4) ^ k_swizzle<D>(c)) * 8 + 4 * g) = ov;
+    }
+  constexpr int CPR = D / 8, RPS = 64 / CPR;
+  const int pch = lane % CPR;
+#pragma unroll
+  for (int i = 0; i < 32 / RPS; ++i) {
+    const int row = i * RPS + lane / CPR;
+    const u32x4_t val = *reinterpret_cast<const u32x4_t*>(stage + row * D + pch * 8);
+    const int r = row0 + row;
+    if (r < rows_all) {
+      const int token = int(divide(uint32_t(r), p.group));
+      const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (r - token * p.G);
+      *reinterpret_cast<u32x4_t*>(p.o + at * D + (pch ^ k_swizzle<D>(row)) * 8) = val;
+    }
+  }
+  if (p.lse != nullptr && g == 0 && row0 + c < rows_all) {
+    const int token = int(divide(uint32_t(row0 + c), p.group));
+    p.lse[(int64_t(u.seq.first + token) * p.Hk + head) * p.G + (row0 + c - token * p.G)] =
+        live ? (m_run + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+  }
+}
+
+// ---- few rows: one wave per unit ---------------------------------------------------------------------------------
+//
+// Single tokens, and a few.  The work is the reading of K and V: a unit is one wave of its own with two sets of
+// K and V tiles in LDS that direct loads fill a step ahead; nothing waits for another wave.
+
+template <int D>
+constexpr int kFewStep = D == 128 ? 32 : 64;  // keys per step: 16 KiB of K and V
+template <int D>
+constexpr size_t kFewLdsBytes = size_t(2) * 2 * kFewStep<D> * D * 2;
+
+template <bool BF16, int D, bool PAGED>
+__global__ void __launch_bounds__(64) serve_few_kernel(const ServeParams p) {
+  constexpr int M = 32, STEP = kFewStep<D>, NTL = STEP / 32, KS = D / 16, DT = D / 32, CPR = D / 8;
+  constexpr int RPC = 64 / CPR, NCH = STEP / RPC, TILE = STEP * D;  // rows per load, loads per tile
+  constexpr int KPER = RPC % 16 == 0 ? 1 : 16 / RPC;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+  uint16_t* sK = reinterpret_cast<uint16_t*>(lds_raw);
+  uint16_t* sV = sK + 2 * TILE;
+  const int lane = threadIdx.x, g = lane >> 5, c = lane & 31;
+  int head, rank;
+  deal_head(p, blockIdx.x, head, rank);
+  if (rank >= p.units) return;
+  const Unit u = p.share > 0.f ? find_part<M>(p, rank, lane) : find_tile<M>(p, rank, lane);
+  if (!u.found) {  // (with parts the joining kernel clears rows behind the last sequence)
+    if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, lane, 64);
+    return;
+  }
+  const int rows_all = u.seq.n * p.G, row0 = u.tile * M;
+  const int row = row0 + c < rows_all ? row0 + c : rows_all - 1;
+  const int token = int(divide(uint32_t(row), p.group));
+  const int limit = p.causal ? u.seq.kv - u.seq.n + token : u.seq.kv - 1;  // the row's last key
+  const int last_row = row0 + M < rows_all ? row0 + M - 1 : rows_all - 1;
+  const int last_key = p.causal ? u.seq.kv - u.seq.n + int(divide(uint32_t(last_row), p.group)) : u.seq.kv - 1;
+  const int first_key = p.causal ? u.seq.kv - u.seq.n + int(divide(uint32_t(row0), p.group)) : u.seq.kv - 1;
+  const int from = u.step0 * kStepKeys;
+  int to = u.steps < steps_of(u.seq.kv) - u.step0 ? (u.step0 + u.steps) * kStepKeys : u.seq.kv;
+  if (to > last_key + 1) to = last_key + 1;  // (keys at or behind `to` are not read)
+  const int nsteps = to > from ? (to - from + STEP - 1) / STEP : 0;
+
+  u32x4_t qf[KS];
+  {
+    const uint16_t* at = p.q + int64_t(u.seq.first + token) * p.q_row + int64_t(head * p.G + (row - token * p.G)) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(at + 16 * s + 8 * g);
+  }
+
+  // Direct loads: instruction i of a tile fills the rows i * RPC .. i * RPC + RPC - 1.
+  const int ld_row = lane / CPR, ld_pch = lane % CPR;
+  PackedRows kr, vr;
+  PageWindow window{0, -1};
+  uint32_t kpitch = D * 2, vpitch = D * 2;
+  if constexpr (!PAGED) {
+    kr = {p.k + int64_t(u.seq.first) * p.k_at.row + head * p.k_at.h, p.k_at.row * 2u, to};
+    vr = {p.v + int64_t(u.seq.first) * p.v_at.row + head * p.v_at.h, p.v_at.row * 2u, to};
+    kpitch = kr.pitch;
+    vpitch = vr.pitch;
+  }
+  uint32_t koff[KPER];
+#pragma unroll
+  for (int i = 0; i < KPER; ++i) koff[i] = uint32_t(ld_row) * kpitch + uint32_t(ld_pch ^ k_swizzle<D>(ld_row + i * RPC)) * 16u;
+  const uint32_t voff = uint32_t(ld_row) * vpitch + uint32_t((((ld_pch >> 1) ^ v_swizzle<D>(ld_row)) << 1) | (ld_pch & 1)) * 16u;
+  const uint32_t lds_k = lds_offset_of(sK), lds_v = lds_offset_of(sV);
+  auto issue = [&](int buf, int key0) {
+    if constexpr (PAGED) {
+      const int w = (key0 >> p.page_shift) >> 6;
+      if (w != window.at) {
+        window.load(p, u.b, w, lane);
+        wait_loads();
+      }
+    }
+    i32x4_t rk, rv;
+    if constexpr (!PAGED) {
+      rk = kr.rows<D>(key0);
+      rv = vr.rows<D>(key0);
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const uint32_t dst = uint32_t(buf) * (TILE * 2u) + uint32_t(i) * 1024u;
+      if constexpr (PAGED) {
+        const int key = key0 + i * RPC;
+        const int page = __builtin_amdgcn_readlane(window.pages, (key >> p.page_shift) & 63);
+        const int64_t at = (((int64_t(page) * p.Hk + head) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * D;
+        int left = to - key;
+        left = left < 0 ? 0 : (left > RPC ? RPC : left);
+        rk = make_buffer_resource(p.k + at, uint32_t(left) * (D * 2u));
+        rv = make_buffer_resource(p.v + at, uint32_t(left) * (D * 2u));
+        buffer_to_lds_b128(rk, koff[i % KPER], 0, lds_k + dst);
+        buffer_to_lds_b128(rv, voff, 0, lds_v + dst);
+      } else {
+        buffer_to_lds_b128(rk, koff[i % KPER], uint32_t(i * RPC) * kpitch, lds_k + dst);
+        buffer_to_lds_b128(rv, voff, uint32_t(i * RPC) * vpitch, lds_v + dst);
+      }
+    }
+  };
+
+  const f32x16_t zero16 = {};
+  f32x16_t ot[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) ot[dt] = zero16;
+  float m_run = -INFINITY, l_run = 0.f;
+  const int i16 = c & 15, j16 = c >> 4;
+  if (nsteps > 0) issue(0, from);
+  for (int it = 0; it < nsteps; ++it) {
+    const int key0 = from + it * STEP, buf = it & 1;
+    if (it + 1 < nsteps) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other set has been read
+      issue(buf ^ 1, key0 + STEP);
+      wait_loads_but<2 * NCH>();
+    } else {
+      wait_loads();
+    }
+    const uint16_t* tK = sK + buf * TILE;
+    const uint16_t* tV = sV + buf * TILE;
+    f32x16_t st[NTL];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int t = 0; t < NTL; ++t) {
+        const int r = 32 * t + c;
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(tK + r * D + ((2 * s + g) ^ k_swizzle<D>(r)) * 8);
+        st[t] = mfma_32x32x16<BF16>(a, qf[s], s == 0 ? zero16 : st[t]);
+      }
+    if (p.softcap > 0.f) cap_scores<NTL>(st, p.softcap, p.cap_c2);
+    if (key0 + STEP - 1 > first_key || key0 + STEP > to) {
+      const int stop = limit < to - 1 ? limit : to - 1;
+      mask_scores<NTL>(st, stop - key0, g);
+    }
+    const float m_new = fmaxf(m_run, max_of<NTL>(st, p.sl2));
+    if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
+      const float m_old = m_run == -INFINITY ? (m_new == -INFINITY ? 0.f : m_new) : m_run;
+      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_old - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ot[dt][r] *= alpha;
+      m_run = m_new;
+    }
+    const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+    u32x4_t pb[NTL][2];
+    static_for<8 * NTL>([&](auto ic) {
+      constexpr int i = decltype(ic)::value, t = i / 8, r = 2 * (i % 8);
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], p.sl2, -m_ref));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r + 1], p.sl2, -m_ref));
+      l_run += p0 + p1;
+      pb[t][r >> 3][(r & 7) >> 1] = pack2<BF16>(p0, p1);
+    });
+#pragma unroll
+    for (int j = 0; j < (STEP / 16) * DT; ++j) {
+      const int ts = j / DT, dt = j % DT;
+      const int vrow = 16 * ts + 4 * g + (i16 >> 2), unit = 2 * dt + j16;
+      const s16x4_t lo = lds_read_tr16(tV + vrow * D + (unit ^ v_swizzle<D>(vrow)) * 16 + (i16 & 3) * 4);
+      const s16x4_t hi = lds_read_tr16(tV + (vrow + 8) * D + (unit ^ v_swizzle<D>(vrow + 8)) * 16 + (i16 & 3) * 4);
+      const u32x2_t lo2 = __builtin_bit_cast(u32x2_t, lo), hi2 = __builtin_bit_cast(u32x2_t, hi);
+      ot[dt] = mfma_32x32x16<BF16>(u32x4_t{lo2[0], lo2[1], hi2[0], hi2[1]}, pb[ts >> 1][ts & 1], ot[dt]);
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, sK, lane);
+}
+
+// ---- many rows: four waves per unit -------------------------------------------------------------------------------
+//
+// A tile of 128 rows, 32 per wave, walks its keys in steps of 64, software-pipelined like the block-sparse forward:
+// iteration i issues the matrix instructions of S^T(i + 1) and of O^T += V^T P^T(i - 1) in slots, and between
+// them the softmax of step i, the operand fetches and the loads of K(i + 2) and V(i).  The exponentials' reference
+// stays where it is as long as the row sums do not outgrow it.
+
+template <int D>
+constexpr size_t kTileLdsBytes = size_t(2) * 2 * kStepKeys * D * 2;
+
+template <bool BF16, int D, bool PAGED>
+__global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p) {
+  constexpr int M = 128, STEP = kStepKeys, NTL = 2, KS = D / 16, DT = D / 32, CPR = D / 8, TILE = STEP * D;
+  constexpr int RPC = 64 / CPR;            // rows filled by a wave's load
+  constexpr int ROW_STRIDE = RPC * 4;      // rows between a thread's loads
+  constexpr int NCH = STEP / ROW_STRIDE;   // loads per thread and tile
+  constexpr int KPER = ROW_STRIDE % 16 == 0 ? 1 : 16 / ROW_STRIDE;
+  static_assert((KPER * ROW_STRIDE) % 16 == 0 && ROW_STRIDE % 4 == 0 && RPC <= 16, "swizzles repeat over a thread's loads");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+  uint16_t* sK = reinterpret_cast<uint16_t*>(lds_raw);  // [2][TILE]
+  uint16_t* sV = sK + 2 * TILE;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c = lane & 31;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int head, rank;
+  deal_head(p, blockIdx.x, head, rank);
+  if (rank >= p.units) return;
+  const Unit u = p.share > 0.f ? find_part<M>(p, rank, lane) : find_tile<M>(p, rank, lane);
+  if (!u.found) {
+    if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, tid, 256);
+    return;
+  }
+  const int shift = u.seq.kv - u.seq.n;  // a token's position, less its number
+  const int rows_all = u.seq.n * p.G, row0 = u.tile * M + 32 * w;
+  const int row = row0 + c < rows_all ? row0 + c : rows_all - 1;
+  const int token = int(divide(uint32_t(row), p.group));
+  const int last_row = u.tile * M + M < rows_all ? u.tile * M + M - 1 : rows_all - 1;
+  const int last_key = p.causal ? shift + int(divide(uint32_t(last_row), p.group)) : u.seq.kv - 1;
+  const int wave_first = row0 < rows_all ? row0 : rows_all - 1;
+  const int first_key = __builtin_amdgcn_readfirstlane(p.causal ? shift + int(divide(uint32_t(wave_first), p.group)) : u.seq.kv - 1);
+  const int from = u.step0 * STEP;
+  int to = u.steps < steps_of(u.seq.kv) - u.step0 ? (u.step0 + u.steps) * STEP : u.seq.kv;
+  if (to > last_key + 1) to = last_key + 1;  // (keys at or behind `to` are not read)
+  to = __builtin_amdgcn_readfirstlane(to);
+  const int nsteps = __builtin_amdgcn_readfirstlane(to > from ? (to - from + STEP - 1) / STEP : 0);
+
+  u32x4_t qf[KS];
+  {
+    const uint16_t* at = p.q + int64_t(u.seq.first + token) * p.q_row + int64_t(head * p.G + (row - token * p.G)) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(at + 16 * s + 8 * g);
+  }
+
+  const int ld_row = PAGED ? lane / CPR : tid / CPR, ld_pch = tid % CPR, sw_row = tid / CPR;
+  PackedRows kr, vr;
+  PageWindow kwin{0, -1}, vwin{0, -1};
+  uint32_t kpitch = D * 2, vpitch = D * 2;
+  if constexpr (!PAGED) {
+    kr = {p.k + int64_t(u.seq.first) * p.k_at.row + head * p.k_at.h, p.k_at.row * 2u, to};
+    vr = {p.v + int64_t(u.seq.first) * p.v_at.row + head * p.v_at.h, p.v_at.row * 2u, to};
+    kpitch = kr.pitch;
+    vpitch = vr.pitch;
+  }
+  uint32_t koff[KPER];
+#pragma unroll
+  for (int i = 0; i < KPER; ++i)
+    koff[i] = uint32_t(ld_row) * kpitch + uint32_t(ld_pch ^ k_swizzle<D>(sw_row + i * ROW_STRIDE)) * 16u;
+  const uint32_t voff = uint32_t(ld_row) * vpitch + uint32_t((((ld_pch >> 1) ^ v_swizzle<D>(sw_row)) << 1) | (ld_pch & 1)) * 16u;
+  const uint32_t lds_k0 = lds_offset_of(sK) + uint32_t(w) * 1024u, lds_v0 = lds_offset_of(sV) + uint32_t(w) * 1024u;
+  // Before the loads of a step's K, or V: its window of page numbers.
+  auto need_window = [&](PageWindow& win, const PageWindow& other, int key0) {
+    if constexpr (PAGED) {
+      const int n = (key0 >> p.page_shift) >> 6;
+      if (n != win.at) {
+        if (n == other.at) {
+          win = other;
+        } else {
+          win.load(p, u.b, n, lane);
+        }
+      }
+    }
+  };
+  // Load n of a tile pair: n < NCH part n of V, else of K.  rk, rv: (packed) the rows from the step's first on.
+  auto issue_load = [&](int n, int buf, int k_key0, int v_key0, const i32x4_t& rk, const i32x4_t& rv) {
+    const bool is_v = n < NCH;
+    const int i = is_v ? n : n - NCH;
+    const uint32_t dst = (is_v ? lds_v0 : lds_k0) + uint32_t(buf) * (TILE * 2u) + uint32_t(i) * 4096u;
+    const uint32_t off = is_v ? voff : koff[i % KPER];
+    if constexpr (PAGED) {
+      const int key = (is_v ? v_key0 : k_key0) + i * ROW_STRIDE + w * RPC;
+      const int page = __builtin_amdgcn_readlane(is_v ? vwin.pages : kwin.pages, (key >> p.page_shift) & 63);
+      const int64_t at = (((int64_t(page) * p.Hk + head) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * D;
+      int left = to - key;
+      left = left < 0 ? 0 : (left > RPC ? RPC : left);
+      buffer_to_lds_b128(make_buffer_resource((is_v ? p.v : p.k) + at, uint32_t(left) * (D * 2u)), off, 0, dst);
+    } else {
+      buffer_to_lds_b128(is_v ? rv : rk, off, uint32_t(i * ROW_STRIDE) * (is_v ? vpitch : kpitch), dst);
+    }
+  };
+  auto rows_of = [&](const PackedRows& r, int key0) {
+    if constexpr (PAGED) {
+      return i32x4_t{};
+    } else {
+      return r.template rows<D>(key0);
+    }
+  };
+
+  auto k_frag = [&](const uint16_t* tK, int s, int t) {
+    const int r = 32 * t + c;
+    return *reinterpret_cast<const u32x4_t*>(tK + r * D + ((2 * s + g) ^ k_swizzle<D>(r)) * 8);
+  };
+  const int i16 = c & 15, j16 = c >> 4;
+  auto v_frag = [&](const uint16_t* tV, int j) {
+    const int ts = j / DT, dt = j % DT;
+    const int vrow = 16 * ts + 4 * g + (i16 >> 2), unit = 2 * dt + j16;
+    const s16x4_t lo = lds_read_tr16(tV + vrow * D + (unit ^ v_swizzle<D>(vrow)) * 16 + (i16 & 3) * 4);
+    const s16x4_t hi = lds_read_tr16(tV + (vrow + 8) * D + (unit ^ v_swizzle<D>(vrow + 8)) * 16 + (i16 & 3) * 4);
+    const u32x2_t lo2 = __builtin_bit_cast(u32x2_t, lo), hi2 = __builtin_bit_cast(u32x2_t, hi);
+    return u32x4_t{lo2[0], lo2[1], hi2[0], hi2[1]};
+  };
+
+  const f32x16_t zero16 = {};
+  f32x16_t ot[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) ot[dt] = zero16;
+  f32x16_t st[2][NTL];
+  u32x4_t pb[2][NTL][2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int t = 0; t < NTL; ++t) {
+      st[a][t] = zero16;
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) pb[a][t][s2] = u32x4_t{0u, 0u, 0u, 0u};
+    }
+  float m_run = -INFINITY, m_ref = 0.f, l_run = 0.f, alpha_pending = 1.f;
+  constexpr uint32_t kOwesRescale = 1, kOwesLook = 2;
+  uint32_t owed = kOwesLook;
+  constexpr int NQK = NTL * KS, NPV_ALL = (STEP / 16) * DT, NL = 2 * NCH, PF = 3;
+  // (as in the block-sparse forward: how far a row may outgrow its reference before the next look, and before the
+  // step itself is done again)
+  constexpr float kSlack = 6.f, kGrown = 0x1p10f, kRedo = 0x1p13f;
+
+  auto weights = [&](auto set_c, auto ic, float& s0, float& s1) {
+    constexpr int SET = decltype(set_c)::value, i = decltype(ic)::value, t = i / 8, r = 2 * (i % 8);
+    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[SET][t][r], p.sl2, -m_ref));
+    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[SET][t][r + 1], p.sl2, -m_ref));
+    if constexpr (i == 0) {
+      s0 = p0;
+      s1 = p1;
+    } else {
+      s0 += p0;
+      s1 += p1;
+    }
+    uint32_t packed = pack2<BF16>(p0, p1);
+    pin(packed);
+    pb[SET][t][r >> 3][(r & 7) >> 1] = packed;
+    pin(s0, s1);
+  };
+  auto set_reference = [&](float m_new) {
+    m_ref = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
+    l_run *= alpha;
+    m_run = m_new;
+    return alpha;
+  };
+  auto look_again = [&]() { return __builtin_amdgcn_ballot_w64(m_run == -INFINITY) != 0 ? kOwesLook : 0u; };
+  auto look = [&](auto set_c) {
+    constexpr int SET = decltype(set_c)::value;
+    const float m_cand = max_of<NTL>(st[SET], p.sl2);
+    owed = 0;
+    if (__builtin_amdgcn_ballot_w64(m_cand > m_run + kSlack) != 0) {
+      alpha_pending = set_reference(vmax(m_run, m_cand));
+      owed = kOwesRescale;
+    }
+    owed |= look_again();
+  };
+  auto redo = [&](auto set_c, float& sum) {
+    constexpr int SET = decltype(set_c)::value;
+    const float alpha = set_reference(vmax(m_run, max_of<NTL>(st[SET], p.sl2)));
+    alpha_pending = owed & kOwesRescale ? alpha_pending * alpha : alpha;
+    float s0, s1;
+    static_for<8 * NTL>([&](auto ic) { weights(set_c, ic, s0, s1); });
+    sum = s0 + s1;
+    owed = kOwesRescale | look_again();
+  };
+  auto rescale = [&]() {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ot[dt][r] *= alpha_pending;
+    owed &= ~kOwesRescale;
+  };
+
+  auto body_prefetch = [&](auto set_c, auto first_c, u32x4_t* opq) {
+    constexpr int SET = decltype(set_c)::value, NPV = decltype(first_c)::value != 0 ? 0 : NPV_ALL;
+    const uint16_t* tK = sK + (SET ^ 1) * TILE;
+    const uint16_t* tV = sV + (SET ^ 1) * TILE;
+    static_for<PF>([&](auto nc) {
+      constexpr int n = decltype(nc)::value;
+      opq[n] = n < NPV ? v_frag(tV, n) : k_frag(tK, (n - NPV) / NTL, (n - NPV) % NTL);
+    });
+  };
+  auto body = [&](auto set_c, auto first_c, int k_key0, int v_key0, u32x4_t* opq) {
+    constexpr int SET = decltype(set_c)::value, NPV = decltype(first_c)::value != 0 ? 0 : NPV_ALL;
+    constexpr int NS = NQK + NPV;
+    constexpr int LSP = (NS / 2) / NL > 0 ? (NS / 2) / NL : 1;
+    constexpr int LPS = (NL * LSP + NS - 1) / NS;
+    constexpr int NPR = 8 * NTL;
+    const uint16_t* tK = sK + (SET ^ 1) * TILE;
+    const uint16_t* tV = sV + (SET ^ 1) * TILE;
+    const i32x4_t rk = rows_of(kr, k_key0), rv = rows_of(vr, v_key0);
+    float rs0, rs1;
+    __builtin_amdgcn_s_setprio(1);
+    static_for<NS>([&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      if constexpr (j < NPV) {
+        constexpr int ts = j / DT, dt = j % DT;
+        ot[dt] = mfma_32x32x16<BF16>(opq[j % PF], pb[SET ^ 1][ts >> 1][ts & 1], ot[dt]);
+      } else {
+        constexpr int s = (j - NPV) / NTL, t = (j - NPV) % NTL;
+        st[SET ^ 1][t] = mfma_32x32x16<BF16>(opq[j % PF], qf[s], s == 0 ? zero16 : st[SET ^ 1][t]);
+      }
+      if constexpr (j + PF < NS) {
+        constexpr int n = j + PF;
+        if constexpr (n < NPV) {
+          opq[j % PF] = v_frag(tV, n);
+        } else {
+          opq[j % PF] = k_frag(tK, (n - NPV) / NTL, (n - NPV) % NTL);
+        }
+      }
+      static_for<LPS>([&](auto lc) {
+        constexpr int n = (j / LSP) * LPS + decltype(lc)::value;
+        if constexpr (j % LSP == 0 && n < NL) issue_load(n, SET, k_key0, v_key0, rk, rv);
+      });
+      constexpr int i_lo = j * NPR / NS, i_hi = (j + 1) * NPR / NS;
+      static_for<i_hi - i_lo>([&](auto dc) { weights(set_c, IntC<i_lo + decltype(dc)::value>{}, rs0, rs1); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_setprio(0);
+    return rs0 + rs1;
+  };
+
+  // Steps behind the last one: loads whose rows all lie behind `to` and arrive as zeros.
+  auto iteration = [&](auto set_c, auto first_c, int it) {
+    constexpr int SET = decltype(set_c)::value;
+    const int key0 = from + it * STEP;
+    wait_loads();
+    __syncthreads();
+    u32x4_t opq[PF];
+    body_prefetch(set_c, first_c, opq);
+    const bool whole = key0 + STEP - 1 <= first_key && key0 + STEP <= to;
+    if ((owed != 0) | (p.softcap > 0.f) | !whole) {
+      if (owed & kOwesRescale) rescale();
+      if (p.softcap > 0.f) cap_scores<NTL>(st[SET], p.softcap, p.cap_c2);
+      if (!whole) {
+        int l = lane;  // (the row's last key is worked out here, not kept in a register over the walk)
+        asm volatile("" : "+v"(l));
+        int limit = to - 1;
+        if (p.causal) {
+          const int r = row0 + (l & 31) < rows_all ? row0 + (l & 31) : rows_all - 1;
+          const int last = shift + int(divide(uint32_t(r), p.group));
+          limit = last < limit ? last : limit;
+        }
+        mask_scores<NTL>(st[SET], limit - key0, l >> 5);
+      }
+      if (owed & kOwesLook) look(set_c);
+    }
+    need_window(vwin, kwin, key0);
+    need_window(kwin, vwin, key0 + 2 * STEP);
+    float sum = body(set_c, first_c, key0 + 2 * STEP, key0, opq);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= kGrown)) != 0, 0)) {
+      owed |= kOwesLook;
+      if (__builtin_amdgcn_ballot_w64(!(sum <= kRedo)) != 0) redo(set_c, sum);
+    }
+    l_run += sum;
+  };
+  if (nsteps > 0) {
+    need_window(kwin, kwin, from);
+    {
+      const i32x4_t r0 = rows_of(kr, from);
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 0, from, 0, r0, r0);
+    }
+    need_window(kwin, kwin, from + STEP);
+    {
+      const i32x4_t r1 = rows_of(kr, from + STEP);
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 1, from + STEP, 0, r1, r1);
+    }
+    wait_loads();
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int t = 0; t < NTL; ++t) st[0][t] = mfma_32x32x16<BF16>(k_frag(sK, s, t), qf[s], s == 0 ? zero16 : st[0][t]);
+    // (the first iteration's loads overwrite the tile that has just been read: its barrier comes first)
+    iteration(IntC<0>{}, IntC<1>{}, 0);
+    if (1 < nsteps) iteration(IntC<1>{}, IntC<0>{}, 1);
+    for (int it = 2; it < nsteps; it += 2) {
+      iteration(IntC<0>{}, IntC<0>{}, it);
+      if (it + 1 < nsteps) iteration(IntC<1>{}, IntC<0>{}, it + 1);
+    }
+    wait_loads();
+    __syncthreads();
+    if (owed & kOwesRescale) rescale();
+    auto drain = [&](auto set_c) {
+      constexpr int SET = decltype(set_c)::value;
+#pragma unroll
+      for (int j = 0; j < NPV_ALL; ++j) {
+        const int ts = j / DT, dt = j % DT;
+        ot[dt] = mfma_32x32x16<BF16>(v_frag(sV + SET * TILE, j), pb[SET][ts >> 1][ts & 1], ot[dt]);
+      }
+    };
+    if ((nsteps - 1) & 1) {
+      drain(IntC<1>{});
+    } else {
+      drain(IntC<0>{});
+    }
+  }
+  // (the K tiles are read by nobody any more: a wave stages its rows in a quarter of them)
+  store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, sK + w * 32 * D, lane);
+}
+
+// Joins the parts of a row: a wave per token and query head.  Clears the rows behind the last sequence too.
+template <bool BF16, int D, int M>
+__global__ void __launch_bounds__(256) serve_join_kernel(const ServeParams p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int Hq = p.Hk * p.G;
+  const int64_t t64 = id / Hq;
+  if (t64 >= p.T) return;
+  const int t = int(t64), h = int(id - t64 * Hq), head = int(divide(uint32_t(h), p.group));
+  const int part = part_steps<M>(p, lane);
+  int before = 0;
+  Unit u{{}, 0, 0, 0, 0, false, false};
+  for (int b0 = 0; b0 < p.B && !u.found; b0 += 64) {
+    const Sequence s = sequence_of(p, b0 + lane);
+    const int units = tiles_of<M>(p, s) * parts_of(s.kv, part);
+    const int end = wave_scan(units);
+    const uint64_t here = __builtin_amdgcn_ballot_w64(t >= s.first && t < s.first + s.n);
+    if (here != 0) {
+      const int at = __builtin_ctzll(here);
+      u.seq = pick(s, at);
+      u.found = true;
+      before += __builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(units, at);
+    } else {
+      before += __builtin_amdgcn_readlane(end, 63);
+    }
+  }
+  uint16_t* out = p.o + id * D;
+  if (!u.found) {
+    for (int d = lane; d < D; d += 64) out[d] = 0;
+    if (p.lse != nullptr && lane == 0) p.lse[id] = -INFINITY;
+    return;
+  }
+  const int parts = parts_of(u.seq.kv, part);
+  if (parts == 1) return;  // written where it was computed
+  const int row = (t - u.seq.first) * p.G + (h - head * p.G);
+  const int64_t slot = before + int64_t(row / M) * parts;
+  const int64_t at = (slot * p.Hk + head) * M + row % M, step = int64_t(p.Hk) * M;
+  float m = -INFINITY;
+  for (int i = lane; i < parts; i += 64) m = fmaxf(m, p.stats[(at + i * step) * 2]);
+  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+  const float m_ref = m == -INFINITY ? 0.f : m;
+  constexpr int N = D >= 64 ? D / 64 : 1;  // neighbouring dimensions of a lane
+  const int d = lane * N;
+  float sum[N] = {}, l = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const float* st = p.stats + (at + i * step) * 2;
+    const float w = __builtin_amdgcn_exp2f(st[0] - m_ref);
+    l += st[1] * w;
+    if (d < D) {
+      const float* x = p.sums + (at + i * step) * D + d;
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum[j] = __builtin_fmaf(x[j], w, sum[j]);
+    }
+  }
+  const bool live = l > 0.f || l != l;
+  const float inv = live ? 1.f / l : 0.f;
+  if (d < D) {
+    if constexpr (N == 2) {
+      *reinterpret_cast<uint32_t*>(out + d) = live ? pack2<BF16>(sum[0] * inv, sum[1] * inv) : 0u;
+    } else {
+      out[d] = live ? uint16_t(pack2<BF16>(sum[0] * inv, 0.f)) : uint16_t(0);
+    }
+  }
+  if (p.lse != nullptr && lane == 0) p.lse[id] = live ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+}  // namespace omni_attn

@@ -33,6 +33,14 @@ EXPORTED_SYMBOLS = (
     "omni_attn_bwd_workspace_bytes",
     "omni_attn_bwd_noalloc_gfx950",
     "omni_attn_bwd_noalloc_max_rows",
+    "omni_attn_qk_rotary_gfx950",
+    "omni_attn_qk_rotary_bwd_workspace_bytes",
+    "omni_attn_qk_rotary_bwd_gfx950",
+    "omni_attn_cache_append_gfx950",
+    "omni_attn_packed_workspace_bytes",
+    "omni_attn_packed_gfx950",
+    "omni_attn_paged_workspace_bytes",
+    "omni_attn_paged_gfx950",
     "omni_attn_mfma_peak_probe_gfx950",
     "omni_attn_status_string",
     "omni_attn_last_hip_error",

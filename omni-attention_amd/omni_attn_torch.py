@@ -788,6 +788,124 @@ def omni_attention(query: Tensor, key: Tensor, value: Tensor, block_mask: OmniBl
 
 
 # ----------------------------------------------------------------------------
+# Rotation, and sequences of different lengths: packed prompts and a paged cache
+# (not in the reference, whose operator takes one padded batch of rotated heads)
+# ----------------------------------------------------------------------------
+
+def omni_rotary_table(rotary_dim: int, max_positions: int, theta: float = 10000.0, scaling: Optional[str] = None,
+                      factor: float = 1.0, original_positions: Optional[int] = None, beta_fast: float = 32.0,
+                      beta_slow: float = 1.0, device: Union[str, torch.device] = "cuda") -> Tensor:
+    """Cosines, then sines, of ``position * theta ** (-2 i / rotary_dim)``: fp32 [max_positions, rotary_dim], made once
+    per model.  Angles are worked out in 64 bits: far positions keep theirs.
+
+    ``scaling`` stretches a model that was trained on ``original_positions`` to ``factor`` times as many:
+      "linear"  every angle divided by ``factor``
+      "ntk"     theta raised so that the slowest angle is divided by ``factor`` and the fastest stays
+      "yarn"    angles that turn more than ``beta_fast`` times over ``original_positions`` stay, those that turn less
+                than ``beta_slow`` times are divided by ``factor``, with a ramp between; cosines and sines are
+                multiplied by ``0.1 ln(factor) + 1``
+    """
+    if rotary_dim < 2 or rotary_dim % 2 != 0 or max_positions < 1:
+        raise ValueError("rotary_dim must be even and positive, max_positions positive")
+    if not theta > 1.0 or not factor >= 1.0 or math.isinf(theta) or math.isinf(factor):
+        raise ValueError("theta must be greater than 1, factor at least 1")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"Unsupported scaling={scaling!r}. Supported values: None, 'linear', 'ntk', 'yarn'.")
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("scaling='ntk' needs rotary_dim of at least 4")
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    pair = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim
+    turn = theta ** -pair
+    magnitude = 1.0
+    if scaling == "linear":
+        turn = turn / factor
+    elif scaling == "yarn":
+        if original_positions is None or original_positions < 1 or not beta_fast > beta_slow > 0:
+            raise ValueError("scaling='yarn' needs original_positions and beta_fast > beta_slow > 0")
+        # the pair that turns `times` times over the original positions
+        at = lambda times: rotary_dim * math.log(original_positions / (times * 2 * math.pi)) / (2 * math.log(theta))
+        low = max(math.floor(at(beta_fast)), 0)
+        high = min(math.ceil(at(beta_slow)), rotary_dim - 1)
+        index = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
+        slow = ((index - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+        turn = turn / factor * slow + turn * (1.0 - slow)
+        magnitude = 0.1 * math.log(factor) + 1.0
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device).unsqueeze(1) * turn
+    return torch.cat([angle.cos() * magnitude, angle.sin() * magnitude], dim=1).to(torch.float32).contiguous()
+
+
+def omni_qk_rotary(query: Tensor, key: Tensor, positions: Tensor, table: Tensor, query_norm: Optional[Tensor] = None,
+                   key_norm: Optional[Tensor] = None, eps: float = 1e-6,
+                   interleaved: bool = False) -> Tuple[Tensor, Tensor]:
+    """Query and key heads normed by their root mean square (with weights ``query_norm``, ``key_norm`` [head_dim], where
+    given) and rotated by their positions, in one pass; differentiable in query, key and the weights.
+
+    query, key   [B, H, S, head_dim] or packed [tokens, H, head_dim], fp16 / bf16, each with its own number of heads; any
+                 strides (rows that are not multiples of 4 elements apart are copied).  head_dim: multiples of 8 up to 256
+    positions    rows of ``table``: [S] or [B, S] (packed: [tokens]), int32 or int64; the tokens of an image may share
+                 one.  Positions outside the table read its first or last row
+    table        omni_rotary_table(rotary_dim, ...); rotary_dim a multiple of 8 up to head_dim, the dimensions behind
+                 it are normed and not rotated
+    interleaved  pairs are (2i, 2i + 1); else (i, i + rotary_dim / 2)
+
+    The results lie in memory as the operands do, so a projection's [B, S, H, D] seen as [B, H, S, D] goes into
+    ``omni_attention`` without a copy."""
+    return _load_extension().omni_attn_qk_rotary(query, key, positions, table, query_norm, key_norm, float(eps),
+                                                 bool(interleaved))
+
+
+def omni_cache_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Tensor, page_table: Tensor,
+                      kv_lens: Tensor, cu_seqlens: Tensor, table: Optional[Tensor] = None,
+                      positions: Optional[Tensor] = None, query: Optional[Tensor] = None,
+                      query_norm: Optional[Tensor] = None, key_norm: Optional[Tensor] = None, eps: float = 1e-6,
+                      interleaved: bool = False) -> Optional[Tensor]:
+    """New tokens of a batch of sequences enter a paged cache: keys normed and rotated on the way (as in
+    ``omni_qk_rotary``; without ``table`` they are not rotated), values as they are.  With ``query`` the tokens' queries
+    are normed and rotated in the same launch and returned.
+
+    key, value   [tokens, kv_heads, head_dim], the sequences' new tokens one behind the other
+    key_pages, value_pages  [num_pages, kv_heads, page_size, head_dim] contiguous, written in place; page_size a power of
+                 two from 16
+    page_table   [sequences, max_pages] int32: the pages of each sequence, in order
+    kv_lens      [sequences] int32: keys of each sequence, the new ones included
+    cu_seqlens   [sequences + 1] int32: sequence b has the tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1, the last of
+                 them at position kv_lens[b] - 1
+    positions    [tokens] table rows to rotate by, where they are not the places in the sequence
+
+    Tokens whose page number or position lies outside the cache are not written, and no row but the new tokens' is.
+    Two new tokens must not name the same row of the cache (what it holds then is not defined).  Query rows of tokens
+    behind the last sequence come back as zeros.  Not differentiable."""
+    return _load_extension().omni_attn_cache_append(key, value, key_pages, value_pages, page_table, kv_lens, cu_seqlens,
+                                                    table, positions, query, query_norm, key_norm, float(eps),
+                                                    bool(interleaved))
+
+
+def omni_attention_packed(query: Tensor, key: Tensor, value: Tensor, cu_seqlens: Tensor, causal: bool = True,
+                          softcap: float = 0.0, return_lse: bool = False):
+    """Attention within each of the sequences that lie packed behind one another: whole prompts, without padding.
+
+    query [tokens, heads, head_dim], key and value [tokens, kv_heads, head_dim] with heads a multiple of kv_heads
+    (head h reads key head h // (heads // kv_heads)), fp16 / bf16, head_dim 32, 64 or 128; cu_seqlens as in
+    ``omni_cache_append``.  ``causal``: a token attends itself and those before it; else its whole sequence.  ``softcap``
+    as in ``omni_attention``.  Returns [tokens, heads, head_dim], with ``return_lse`` also the fp32 logsumexp
+    [tokens, heads].  Tokens behind the last sequence get zeros (-inf).  Not differentiable; for training, padded
+    batches go through ``omni_attention``."""
+    return _load_extension().omni_attn_packed(query, key, value, cu_seqlens, bool(causal), float(softcap), bool(return_lse))
+
+
+def omni_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_table: Tensor, kv_lens: Tensor,
+                         cu_seqlens: Tensor, causal: bool = True, softcap: float = 0.0, return_lse: bool = False):
+    """Attention of new tokens (one per sequence, a few, a chunk of a prompt) over the keys that a paged cache holds,
+    theirs included: ``omni_cache_append`` comes first.  Arguments as there and in ``omni_attention_packed``; the last
+    token of sequence b is at position kv_lens[b] - 1.  Without ``causal`` every token attends all kv_lens[b] keys, as the
+    tokens of an image attend one another.  Page numbers outside the cache are cut to it; rows behind kv_lens[b] are
+    never read."""
+    return _load_extension().omni_attn_paged(query, key_pages, value_pages, page_table, kv_lens, cu_seqlens, bool(causal),
+                                             float(softcap), bool(return_lse))
+
+
+# ----------------------------------------------------------------------------
 # Utilities (omni_attn_torch.py:1287-1364, generate_attn_data.py:87-107)
 # ----------------------------------------------------------------------------
 

@@ -1,0 +1,226 @@
+"""Attention of packed sequences, over their own keys and over a paged cache, against the plain form in 64 bits: every
+kernel (few rows and tiles, whole and in parts), head layouts, lengths from nothing to long ones, stale and bad pages."""
+import math
+
+import pytest
+import torch
+
+import omni_attn_torch as oat
+from serving_helpers import attention, attention_bound, offsets
+
+pytestmark = pytest.mark.gpu
+
+
+def _compare(o, lse, q, seqs, causal, softcap, dtype, what):
+    """seqs: (first token, tokens, k, v) per sequence, k and v [kv, Hk, D]."""
+    D = q.shape[-1]
+    assert o.shape == q.shape and o.dtype == dtype and lse.dtype == torch.float32 and lse.shape == q.shape[:2]
+    covered = 0
+    for t0, n, k, v in seqs:
+        covered = max(covered, t0 + n)
+        if n == 0:
+            continue
+        ro, mean, rl = attention(q[t0:t0 + n], k, v, k.shape[0] - n, causal, softcap)
+        go, gl = o[t0:t0 + n].double(), lse[t0:t0 + n].double()
+        empty = torch.isinf(rl)
+        assert torch.equal(torch.isinf(gl) & (gl < 0), empty), f"{what}: rows without a key differ"
+        assert bool((go[empty] == 0).all()), what
+        if k.shape[0] == 0:
+            continue
+        smax = (q[t0:t0 + n].double().norm(dim=-1).max() * k.double().norm(dim=-1).max()).item() / math.sqrt(D)
+        vmax = v.double().abs().sum(0).max().item()
+        over = (go - ro).abs() - attention_bound(ro, mean, vmax, dtype, softcap, D, smax)
+        assert bool((over <= 0).all()), f"{what}: sequence at {t0} beyond its bound by {over.max().item():.3e}"
+        # a logsumexp is a score and a logarithm in 32 bits
+        room = (D + 8) * 2.0 ** -24 * smax + 8 * 2.0 ** -23 * softcap + 2.0 ** -21 * (1 + rl[~empty].abs())
+        assert bool(((gl - rl)[~empty].abs() <= room).all()), f"{what}: logsumexp"
+    assert bool((o[covered:] == 0).all()) and bool(torch.isinf(lse[covered:]).all()), f"{what}: rows behind the last sequence"
+
+
+def _packed(gen, device, dtype, lens, Hq, Hk, D, behind=2):
+    T = sum(lens) + behind
+    make = lambda H: torch.randn(T, H, D, generator=gen).to(device=device, dtype=dtype)
+    return make(Hq), make(Hk), make(Hk), torch.tensor(offsets(lens), dtype=torch.int32, device=device)
+
+
+LENS = {
+    "one": [1], "empty_between": [1, 0, 5, 0], "tile_borders": [63, 64, 65, 127, 128, 129], "prompts": [300, 17, 1, 41],
+    "long": [1000], "short_many": [3] * 70 + [0] * 5 + [9] * 60, "none": [0, 0],
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("lens", list(LENS))
+@pytest.mark.parametrize("Hq,Hk,causal,softcap", [(1, 1, True, 0.0), (8, 2, True, 0.0), (6, 2, False, 0.0), (8, 8, True, 20.0),
+                                                   (16, 1, False, 15.0), (3, 1, True, 0.0)])
+def test_packed(gpu_device, dtype, D, lens, Hq, Hk, causal, softcap):
+    gen = torch.Generator().manual_seed(D + Hq)
+    n = LENS[lens]
+    q, k, v, cu = _packed(gen, gpu_device, dtype, n, Hq, Hk, D)
+    o, lse = oat.omni_attention_packed(q, k, v, cu, causal=causal, softcap=softcap, return_lse=True)
+    at = offsets(n)
+    _compare(o, lse, q, [(a, b - a, k[a:b], v[a:b]) for a, b in zip(at, at[1:])], causal, softcap, dtype, lens)
+    assert torch.equal(oat.omni_attention_packed(q, k, v, cu, causal=causal, softcap=softcap), o)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,Hq,Hk,D", [
+    ([1500, 2048, 700, 33, 128, 1], 32, 8, 128),   # tiles, whole: their order goes by length
+    ([1024] * 3, 16, 16, 64), ([2000, 100], 24, 24, 32),
+    ([40] * 330, 8, 8, 64)])                       # few rows, whole
+def test_packed_whole_tiles(gpu_device, dtype, lens, Hq, Hk, D):
+    gen = torch.Generator().manual_seed(Hq)
+    q, k, v, cu = _packed(gen, gpu_device, dtype, lens, Hq, Hk, D, behind=300)
+    o, lse = oat.omni_attention_packed(q, k, v, cu, return_lse=True)
+    at = offsets(lens)
+    _compare(o, lse, q, [(a, b - a, k[a:b], v[a:b]) for a, b in zip(at, at[1:])], True, 0.0, dtype, "whole")
+
+
+def test_packed_rows_of_a_fused_projection(gpu_device):
+    gen = torch.Generator().manual_seed(1)
+    dtype, T, Hq, Hk, D = torch.bfloat16, 200, 8, 2, 64
+    both = torch.randn(T, Hq + 2 * Hk, D, generator=gen).to(device=gpu_device, dtype=dtype)
+    q, k, v = both[:, :Hq], both[:, Hq:Hq + Hk], both[:, Hq + Hk:]
+    cu = torch.tensor([0, 120, 200], dtype=torch.int32, device=gpu_device)
+    want = oat.omni_attention_packed(q.contiguous(), k.contiguous(), v.contiguous(), cu, return_lse=True)
+    for x in ((q, k, v), (q, k.contiguous(), v), (torch.cat([q, q], -1)[..., :D], k, v.transpose(0, 1).contiguous().transpose(0, 1))):
+        got = oat.omni_attention_packed(*x, cu, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    odd = torch.empty(T, Hq, D + 1, dtype=dtype, device=gpu_device)[..., 1:]  # copied
+    odd.copy_(q)
+    assert torch.equal(oat.omni_attention_packed(odd, k, v, cu), want[0])
+
+
+def test_packed_agrees_with_the_block_sparse_operator(gpu_device):
+    """One sequence per batch element, as many key heads as query heads, a causal block mask: the same function."""
+    gen = torch.Generator().manual_seed(12)
+    dtype, B, H, S, D = torch.bfloat16, 2, 4, 512, 128
+    q, k, v = (torch.randn(B, S, H, D, generator=gen).to(device=gpu_device, dtype=dtype) for _ in range(3))
+    mask = oat.create_causal_omni_block_mask(B, H, S, S, device=gpu_device)
+    ref = oat.omni_attention(*(t.transpose(1, 2) for t in (q, k, v)), mask).transpose(1, 2)
+    cu = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=gpu_device)
+    got = oat.omni_attention_packed(*(t.reshape(B * S, H, D) for t in (q, k, v)), cu).view(B, S, H, D)
+    # two roundings of weights and results, each half a step of values of at most 4
+    assert (got.float() - ref.float()).abs().max().item() <= 4 * 4 * torch.finfo(dtype).eps / 2
+
+
+def _paged(gen, device, dtype, lens, kv, Hq, Hk, D, page, behind=2, spare=2):
+    T = sum(lens) + behind
+    q = torch.randn(T, Hq, D, generator=gen).to(device=device, dtype=dtype)
+    need = [-(-n // page) for n in kv]
+    num = sum(need) + spare
+    order = torch.randperm(num, generator=gen).to(torch.int32)
+    table = torch.full((len(lens), max(need + [1]) + 2), 2 ** 30, dtype=torch.int32)  # (bad numbers behind each sequence)
+    pools = [torch.full((num, Hk, page, D), float("nan"), dtype=dtype, device=device) for _ in range(2)]
+    keys, at = [], 0
+    for b, n in enumerate(kv):
+        table[b, :need[b]] = order[at:at + need[b]]
+        own = order[at:at + need[b]].long().to(device)
+        at += need[b]
+        rows = [torch.randn(n, Hk, D, generator=gen).to(device=device, dtype=dtype) for _ in range(2)]
+        for pool, x in zip(pools, rows):  # (rows behind the sequence stay NaN)
+            wide = torch.full((need[b] * page, Hk, D), float("nan"), dtype=dtype, device=device)
+            wide[:n] = x
+            if need[b]:
+                pool[own] = wide.view(need[b], page, Hk, D).transpose(1, 2)
+        keys.append(rows)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+    return q, pools, table.to(device), i32(kv), i32(offsets(lens)), keys
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("lens,kv,Hq,Hk,causal,softcap", [
+    ([1], [1], 8, 8, True, 0.0), ([1], [700], 32, 8, True, 0.0),
+    ([1] * 7, [1, 15, 16, 17, 500, 64, 1111], 8, 2, True, 0.0), ([1, 0, 1, 1], [90, 33, 0, 5], 4, 1, True, 20.0),
+    ([3, 1, 8], [3, 130, 77], 6, 2, True, 0.0), ([5, 2], [5, 300], 4, 4, False, 0.0),
+    ([70, 200, 1], [1500, 200, 40], 8, 2, True, 0.0), ([130], [900], 2, 1, False, 30.0),
+    ([4, 40], [2, 30], 2, 2, True, 0.0)])  # (fewer keys than tokens: the first tokens have none)
+def test_paged(gpu_device, dtype, D, page, lens, kv, Hq, Hk, causal, softcap):
+    gen = torch.Generator().manual_seed(page + D + len(lens))
+    q, (kp, vp), table, kv_lens, cu, keys = _paged(gen, gpu_device, dtype, lens, kv, Hq, Hk, D, page)
+    o, lse = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu, causal=causal, softcap=softcap, return_lse=True)
+    at = offsets(lens)
+    _compare(o, lse, q, [(at[b], lens[b], *keys[b]) for b in range(len(lens))], causal, softcap, dtype, f"page {page}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_paged_many_sequences_and_long_ones(gpu_device, dtype):
+    gen = torch.Generator().manual_seed(4)
+    for lens, kv, Hq, Hk, D in (([1] * 150, [1 + 37 * i % 400 for i in range(150)], 8, 2, 64), ([1, 1], [30000, 3], 16, 2, 128),
+                                ([260, 1], [9000, 20], 4, 1, 128)):
+        q, (kp, vp), table, kv_lens, cu, keys = _paged(gen, gpu_device, dtype, lens, kv, Hq, Hk, D, 32)
+        o, lse = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu, return_lse=True)
+        at = offsets(lens)
+        _compare(o, lse, q, [(at[b], lens[b], *keys[b]) for b in range(len(lens))], True, 0.0, dtype, str(kv[:3]))
+
+
+def test_bad_pages_do_not_fault_and_far_pages_are_read(gpu_device):
+    dtype, Hk, D, page = torch.float16, 8, 128, 64
+    num = (1 << 31) // (Hk * D * page) + 2  # more than 2^31 elements
+    kp, vp = (torch.zeros(num, Hk, page, D, dtype=dtype, device=gpu_device) for _ in range(2))
+    gen = torch.Generator().manual_seed(3)
+    for pool in (kp, vp):
+        pool[num - 2:] = torch.randn(2, Hk, page, D, generator=gen).to(device=gpu_device, dtype=dtype)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu_device)
+    q = torch.randn(101, 16, D, generator=gen).to(device=gpu_device, dtype=dtype)
+    keys = [pool[num - 2:].transpose(1, 2).reshape(2 * page, Hk, D) for pool in (kp, vp)]
+    for table in ([[num - 2, num - 1, -1]] * 2, [[num - 2, 2 ** 31 - 1, 5]] * 2):  # (a number beyond the cache is its last page)
+        for lens in ([1, 1], [100, 1]):
+            T = sum(lens)
+            o, lse = oat.omni_attention_paged(q[:T], kp, vp, i32(table), i32([100, 128]), i32(offsets(lens)), return_lse=True)
+            at = offsets(lens)
+            seqs = [(at[b], lens[b], keys[0][:n], keys[1][:n]) for b, n in enumerate((100, 128))]
+            _compare(o, lse, q[:T], seqs, True, 0.0, dtype, "far")
+    # lengths beyond the page table and below zero are cut, offsets that run backwards are empty sequences
+    o = oat.omni_attention_paged(q[:2], kp, vp, i32([[num - 2], [0]]), i32([10 ** 6, -5]), i32([0, 1, 2]))
+    want = oat.omni_attention_paged(q[:1], kp, vp, i32([[num - 2]]), i32([64]), i32([0, 1]))
+    assert torch.equal(o[:1], want) and bool((o[1] == 0).all())
+    oat.omni_attention_paged(q[:9], kp, vp, i32([[0], [1]]), i32([64, 64]), i32([7, 2, 500]))
+    torch.cuda.synchronize()
+
+
+def test_graph_replay_with_other_lengths_and_another_stream(gpu_device):
+    """Lengths and pages are read on the device: a captured step serves other lengths, and two captured steps that use
+    one after the other do not disturb each other."""
+    gen = torch.Generator().manual_seed(10)
+    dtype, B, Hq, Hk, D, page = torch.bfloat16, 5, 8, 2, 64, 16
+    kp, vp = (torch.randn(B * 40, Hk, page, D, generator=gen).to(device=gpu_device, dtype=dtype) for _ in range(2))
+    table = torch.randperm(B * 40, generator=gen).to(torch.int32).view(B, 40).to(gpu_device)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=gpu_device)
+    q = torch.randn(B, Hq, D, generator=gen).to(device=gpu_device, dtype=dtype)
+    k, v = (torch.randn(B, Hk, D, generator=gen).to(device=gpu_device, dtype=dtype) for _ in range(2))
+    kv_lens = torch.full((B,), 17, dtype=torch.int32, device=gpu_device)
+    angles = oat.omni_rotary_table(D, 640, device=gpu_device)
+
+    def step():
+        y = oat.omni_cache_append(k, v, kp, vp, table, kv_lens, cu, table=angles, query=q)
+        return oat.omni_attention_paged(y, kp, vp, table, kv_lens, cu, return_lse=True)
+
+    side = torch.cuda.Stream(device=gpu_device)
+    side.wait_stream(torch.cuda.current_stream(gpu_device))
+    with torch.cuda.stream(side):
+        on_side = step()
+    side.synchronize()
+    for a, b in zip(on_side, step()):
+        assert torch.equal(a, b)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for graph in graphs:
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(step())
+    torch.cuda.synchronize()
+    for rep in range(4):
+        kv_lens.copy_(torch.randint(1, 640, (B,), generator=gen).to(torch.int32))
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=gen).to(dtype))
+        eager = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            for a, b in zip(out, eager):
+                assert torch.equal(a, b), rep
