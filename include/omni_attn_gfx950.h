@@ -404,7 +404,7 @@ int omni_attn_packed_gfx950(const void* q, const void* k, const void* v, omni_at
                             omni_attn_strides v_at, void* o, float* lse_or_null, const int32_t* cu_seqlens,
                             void* workspace, size_t workspace_bytes, int tokens, int sequences, int Hq, int Hk, int D,
                             int causal, int dtype, float softcap, void* stream);
-size_t omni_attn_paged_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D);
+size_t omni_attn_paged_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D, int page_size, int max_pages);
 int omni_attn_paged_gfx950(const void* q, omni_attn_strides q_at, const void* k_pages, const void* v_pages, void* o,
                            float* lse_or_null, const int32_t* page_table, const int32_t* kv_lens,
                            const int32_t* cu_seqlens, void* workspace, size_t workspace_bytes, int tokens,

@@ -54,7 +54,7 @@ RESOURCES_JSON = os.path.join(OBJ, "kernel_resources.json")
 MIN_WAVES_PER_SIMD = {"fwd_kernel": 2, "fwd_ksplit": 2, "bwd_dq_kernel": 2, "bwd_dq_short": 2, "bwd_dq_ksplit": 2,
                       "bwd_dkdv_kernel": 2, "bwd_dkdv_split": 2, "fwd_generic_": 2, "serve_tile": 2, "serve_few": 2,
                       "qk_rotary_kernel": 3, "cache_append_kernel": 3, "qk_rotary_bwd": 2}
-SGPR_SPILLS_ALLOWED = ("bwd_dq_", "bwd_dkdv_", "fwd_ksplit", "fwd_generic_", "serve_tile", "qk_rotary_bwd")
+SGPR_SPILLS_ALLOWED = ("bwd_dq_", "bwd_dkdv_", "fwd_ksplit", "fwd_generic_", "serve_", "qk_rotary_bwd")
 # For the generic kernel scratch memory is what counts.  Forms that read rows at any alignment (E1E) have some: up to 32 columns
 # and 97 - 128 in fp16 (two registers' worth; at B=1 H=8 S=2048 D=125 48.5 us, 52.9 without, where the addresses of the
 # loads are worked out anew in every step) and 225 - 256 (half a tile's rows in flight in registers; with four waves, which

@@ -416,7 +416,8 @@ pybind11::object omni_attn_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tenso
   }
   if (some) {
     q = in_rows(q, 8);
-    const size_t bytes = omni_attn_paged_workspace_bytes(int(T), int(B), int(Hq), int(pages.Hk), int(D));
+    const size_t bytes = omni_attn_paged_workspace_bytes(int(T), int(B), int(Hq), int(pages.Hk), int(D), int(pages.size),
+                                                         int(page_table.size(1)));
     Tensor workspace;
     if (bytes) workspace = torch::empty({int64_t((bytes + 3) / 4)}, q.options().dtype(torch::kFloat32));
     const int rc = omni_attn_paged_gfx950(q.data_ptr(), strides_of(q), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),

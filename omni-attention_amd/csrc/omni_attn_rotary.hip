@@ -291,9 +291,19 @@ __global__ void __launch_bounds__(kBlockWaves * 64) cache_append_kernel(AppendPa
   const uint16_t* vin = ap.v + token * ap.v_at.row;
   uint16_t* qout = p.q.out + token * p.q.out_at.row;
   // the token's sequence: as many as end at or before it come first
+  // (a lane looks at every per-th first, then at those between)
+  const int per = (ap.sequences + 63) / 64;
   int b = 0;
-  for (int j0 = 0; j0 < ap.sequences; j0 += 64)
-    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j0 + lane < ap.sequences && ap.cu[1 + j0 + lane] <= token));
+  if (per > 1) {
+    const int64_t last = int64_t(lane + 1) * per;  // end of the lane's sequences
+    b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(last <= ap.sequences && ap.cu[last <= ap.sequences ? last : 0] <= token)) * per;
+  }
+  const int from = b;
+  for (int j0 = 0; j0 < per * 64 && from + j0 < ap.sequences && j0 < (per > 1 ? per : 64); j0 += 64) {
+    const int j = from + j0 + lane;
+    const bool in = j < ap.sequences && (per == 1 || j0 + lane < per);
+    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && ap.cu[1 + (in ? j : 0)] <= token));
+  }
   int64_t position = -1;
   uint16_t *krow = nullptr, *vrow = nullptr;
   bool owned = false;

@@ -11,13 +11,13 @@ namespace omni_attn {
 int device_units(int* n_xcd, int* cus);
 
 template <bool BF16, int D>
-int launch_serve(const ServeParams& p, bool tiles, unsigned blocks, hipStream_t stream);
-template <> int launch_serve<false, 32>(const ServeParams&, bool, unsigned, hipStream_t);
-template <> int launch_serve<false, 64>(const ServeParams&, bool, unsigned, hipStream_t);
-template <> int launch_serve<false, 128>(const ServeParams&, bool, unsigned, hipStream_t);
-template <> int launch_serve<true, 32>(const ServeParams&, bool, unsigned, hipStream_t);
-template <> int launch_serve<true, 64>(const ServeParams&, bool, unsigned, hipStream_t);
-template <> int launch_serve<true, 128>(const ServeParams&, bool, unsigned, hipStream_t);
+int launch_serve(const ServeParams& p, int waves, unsigned blocks, hipStream_t stream);
+template <> int launch_serve<false, 32>(const ServeParams&, int, unsigned, hipStream_t);
+template <> int launch_serve<false, 64>(const ServeParams&, int, unsigned, hipStream_t);
+template <> int launch_serve<false, 128>(const ServeParams&, int, unsigned, hipStream_t);
+template <> int launch_serve<true, 32>(const ServeParams&, int, unsigned, hipStream_t);
+template <> int launch_serve<true, 64>(const ServeParams&, int, unsigned, hipStream_t);
+template <> int launch_serve<true, 128>(const ServeParams&, int, unsigned, hipStream_t);
 
 namespace {
 
@@ -39,6 +39,13 @@ int check_sizes(int T, int B, int Hq, int Hk, int D) {
   return OMNI_ATTN_OK;
 }
 
+// (a wave's load fills up to 16 rows, of one page)
+int check_pages(int num_pages, int page_size, int max_pages) {
+  if (num_pages <= 0 || max_pages <= 0 || page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)) != 0)
+    return OMNI_ATTN_ERR_BAD_SHAPE;
+  return (long long)max_pages * page_size > 0x3fffffffLL ? OMNI_ATTN_ERR_TOO_LARGE : OMNI_ATTN_OK;
+}
+
 int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes, int dtype, float softcap, void* stream) {
   if (!(softcap >= 0.f) || std::isinf(softcap)) return OMNI_ATTN_ERR_BAD_SHAPE;
   if (dtype != OMNI_ATTN_DTYPE_F16 && dtype != OMNI_ATTN_DTYPE_BF16) return OMNI_ATTN_ERR_UNSUPPORTED_DTYPE;
@@ -48,18 +55,21 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
     return OMNI_ATTN_ERR_LAUNCH;
   }
   p.G = Hq / p.Hk;
+  p.per_lane = (p.B + 63) / 64;
   p.group = fast_div(uint32_t(p.G));
   p.heads = fast_div(uint32_t(p.Hk));
-  const ServePlan plan = plan_serve(p.T, p.B, p.Hk, p.G, p.page_table != nullptr, cus);
+  const ServePlan plan = plan_serve(p.T, p.B, p.Hk, p.G, p.page_table != nullptr ? int64_t(p.max_pages) << p.page_shift : 0, cus);
   const int64_t blocks = serve_blocks(plan.units, p.Hk, p.n_xcd);
   if (blocks > 0x7fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
   p.share = plan.share;
+  p.least_steps = plan.least_steps;
   p.units = int(plan.units);
   if (plan.share != 0.f) {
-    if (!workspace || workspace_bytes < plan.workspace_bytes(p.Hk, D)) return OMNI_ATTN_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < plan.workspace_bytes(p.T, p.Hk, D)) return OMNI_ATTN_ERR_WORKSPACE;
     if (misaligned(workspace, 16)) return OMNI_ATTN_ERR_MISALIGNED;
     p.sums = static_cast<float*>(workspace);
     p.stats = p.sums + plan.units * p.Hk * plan.rows() * D;
+    p.joins = reinterpret_cast<int32_t*>(p.stats + plan.units * p.Hk * plan.rows() * 2);
   }
   p.softcap = softcap;
   p.cap_c2 = softcap > 0.f ? float(2.0 * 1.4426950408889634 / (std::sqrt(double(D)) * double(softcap))) : 0.f;
@@ -69,9 +79,9 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
   const unsigned n = unsigned(blocks);
   int e;
   switch (D) {
-    case 32: e = bf ? launch_serve<true, 32>(p, plan.tiles, n, s) : launch_serve<false, 32>(p, plan.tiles, n, s); break;
-    case 64: e = bf ? launch_serve<true, 64>(p, plan.tiles, n, s) : launch_serve<false, 64>(p, plan.tiles, n, s); break;
-    default: e = bf ? launch_serve<true, 128>(p, plan.tiles, n, s) : launch_serve<false, 128>(p, plan.tiles, n, s); break;
+    case 32: e = bf ? launch_serve<true, 32>(p, plan.waves, n, s) : launch_serve<false, 32>(p, plan.waves, n, s); break;
+    case 64: e = bf ? launch_serve<true, 64>(p, plan.waves, n, s) : launch_serve<false, 64>(p, plan.waves, n, s); break;
+    default: e = bf ? launch_serve<true, 128>(p, plan.waves, n, s) : launch_serve<false, 128>(p, plan.waves, n, s); break;
   }
   if (e != 0) {
     record_hip_error(e);
@@ -80,24 +90,26 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
   return OMNI_ATTN_OK;
 }
 
-size_t workspace_of(int T, int B, int Hq, int Hk, int D, bool paged) {
+size_t workspace_of(int T, int B, int Hq, int Hk, int D, int64_t capacity) {
   int xcds = 0, cus = 0;
   if (check_sizes(T, B, Hq, Hk, D) != OMNI_ATTN_OK) return 0;
   if (const int e = device_units(&xcds, &cus)) {
     record_hip_error(e);
     return 0;
   }
-  return plan_serve(T, B, Hk, Hq / Hk, paged, cus).workspace_bytes(Hk, D);
+  return plan_serve(T, B, Hk, Hq / Hk, capacity, cus).workspace_bytes(T, Hk, D);
 }
 
 }  // namespace
 }  // namespace omni_attn
 
 extern "C" size_t omni_attn_packed_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D) {
-  return omni_attn::workspace_of(tokens, sequences, Hq, Hk, D, false);
+  return omni_attn::workspace_of(tokens, sequences, Hq, Hk, D, 0);
 }
-extern "C" size_t omni_attn_paged_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D) {
-  return omni_attn::workspace_of(tokens, sequences, Hq, Hk, D, true);
+extern "C" size_t omni_attn_paged_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D, int page_size,
+                                                  int max_pages) {
+  if (omni_attn::check_pages(1, page_size, max_pages) != OMNI_ATTN_OK) return 0;
+  return omni_attn::workspace_of(tokens, sequences, Hq, Hk, D, int64_t(page_size) * max_pages);
 }
 
 extern "C" int omni_attn_packed_gfx950(const void* q, const void* k, const void* v, omni_attn_strides q_at,
@@ -143,10 +155,7 @@ extern "C" int omni_attn_paged_gfx950(const void* q, omni_attn_strides q_at, con
     return OMNI_ATTN_ERR_MISALIGNED;
   if (const int rc = check_sizes(tokens, sequences, Hq, Hk, D)) return rc;
   if (const int rc = check_rows(q_at)) return rc;
-  // (a wave's load fills up to 16 rows, of one page)
-  if (num_pages <= 0 || max_pages <= 0 || page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)) != 0)
-    return OMNI_ATTN_ERR_BAD_SHAPE;
-  if ((long long)max_pages * page_size > 0x3fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
+  if (const int rc = check_pages(num_pages, page_size, max_pages)) return rc;
   ServeParams p{};
   p.q = static_cast<const uint16_t*>(q);
   p.k = static_cast<const uint16_t*>(k_pages);

@@ -33,14 +33,17 @@ struct ServeParams {
   const int32_t* page_table;  // [B, max_pages]
   int num_pages, max_pages, page_shift;
   int B, T, Hk, G;
+  int per_lane;        // sequences per lane of a wave: B / 64, up
   FastDiv group;       // by G
   FastDiv heads;       // by Hk
   int n_xcd;
   int causal;
   float share;         // units per key head that the batch's steps are shared over; 0: whole tiles
+  int least_steps;     // ... and the steps that a part may have in any case
   int units;           // units per key head that there is a place for
   float* sums;         // [units, Hk, M, D] unscaled O of parts
   float* stats;        // [units, Hk, M, 2] their reference points (log2 domain) and sums of weights
+  int32_t* joins;      // [T, 4] of a token: first token and number of parts of its sequence, number of its first unit
   float sl2, softcap, cap_c2;
 };
 
@@ -96,118 +99,142 @@ __device__ __forceinline__ int tiles_of(const ServeParams& p, const Sequence& s)
 }
 __device__ __forceinline__ int steps_of(int keys) { return (keys + kStepKeys - 1) / kStepKeys; }
 
-// Steps of a part: the batch's steps over the units they are shared by (the same number in every wave of both
-// kernels: the same sums in the same order), at least two.
-template <int M>
-__device__ __forceinline__ int part_steps(const ServeParams& p, int lane) {
-  float all = 0.f;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const Sequence s = sequence_of(p, b0 + lane);
-    all += wave_sum(float(tiles_of<M>(p, s)) * float(steps_of(s.kv)));
+// The sequences of a batch: a lane has p.per_lane neighbours, of up to 64 sequences one, which stays in registers.
+struct Batch {
+  Sequence own;
+  __device__ __forceinline__ Batch(const ServeParams& p, int lane) : own(sequence_of(p, lane)) {}
+  // f(sequence) summed over a lane's sequences.
+  template <class F>
+  __device__ __forceinline__ auto sum(const ServeParams& p, int lane, F&& f) const {
+    auto all = f(own);
+    if (p.per_lane > 1) {
+      all = f(sequence_of(p, lane * p.per_lane));
+#pragma unroll 4
+      for (int i = 1; i < p.per_lane; ++i) all += f(sequence_of(p, lane * p.per_lane + i));
+    }
+    return all;
   }
+};
+__device__ __forceinline__ Sequence pick(const Sequence& s, int lane) {
+  return {__builtin_amdgcn_readlane(s.first, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.kv, lane)};
+}
+// Of numbers 0, 1, ... given out to the sequences in order, f(sequence) to each: who has number `rank`.
+struct Place {
+  Sequence seq;
+  int b, in;  // the sequence, and which of its numbers; b -1: nobody's, of `in` that were given out
+};
+template <class F>
+__device__ __forceinline__ Place place_of(const ServeParams& p, const Batch& batch, int rank, int lane, F&& f) {
+  const int mine = batch.sum(p, lane, f), end = wave_scan(mine);
+  const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
+  if (beyond == 0) return Place{{}, -1, __builtin_amdgcn_readlane(end, 63)};
+  const int at = __builtin_ctzll(beyond);
+  rank -= __builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(mine, at);
+  if (p.per_lane == 1) return Place{pick(batch.own, at), at, rank};
+  for (int i0 = 0;; i0 += 64) {  // (one of the lane's sequences has it)
+    const int i = i0 + lane;
+    const Sequence s = sequence_of(p, i < p.per_lane ? at * p.per_lane + i : p.B);
+    const int n = f(s), last = wave_scan(n);
+    const uint64_t here = __builtin_amdgcn_ballot_w64(last > rank);
+    if (here != 0 || i0 + 64 >= p.per_lane) {
+      const int who = here != 0 ? __builtin_ctzll(here) : 0;
+      return Place{pick(s, who), at * p.per_lane + i0 + who,
+                   rank - (__builtin_amdgcn_readlane(last, who) - __builtin_amdgcn_readlane(n, who))};
+    }
+    rank -= __builtin_amdgcn_readlane(last, 63);
+  }
+}
+
+// A sequence's keys in parts of at most `most` steps: as few as that takes, as even as whole steps allow.
+struct Parts {
+  int n, steps;
+};
+__device__ __forceinline__ Parts parts_of(int kv, int most) {
+  const int all = steps_of(kv);
+  if (all <= most) return {1, all};
+  const int n = int(uint32_t(all + most - 1) / uint32_t(most)), each = int(uint32_t(all + n - 1) / uint32_t(n));
+  return {int(uint32_t(all + each - 1) / uint32_t(each)), each};
+}
+// The most steps of a part: the batch's steps over the units that they are shared by.  (The same number in every
+// wave: the same sums in the same order.)
+template <int M>
+__device__ __forceinline__ int part_steps(const ServeParams& p, const Batch& batch, int lane) {
+  const float all = wave_sum(batch.sum(p, lane, [&](const Sequence& s) { return float(tiles_of<M>(p, s)) * float(steps_of(s.kv)); }));
   const float steps = ceilf(all / p.share);
   const int part = steps < 1e9f ? int(steps) : 1000000000;
-  return __builtin_amdgcn_readfirstlane(part < 2 ? 2 : part);
-}
-__device__ __forceinline__ int parts_of(int kv, int part) {
-  const int steps = steps_of(kv);
-  return steps <= part ? 1 : (steps + part - 1) / part;
+  return __builtin_amdgcn_readfirstlane(part < p.least_steps ? p.least_steps : part);
 }
 
 struct Unit {
   Sequence seq;
   int b, tile;
   int step0, steps;  // range of steps (all that the tile has may be fewer)
+  int base, parts;   // (shared by parts) number of the sequence's first unit, parts of each of its tiles
   bool part;         // one of several: its sums are joined later
-  bool found;
+  bool found;        // no: step0 is the number of units that there are
 };
-__device__ __forceinline__ Sequence pick(const Sequence& s, int lane) {
-  return {__builtin_amdgcn_readlane(s.first, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.kv, lane)};
-}
 
 // Unit number `rank` of tiles that are shared by parts: sequences in order, tiles in order, parts in order.
 template <int M>
-__device__ __forceinline__ Unit find_part(const ServeParams& p, int rank, int lane) {
-  const int part = part_steps<M>(p, lane);
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const Sequence s = sequence_of(p, b0 + lane);
-    const int tiles = tiles_of<M>(p, s), parts = parts_of(s.kv, part);
-    const int end = wave_scan(tiles * parts);
-    const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
-    if (beyond != 0) {
-      const int at = __builtin_ctzll(beyond);
-      Unit u;
-      u.seq = pick(s, at);
-      u.b = b0 + at;
-      const int n = __builtin_amdgcn_readlane(parts, at);
-      const int in = rank - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(tiles, at) * n);
-      u.tile = int(uint32_t(in) / uint32_t(n));
-      u.step0 = (in - u.tile * n) * part;
-      u.steps = part;
-      u.part = n > 1;
-      u.found = true;
-      return u;
-    }
-    rank -= __builtin_amdgcn_readlane(end, 63);
-  }
-  return Unit{{}, 0, 0, 0, 0, false, false};
+__device__ __forceinline__ Unit find_part(const ServeParams& p, const Batch& batch, int rank, int lane) {
+  const int most = part_steps<M>(p, batch, lane);
+  const Place at = place_of(p, batch, rank, lane, [&](const Sequence& s) { return tiles_of<M>(p, s) * parts_of(s.kv, most).n; });
+  if (at.b < 0) return Unit{{}, 0, 0, at.in, 0, 0, 0, false, false};
+  const Parts parts = parts_of(at.seq.kv, most);
+  const int tile = int(uint32_t(at.in) / uint32_t(parts.n));
+  return Unit{at.seq, at.b, tile, (at.in - tile * parts.n) * parts.steps, parts.steps, rank - at.in, parts.n, parts.n > 1, true};
 }
 
-// Unit number `rank` of whole tiles, those with most steps first: a launch then ends with short ones.  Steps are
-// compared in sixteen levels, which four rounds of counting find.
+// Unit number `rank` of whole tiles.  Of up to 64 sequences those with most steps come first, so that a launch ends with
+// short ones: steps are compared in sixteen levels, which four rounds of counting find.  More sequences come in order,
+// the last tile of each first.
 template <int M>
-__device__ __forceinline__ Unit find_tile(const ServeParams& p, int rank, int lane) {
+__device__ __forceinline__ Unit find_tile(const ServeParams& p, const Batch& batch, int rank, int lane) {
   constexpr int kLog = M == 128 ? 7 : 5;
   static_assert(M == 1 << kLog, "rows of a tile");
-  Unit u{{}, 0, 0, 0, 0x7fffffff, false, false};
-  int most = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const Sequence s = sequence_of(p, b0 + lane);
-    most = wave_max(s.n > 0 && steps_of(s.kv) > most ? steps_of(s.kv) : most);
+  constexpr int kAll = 0x7fffffff;
+  if (p.B == 1 || p.per_lane > 1) {
+    const Place at = place_of(p, batch, rank, lane, [&](const Sequence& s) { return tiles_of<M>(p, s); });
+    if (at.b < 0) return Unit{{}, 0, 0, at.in, 0, 0, 1, false, false};
+    return Unit{at.seq, at.b, tiles_of<M>(p, at.seq) - 1 - at.in, 0, kAll, 0, 1, false, true};
   }
+  const Sequence& s = batch.own;
+  const int most = wave_max(s.n > 0 ? steps_of(s.kv) : 0);
   int unit = 0;  // log2 of the steps of a level
   while ((most >> unit) > 15) ++unit;
   // tiles of a sequence with at least `steps` steps (its last ones)
-  auto long_tiles = [&](const Sequence& s, int steps) {
-    const int tiles = tiles_of<M>(p, s);
+  const int tiles = tiles_of<M>(p, s);
+  auto long_tiles = [&](int steps) {
     if (steps <= 0) return tiles;
     if (!p.causal) return steps_of(s.kv) >= steps ? tiles : 0;
     const int64_t token = int64_t(kStepKeys) * (steps - 1) - (s.kv - s.n);  // first token whose keys reach so far
     if (token >= s.n) return 0;
     return token <= 0 ? tiles : tiles - int((token * p.G) >> kLog);
   };
-  auto count = [&](int level) {
-    int n = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) n += wave_sum(long_tiles(sequence_of(p, b0 + lane), level << unit));
-    return n;
-  };
-  const int all = count(0);
-  if (all <= rank) {
-    u.step0 = all;  // (what the caller needs to know where no unit is left)
-    return u;
-  }
-  int level = 0;
-  for (int bit = 8; bit != 0; bit >>= 1)
-    if (count(level | bit) > rank) level |= bit;
-  rank -= level == 15 ? 0 : count(level + 1);
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const Sequence s = sequence_of(p, b0 + lane);
-    const int from = long_tiles(s, level << unit);
-    const int mine = from - (level == 15 ? 0 : long_tiles(s, (level + 1) << unit));
-    const int end = wave_scan(mine);
-    const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
-    if (beyond != 0) {
-      const int at = __builtin_ctzll(beyond);
-      u.seq = pick(s, at);
-      u.b = b0 + at;
-      const int in = rank - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(mine, at));
-      u.tile = tiles_of<M>(p, u.seq) - __builtin_amdgcn_readlane(from, at) + __builtin_amdgcn_readlane(mine, at) - 1 - in;
-      u.found = true;
-      return u;
+  const int all = wave_sum(tiles);
+  if (all <= rank) return Unit{{}, 0, 0, all, 0, 0, 1, false, false};
+  int level = 0, longer = 0;  // (tiles above the level)
+  for (int bit = 8; bit != 0; bit >>= 1) {
+    const int n = wave_sum(long_tiles((level | bit) << unit));
+    if (n > rank) {
+      level |= bit;
+    } else {
+      longer = n;
     }
-    rank -= __builtin_amdgcn_readlane(end, 63);
   }
-  return u;
+  const int from = long_tiles(level << unit), mine = from - (level == 15 ? 0 : long_tiles((level + 1) << unit));
+  const int end = wave_scan(mine);
+  rank -= longer;
+  const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
+  const int at = beyond != 0 ? __builtin_ctzll(beyond) : 0;
+  const int in = rank - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(mine, at));
+  const int tile = __builtin_amdgcn_readlane(tiles - from + mine, at) - 1 - in;
+  return Unit{pick(s, at), at, tile, 0, kAll, 0, 1, false, true};
+}
+template <int M>
+__device__ __forceinline__ Unit find_unit(const ServeParams& p, int rank, int lane) {
+  const Batch batch(p, lane);
+  return p.share > 0.f ? find_part<M>(p, batch, rank, lane) : find_tile<M>(p, batch, rank, lane);
 }
 
 // Workgroup -> (key head, rank).  Ids go round-robin over the XCDs: the heads are dealt to the XCDs, so that the
@@ -270,14 +297,7 @@ struct PageWindow {
   }
 };
 
-// O of a lane's row over the steps of a unit, and what its softmax needs.
-template <int DT>
-struct RowSums {
-  f32x16_t ot[DT];
-  float m_run, l_run;
-};
-
-// Weights of one step for a tile of 32 rows, written for a wave that has the step's scores of a row in a lane pair.
+// cap tanh(x / cap) of the scores.
 template <int NTL>
 __device__ __forceinline__ void cap_scores(f32x16_t (&st)[NTL], float cap, float c2) {
   static_for<16 * NTL>([&](auto ec) {
@@ -307,16 +327,28 @@ __device__ __forceinline__ float max_of(const f32x16_t (&st)[NTL], float sl2) {
   return pair_max(vmax(a, b)) * sl2;
 }
 
+// What the joining kernel needs to know of the unit's tokens; the first part of a tile tells it.
+template <int M>
+__device__ __forceinline__ void tell_joins(const ServeParams& p, const Unit& u, int head, int rows_all, int tid) {
+  typedef __attribute__((ext_vector_type(4))) int32_t i32x4;
+  if (p.share == 0.f || head != 0 || u.step0 != 0 || tid >= M) return;
+  const int row = u.tile * M + tid;
+  if (row >= rows_all) return;
+  const int token = int(divide(uint32_t(row), p.group));
+  *reinterpret_cast<i32x4*>(p.joins + (int64_t(u.seq.first) + token) * 4) = i32x4{u.seq.first, u.parts, u.base, 0};
+}
+
 // Where a unit's results go.
 template <bool BF16, int D, int M>
 __device__ __forceinline__ void store_rows(const ServeParams& p, const Unit& u, int head, int slot, int row0, int rows_all,
-                                           f32x16_t (&ot)[D / 32], float m_run, float l_run, uint16_t* stage, int lane) {
-  // row0: first row of the wave in the sequence; slot: number of the unit
+                                           f32x16_t (&ot)[D / 32], float m_run, float l_run, uint32_t skip, uint16_t* stage,
+                                           int lane) {
+  // row0: first row of the wave in the sequence; slot: number of the unit; skip: rows that are left out, by bit
   const int c = lane & 31, g = lane >> 5;
   const float l = pair_sum(l_run);
   if (u.part) {
     const int in_tile = (row0 & (M - 1)) + c;
-    if (row0 + c < rows_all) {
+    if (row0 + c < rows_all && !(skip >> c & 1)) {
       float* at = p.sums + ((int64_t(slot) * p.Hk + head) * M + in_tile) * D;
       typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 #pragma unroll
@@ -352,47 +384,144 @@ __device__ __forceinline__ void store_rows(const ServeParams& p, const Unit& u, 
     const int row = i * RPS + lane / CPR;
     const u32x4_t val = *reinterpret_cast<const u32x4_t*>(stage + row * D + pch * 8);
     const int r = row0 + row;
-    if (r < rows_all) {
+    if (r < rows_all && !(skip >> row & 1)) {
       const int token = int(divide(uint32_t(r), p.group));
       const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (r - token * p.G);
       *reinterpret_cast<u32x4_t*>(p.o + at * D + (pch ^ k_swizzle<D>(row)) * 8) = val;
     }
   }
-  if (p.lse != nullptr && g == 0 && row0 + c < rows_all) {
+  if (p.lse != nullptr && g == 0 && row0 + c < rows_all && !(skip >> c & 1)) {
     const int token = int(divide(uint32_t(row0 + c), p.group));
     p.lse[(int64_t(u.seq.first + token) * p.Hk + head) * p.G + (row0 + c - token * p.G)] =
         live ? (m_run + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
   }
 }
 
-// ---- few rows: one wave per unit ---------------------------------------------------------------------------------
+// Rows whose sums are no numbers, in a unit where rows attend different keys: a weight of zero times a value that is
+// infinite or no number, of a key that the row does not attend, may have made them so.  Such a row (and one that is no
+// number by right) is summed again, over its own keys alone: a lane per key for the scores, a lane per dimensions for
+// the sums.  Slow, and never entered otherwise.  Returns the row's O in the lanes' dimensions (two per lane at
+// head_dim 128), its reference and its sum.
+template <bool BF16, int D, bool PAGED>
+__device__ __forceinline__ const uint16_t* key_row(const ServeParams& p, const Unit& u, int head, int key, bool is_v) {
+  if constexpr (PAGED) {
+    int page = p.page_table[int64_t(u.b) * p.max_pages + (key >> p.page_shift)];
+    page = page < 0 ? 0 : (page >= p.num_pages ? p.num_pages - 1 : page);
+    return (is_v ? p.v : p.k) + (((int64_t(page) * p.Hk + head) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * D;
+  } else {
+    const RowStrides& at = is_v ? p.v_at : p.k_at;
+    return (is_v ? p.v : p.k) + (int64_t(u.seq.first) + key) * at.row + head * at.h;
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ float widen16(uint32_t x) {
+  if constexpr (BF16) {
+    return __builtin_bit_cast(float, x << 16);
+  } else {
+    return float(__builtin_bit_cast(_Float16, uint16_t(x)));
+  }
+}
+template <bool BF16, int D, int M, bool PAGED>
+__device__ void sum_rows_again(const ServeParams& p, const Unit& u, int head, int slot, int row0, uint32_t rows, int from,
+                               int to, int lane) {
+  const int shift = u.seq.kv - u.seq.n;
+  for (; rows != 0; rows &= rows - 1) {
+    const int row = row0 + __builtin_ctz(rows), token = int(divide(uint32_t(row), p.group));
+    const int end = shift + token + 1 < to ? shift + token + 1 : to;
+    const uint16_t* q = p.q + int64_t(u.seq.first + token) * p.q_row + int64_t(head * p.G + (row - token * p.G)) * p.q_head;
+    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+    const int d = D == 128 ? 2 * lane : (lane < D ? lane : D - 1);
+    for (int key0 = from; key0 < end; key0 += 64) {
+      float x = -INFINITY;
+      if (key0 + lane < end) {
+        const uint16_t* k = key_row<BF16, D, PAGED>(p, u, head, key0 + lane, false);
+        x = 0.f;
+        for (int i = 0; i < D; ++i) x = __builtin_fmaf(widen16<BF16>(q[i]), widen16<BF16>(k[i]), x);
+        if (p.softcap > 0.f)
+          x = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * p.cap_c2) + 1.f), -2.f * p.softcap, p.softcap);
+        x *= p.sl2;
+      }
+      float most = x;
+      for (int i = 1; i < 64; i <<= 1) most = fmaxf(most, __shfl_xor(most, i));
+      const float m_new = fmaxf(m, most), m_ref = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_ref);
+      const float w = __builtin_amdgcn_exp2f(x - m_ref);
+      l = l * alpha + wave_sum(w);
+      o0 *= alpha;
+      o1 *= alpha;
+      m = m_new;
+      for (int j = 0; j < 64 && key0 + j < end; ++j) {
+        const float wj = __shfl(w, j);
+        const uint16_t* v = key_row<BF16, D, PAGED>(p, u, head, key0 + j, true);
+        o0 = __builtin_fmaf(wj, widen16<BF16>(v[d]), o0);
+        if constexpr (D == 128) o1 = __builtin_fmaf(wj, widen16<BF16>(v[d + 1]), o1);
+      }
+    }
+    if (u.part) {
+      const int64_t at = (int64_t(slot) * p.Hk + head) * M + (row & (M - 1));
+      if (lane < D) p.sums[at * D + d] = o0;
+      if constexpr (D == 128) p.sums[at * D + d + 1] = o1;
+      if (lane == 0) {
+        p.stats[at * 2] = m;
+        p.stats[at * 2 + 1] = l;
+      }
+      continue;
+    }
+    const bool live = l > 0.f || l != l;
+    const float inv = live ? 1.f / l : 0.f;
+    const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (row - token * p.G);
+    const uint32_t packed = live ? pack2<BF16>(o0 * inv, o1 * inv) : 0u;
+    if (lane < D) p.o[at * D + d] = uint16_t(packed);
+    if constexpr (D == 128) p.o[at * D + d + 1] = uint16_t(packed >> 16);
+    if (p.lse != nullptr && lane == 0) p.lse[at] = live ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+  }
+}
+// The rows of a wave whose O holds something that is no number (or infinite), bit by row.
+template <int DT>
+__device__ __forceinline__ uint32_t odd_rows(const f32x16_t (&ot)[DT]) {
+  float x = 0.f;
+  static_for<16 * DT>([&](auto ec) {
+    constexpr int e = decltype(ec)::value;
+    x = __builtin_fmaf(ot[e / 16][e % 16], 0.f, x);
+  });
+  const uint64_t odd = __builtin_amdgcn_ballot_w64(!(x == 0.f));
+  return uint32_t(odd) | uint32_t(odd >> 32);
+}
+
+__device__ __forceinline__ uint32_t live_rows(int rows) { return rows >= 32 ? ~0u : (rows <= 0 ? 0u : (1u << rows) - 1u); }
+
+// ---- few rows ---------------------------------------------------------------------------------------------------
 //
-// Single tokens, and a few.  The work is the reading of K and V: a unit is one wave of its own with two sets of
-// K and V tiles in LDS that direct loads fill a step ahead; nothing waits for another wave.
+// Single tokens, a few, and short prompts: tiles of 32 rows.  The work is the reading of K and V: a wave has a K and a V
+// tile of its own in LDS; the loads of the next K go out once the scores have been made of this one, those of the next V
+// behind the second product, and nothing waits for another wave.  KG waves of a workgroup share the steps of a unit (wave
+// i takes the steps i, i + KG, ...) and add up their results in LDS.
 
 template <int D>
 constexpr int kFewStep = D == 128 ? 32 : 64;  // keys per step: 16 KiB of K and V
 template <int D>
-constexpr size_t kFewLdsBytes = size_t(2) * 2 * kFewStep<D> * D * 2;
+constexpr size_t kFewLdsBytes = size_t(2) * kFewStep<D> * D * 2 + 256;  // of a wave: tiles, and room for its rows' statistics
 
-template <bool BF16, int D, bool PAGED>
-__global__ void __launch_bounds__(64) serve_few_kernel(const ServeParams p) {
+template <bool BF16, int D, bool PAGED, int KG>
+__global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p) {
   constexpr int M = 32, STEP = kFewStep<D>, NTL = STEP / 32, KS = D / 16, DT = D / 32, CPR = D / 8;
   constexpr int RPC = 64 / CPR, NCH = STEP / RPC, TILE = STEP * D;  // rows per load, loads per tile
   constexpr int KPER = RPC % 16 == 0 ? 1 : 16 / RPC;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
-  uint16_t* sK = reinterpret_cast<uint16_t*>(lds_raw);
-  uint16_t* sV = sK + 2 * TILE;
-  const int lane = threadIdx.x, g = lane >> 5, c = lane & 31;
+  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint16_t* sK = reinterpret_cast<uint16_t*>(lds_raw + kg * kFewLdsBytes<D>);
+  uint16_t* sV = sK + TILE;
+  const int lane = threadIdx.x & 63, g = lane >> 5, c = lane & 31;
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
-  const Unit u = p.share > 0.f ? find_part<M>(p, rank, lane) : find_tile<M>(p, rank, lane);
+  const Unit u = find_unit<M>(p, rank, lane);
   if (!u.found) {  // (with parts the joining kernel clears rows behind the last sequence)
-    if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, lane, 64);
+    if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, threadIdx.x, 64 * KG);
     return;
   }
   const int rows_all = u.seq.n * p.G, row0 = u.tile * M;
+  tell_joins<M>(p, u, head, rows_all, threadIdx.x);
   const int row = row0 + c < rows_all ? row0 + c : rows_all - 1;
   const int token = int(divide(uint32_t(row), p.group));
   const int limit = p.causal ? u.seq.kv - u.seq.n + token : u.seq.kv - 1;  // the row's last key
@@ -427,35 +556,27 @@ __global__ void __launch_bounds__(64) serve_few_kernel(const ServeParams p) {
   for (int i = 0; i < KPER; ++i) koff[i] = uint32_t(ld_row) * kpitch + uint32_t(ld_pch ^ k_swizzle<D>(ld_row + i * RPC)) * 16u;
   const uint32_t voff = uint32_t(ld_row) * vpitch + uint32_t((((ld_pch >> 1) ^ v_swizzle<D>(ld_row)) << 1) | (ld_pch & 1)) * 16u;
   const uint32_t lds_k = lds_offset_of(sK), lds_v = lds_offset_of(sV);
-  auto issue = [&](int buf, int key0) {
+  auto need_window = [&](int key0) {
     if constexpr (PAGED) {
-      const int w = (key0 >> p.page_shift) >> 6;
-      if (w != window.at) {
-        window.load(p, u.b, w, lane);
-        wait_loads();
-      }
+      const int n = (key0 >> p.page_shift) >> 6;
+      if (n != window.at) window.load(p, u.b, n, lane);
     }
-    i32x4_t rk, rv;
-    if constexpr (!PAGED) {
-      rk = kr.rows<D>(key0);
-      rv = vr.rows<D>(key0);
-    }
+  };
+  auto issue = [&](bool is_v, int key0) {
+    i32x4_t r;
+    if constexpr (!PAGED) r = is_v ? vr.rows<D>(key0) : kr.rows<D>(key0);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const uint32_t dst = uint32_t(buf) * (TILE * 2u) + uint32_t(i) * 1024u;
+      const uint32_t dst = (is_v ? lds_v : lds_k) + uint32_t(i) * 1024u, off = is_v ? voff : koff[i % KPER];
       if constexpr (PAGED) {
         const int key = key0 + i * RPC;
         const int page = __builtin_amdgcn_readlane(window.pages, (key >> p.page_shift) & 63);
         const int64_t at = (((int64_t(page) * p.Hk + head) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * D;
         int left = to - key;
         left = left < 0 ? 0 : (left > RPC ? RPC : left);
-        rk = make_buffer_resource(p.k + at, uint32_t(left) * (D * 2u));
-        rv = make_buffer_resource(p.v + at, uint32_t(left) * (D * 2u));
-        buffer_to_lds_b128(rk, koff[i % KPER], 0, lds_k + dst);
-        buffer_to_lds_b128(rv, voff, 0, lds_v + dst);
+        buffer_to_lds_b128(make_buffer_resource((is_v ? p.v : p.k) + at, uint32_t(left) * (D * 2u)), off, 0, dst);
       } else {
-        buffer_to_lds_b128(rk, koff[i % KPER], uint32_t(i * RPC) * kpitch, lds_k + dst);
-        buffer_to_lds_b128(rv, voff, uint32_t(i * RPC) * vpitch, lds_v + dst);
+        buffer_to_lds_b128(r, off, uint32_t(i * RPC) * (is_v ? vpitch : kpitch), dst);
       }
     }
   };
@@ -466,18 +587,17 @@ __global__ void __launch_bounds__(64) serve_few_kernel(const ServeParams p) {
   for (int dt = 0; dt < DT; ++dt) ot[dt] = zero16;
   float m_run = -INFINITY, l_run = 0.f;
   const int i16 = c & 15, j16 = c >> 4;
-  if (nsteps > 0) issue(0, from);
-  for (int it = 0; it < nsteps; ++it) {
-    const int key0 = from + it * STEP, buf = it & 1;
-    if (it + 1 < nsteps) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other set has been read
-      issue(buf ^ 1, key0 + STEP);
-      wait_loads_but<2 * NCH>();
-    } else {
-      wait_loads();
-    }
-    const uint16_t* tK = sK + buf * TILE;
-    const uint16_t* tV = sV + buf * TILE;
+  if (kg < nsteps) {
+    need_window(from + kg * STEP);
+    issue(false, from + kg * STEP);
+    issue(true, from + kg * STEP);
+  }
+  const uint16_t* tK = sK;
+  const uint16_t* tV = sV;
+  for (int it = kg; it < nsteps; it += KG) {
+    const int key0 = from + it * STEP;
+    const bool more = it + KG < nsteps;
+    wait_loads_but<NCH>();  // V may be under way
     f32x16_t st[NTL];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -487,6 +607,11 @@ __global__ void __launch_bounds__(64) serve_few_kernel(const ServeParams p) {
         const u32x4_t a = *reinterpret_cast<const u32x4_t*>(tK + r * D + ((2 * s + g) ^ k_swizzle<D>(r)) * 8);
         st[t] = mfma_32x32x16<BF16>(a, qf[s], s == 0 ? zero16 : st[t]);
       }
+    if (more) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+      need_window(key0 + KG * STEP);
+      issue(false, key0 + KG * STEP);
+    }
     if (p.softcap > 0.f) cap_scores<NTL>(st, p.softcap, p.cap_c2);
     if (key0 + STEP - 1 > first_key || key0 + STEP > to) {
       const int stop = limit < to - 1 ? limit : to - 1;
@@ -512,6 +637,11 @@ __global__ void __launch_bounds__(64) serve_few_kernel(const ServeParams p) {
       l_run += p0 + p1;
       pb[t][r >> 3][(r & 7) >> 1] = pack2<BF16>(p0, p1);
     });
+    if (more) {
+      wait_loads_but<NCH>();  // the next K may be under way
+    } else {
+      wait_loads();
+    }
 #pragma unroll
     for (int j = 0; j < (STEP / 16) * DT; ++j) {
       const int ts = j / DT, dt = j % DT;
@@ -521,9 +651,76 @@ __global__ void __launch_bounds__(64) serve_few_kernel(const ServeParams p) {
       const u32x2_t lo2 = __builtin_bit_cast(u32x2_t, lo), hi2 = __builtin_bit_cast(u32x2_t, hi);
       ot[dt] = mfma_32x32x16<BF16>(u32x4_t{lo2[0], lo2[1], hi2[0], hi2[1]}, pb[ts >> 1][ts & 1], ot[dt]);
     }
+    if (more) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
+      issue(true, key0 + KG * STEP);
+    }
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, sK, lane);
+  const bool several = p.causal && first_key < last_key;  // rows that attend different keys
+  if constexpr (KG == 1) {
+    const uint32_t odd = several ? odd_rows<DT>(ot) & live_rows(rows_all - row0) : 0u;
+    store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, odd, sK, lane);
+    if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
+  } else {
+    // Every wave's maxima and sums, then its O against the common maximum, into its own tiles; each wave adds up and
+    // stores a share of the columns.
+    constexpr int PIECES = DT * 4, MINE = PIECES / KG;  // 4-register pieces of a lane's O
+    constexpr size_t kStats = kFewLdsBytes<D> - 256;
+    static_assert(PIECES % KG == 0 && size_t(32) * D * 4 <= kStats, "merge layout");
+    typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+    auto piece_at = [&](int i, int piece) { return reinterpret_cast<f32x4_t*>(lds_raw + i * kFewLdsBytes<D>) + piece * 64 + lane; };
+    auto stat_at = [&](int i) { return reinterpret_cast<float*>(lds_raw + i * kFewLdsBytes<D> + kStats) + 2 * c; };
+    const float l = pair_sum(l_run);
+    const uint32_t mine_odd = several ? odd_rows<DT>(ot) : 0u;
+    if (g == 0) {
+      stat_at(kg)[0] = m_run;
+      stat_at(kg)[1] = mine_odd >> c & 1 ? __builtin_nanf("") : l;
+    }
+    static_for<PIECES>([&](auto pc) {
+      constexpr int piece = decltype(pc)::value, dt = piece / 4, r = 4 * (piece % 4);
+      *piece_at(kg, piece) = f32x4_t{ot[dt][r], ot[dt][r + 1], ot[dt][r + 2], ot[dt][r + 3]};
+    });
+    __syncthreads();
+    float m_all = -INFINITY, l_all = 0.f, scale[KG];
+#pragma unroll
+    for (int i = 0; i < KG; ++i) m_all = fmaxf(m_all, stat_at(i)[0]);
+    const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+#pragma unroll
+    for (int i = 0; i < KG; ++i) {
+      scale[i] = __builtin_amdgcn_exp2f(stat_at(i)[0] - m_ref);
+      l_all += stat_at(i)[1] * scale[i];
+    }
+    const bool live = l_all > 0.f || l_all != l_all;
+    const float inv = u.part ? 1.f : (live ? 1.f / l_all : 0.f);
+    const uint32_t odd = several ? uint32_t(__builtin_amdgcn_ballot_w64(l_all != l_all)) & live_rows(rows_all - row0) : 0u;
+    const bool mine = row0 + c < rows_all && !(odd >> c & 1);
+    const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (row - token * p.G);
+    const int64_t part_at = (int64_t(rank) * p.Hk + head) * M + c;
+#pragma unroll
+    for (int n = 0; n < MINE; ++n) {
+      const int piece = kg * MINE + n;
+      f32x4_t x = *piece_at(0, piece) * scale[0];
+#pragma unroll
+      for (int i = 1; i < KG; ++i) x += *piece_at(i, piece) * scale[i];
+      if (!mine) continue;
+      if (u.part) {
+        *reinterpret_cast<f32x4_t*>(p.sums + part_at * D + 8 * piece + 4 * g) = x;
+      } else {
+        const u32x2_t ov = {live ? pack2<BF16>(x[0] * inv, x[1] * inv) : 0u, live ? pack2<BF16>(x[2] * inv, x[3] * inv) : 0u};
+        *reinterpret_cast<u32x2_t*>(p.o + at * D + 8 * piece + 4 * g) = ov;
+      }
+    }
+    if (kg == 0 && g == 0 && mine) {
+      if (u.part) {
+        p.stats[part_at * 2] = m_all;
+        p.stats[part_at * 2 + 1] = l_all;
+      } else if (p.lse != nullptr) {
+        p.lse[at] = live ? (m_all + __builtin_amdgcn_logf(l_all)) * 0.6931471805599453f : -INFINITY;
+      }
+    }
+    if (kg == 0 && odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
+  }
 }
 
 // ---- many rows: four waves per unit -------------------------------------------------------------------------------
@@ -552,13 +749,14 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
-  const Unit u = p.share > 0.f ? find_part<M>(p, rank, lane) : find_tile<M>(p, rank, lane);
+  const Unit u = find_unit<M>(p, rank, lane);
   if (!u.found) {
     if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, tid, 256);
     return;
   }
   const int shift = u.seq.kv - u.seq.n;  // a token's position, less its number
   const int rows_all = u.seq.n * p.G, row0 = u.tile * M + 32 * w;
+  tell_joins<M>(p, u, head, rows_all, tid);
   const int row = row0 + c < rows_all ? row0 + c : rows_all - 1;
   const int token = int(divide(uint32_t(row), p.group));
   const int last_row = u.tile * M + M < rows_all ? u.tile * M + M - 1 : rows_all - 1;
@@ -846,73 +1044,75 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
     }
   }
   // (the K tiles are read by nobody any more: a wave stages its rows in a quarter of them)
-  store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, sK + w * 32 * D, lane);
+  const uint32_t odd = p.causal && first_key < last_key ? odd_rows<DT>(ot) & live_rows(rows_all - row0) : 0u;
+  store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, odd, sK + w * 32 * D, lane);
+  if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
 }
 
-// Joins the parts of a row: a wave per token and query head.  Clears the rows behind the last sequence too.
+// Joins the parts of a row.  A wave has one token and R of its heads, 16 bytes of a part's row per lane.  Clears the rows
+// behind the last sequence too.
+template <int D>
+constexpr int kJoinRows = 256 / D;
 template <bool BF16, int D, int M>
 __global__ void __launch_bounds__(256) serve_join_kernel(const ServeParams p) {
+  typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+  constexpr int R = kJoinRows<D>, LPR = 64 / R;  // lanes per row
   const int lane = threadIdx.x & 63;
-  const int64_t id = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int Hq = p.Hk * p.G;
-  const int64_t t64 = id / Hq;
-  if (t64 >= p.T) return;
-  const int t = int(t64), h = int(id - t64 * Hq), head = int(divide(uint32_t(h), p.group));
-  const int part = part_steps<M>(p, lane);
-  int before = 0;
-  Unit u{{}, 0, 0, 0, 0, false, false};
-  for (int b0 = 0; b0 < p.B && !u.found; b0 += 64) {
-    const Sequence s = sequence_of(p, b0 + lane);
-    const int units = tiles_of<M>(p, s) * parts_of(s.kv, part);
-    const int end = wave_scan(units);
-    const uint64_t here = __builtin_amdgcn_ballot_w64(t >= s.first && t < s.first + s.n);
-    if (here != 0) {
-      const int at = __builtin_ctzll(here);
-      u.seq = pick(s, at);
-      u.found = true;
-      before += __builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(units, at);
-    } else {
-      before += __builtin_amdgcn_readlane(end, 63);
+  const uint32_t id = blockIdx.x * 4u + uint32_t(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  const int Hq = p.Hk * p.G, groups = (Hq + R - 1) / R;
+  const int t = int(id / uint32_t(groups)), h = int(id - uint32_t(t) * uint32_t(groups)) * R + lane / LPR;
+  if (t >= p.T) return;
+  const bool behind = t >= p.cu[p.B];
+  const int32_t* told = p.joins + int64_t(t) * 4;
+  const int first = load_uniform(told), parts = behind ? 0 : load_uniform(told + 1), before = load_uniform(told + 2);
+  if (parts == 1) return;  // written where it was computed
+  const bool mine = h < Hq;
+  const int d = (lane & (LPR - 1)) * 4;
+  const int64_t out = int64_t(t) * Hq + h;
+  if (behind) {
+    if (mine) {
+      *reinterpret_cast<u32x2_t*>(p.o + out * D + d) = u32x2_t{0u, 0u};
+      if (p.lse != nullptr && d == 0) p.lse[out] = -INFINITY;
     }
-  }
-  uint16_t* out = p.o + id * D;
-  if (!u.found) {
-    for (int d = lane; d < D; d += 64) out[d] = 0;
-    if (p.lse != nullptr && lane == 0) p.lse[id] = -INFINITY;
     return;
   }
-  const int parts = parts_of(u.seq.kv, part);
-  if (parts == 1) return;  // written where it was computed
-  const int row = (t - u.seq.first) * p.G + (h - head * p.G);
-  const int64_t slot = before + int64_t(row / M) * parts;
-  const int64_t at = (slot * p.Hk + head) * M + row % M, step = int64_t(p.Hk) * M;
+  const int head = int(divide(uint32_t(mine ? h : Hq - 1), p.group));
+  const int row = (t - first) * p.G + ((mine ? h : Hq - 1) - head * p.G);
+  // (a token that no sequence has, where the offsets run backwards, has been told nothing)
+  if (parts < 1 || first < 0 || first > t || before < 0 || before + (int64_t(row / M) + 1) * parts > p.units) return;
+  const int64_t at = ((before + int64_t(row / M) * parts) * p.Hk + head) * M + row % M, step = int64_t(p.Hk) * M;
   float m = -INFINITY;
-  for (int i = lane; i < parts; i += 64) m = fmaxf(m, p.stats[(at + i * step) * 2]);
-  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-  const float m_ref = m == -INFINITY ? 0.f : m;
-  constexpr int N = D >= 64 ? D / 64 : 1;  // neighbouring dimensions of a lane
-  const int d = lane * N;
-  float sum[N] = {}, l = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float* st = p.stats + (at + i * step) * 2;
-    const float w = __builtin_amdgcn_exp2f(st[0] - m_ref);
-    l += st[1] * w;
-    if (d < D) {
-      const float* x = p.sums + (at + i * step) * D + d;
+  for (int i = lane & (LPR - 1); i < parts; i += LPR) m = fmaxf(m, p.stats[(at + i * step) * 2]);
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum[j] = __builtin_fmaf(x[j], w, sum[j]);
+  for (int x = 1; x < LPR; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+  const float m_ref = m == -INFINITY ? 0.f : m;
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int i0 = 0; i0 < parts; i0 += 4) {
+    f32x4_t x[4];
+    float w[4], lw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // (the last part again in the place of those that there are not)
+      const int i = i0 + j < parts ? i0 + j : parts - 1;
+      x[j] = *reinterpret_cast<const f32x4_t*>(p.sums + (at + i * step) * D + d);
+      w[j] = p.stats[(at + i * step) * 2];
+      lw[j] = p.stats[(at + i * step) * 2 + 1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i0 + j >= parts) break;
+      const float f = __builtin_amdgcn_exp2f(w[j] - m_ref);
+      l = __builtin_fmaf(lw[j], f, l);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] = __builtin_fmaf(x[j][k], f, sum[k]);
     }
   }
+  if (!mine) return;
   const bool live = l > 0.f || l != l;
   const float inv = live ? 1.f / l : 0.f;
-  if (d < D) {
-    if constexpr (N == 2) {
-      *reinterpret_cast<uint32_t*>(out + d) = live ? pack2<BF16>(sum[0] * inv, sum[1] * inv) : 0u;
-    } else {
-      out[d] = live ? uint16_t(pack2<BF16>(sum[0] * inv, 0.f)) : uint16_t(0);
-    }
-  }
-  if (p.lse != nullptr && lane == 0) p.lse[id] = live ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+  const u32x2_t ov = {live ? pack2<BF16>(sum[0] * inv, sum[1] * inv) : 0u, live ? pack2<BF16>(sum[2] * inv, sum[3] * inv) : 0u};
+  *reinterpret_cast<u32x2_t*>(p.o + out * D + d) = ov;
+  if (p.lse != nullptr && d == 0) p.lse[out] = live ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 }  // namespace omni_attn

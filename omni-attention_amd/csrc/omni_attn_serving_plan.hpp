@@ -8,24 +8,49 @@
 namespace omni_attn {
 
 struct ServePlan {
-  bool tiles;      // tiles of 128 rows and four waves; else 32 rows and a wave of its own
+  int waves;       // 0: tiles of 128 rows and four waves; else tiles of 32 rows and so many waves
   float share;     // units per key head that the steps are shared over, 0: whole tiles
+  int least_steps; // steps that a part may have in any case
   int64_t units;   // units per key head that there is a place for
-  int rows() const { return tiles ? 128 : 32; }
-  size_t workspace_bytes(int Hk, int D) const {
-    return share == 0.f ? 0 : size_t(units) * size_t(Hk) * size_t(rows()) * size_t(D + 2) * sizeof(float);
+  int rows() const { return waves == 0 ? 128 : 32; }
+  size_t workspace_bytes(int64_t T, int Hk, int D) const {  // the parts' rows and statistics, and four words per token
+    return share == 0.f ? 0 : size_t(units) * size_t(Hk) * size_t(rows()) * size_t(D + 2) * sizeof(float) + size_t(T) * 16;
   }
 };
 
-// T tokens in B sequences, Hk key heads with G query heads each; cus: compute units.
-inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, bool paged, int cus) {
+// T tokens in B sequences, Hk key heads with G query heads each; capacity: keys that a page table has room for, 0:
+// packed; cus: compute units.  Lengths are not known here: a sequence is taken to have T / B tokens, and keys of a
+// cache that there may be any number of.
+inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, int64_t capacity, int cus) {
   ServePlan s;
-  s.tiles = T * G > 64 * B;
-  const int64_t slots = int64_t(cus) * (s.tiles ? 2 : 5);
-  // tiles of all sequences, at most: each has one that is not full
-  const int64_t tiles = T * G / s.rows() + B;
-  const int64_t wanted = s.tiles ? slots : 2 * slots;
-  const bool parts = s.tiles ? tiles * Hk < slots : (paged || tiles * Hk < wanted);
+  const int64_t rows = T * G;
+  const auto tiles_of = [&](int64_t M) { return rows / M + B; };  // at most: every sequence has one that is not full
+  const int64_t keys = capacity != 0 ? capacity : T / B;
+  int64_t wanted = 0;  // units in all, where tiles are shared by parts
+  s.least_steps = 2;
+  if (rows <= 64 * B) {
+    // Single tokens, a few.  One wave per tile where keys are few and tiles more than the card holds at a time: D=128, 32 / 8
+    // heads, 512 sequences of 30 - 100 keys 34 us, 58 with four waves, 110 with four and parts; 256 of 100 - 300 keys 41, 47
+    // and 61; 200 prompts of 60 tokens 24 and 41.  Else four waves and parts: 8 tokens after 2000 keys 22 us, 34 with whole
+    // tiles, 106 with one wave; after 60000 keys 345, 900 and 3232; 64 tokens after 500 - 1500 keys 50 us, 44 with whole tiles
+    // (lengths are not known here).  Twice as many units or half as many: within 3 %.
+    s.waves = (keys <= 512 && tiles_of(32) * Hk > 4 * cus) || (capacity == 0 && keys <= 128) ? 1 : 4;
+    if (s.waves == 4 && keys > 512) wanted = 4 * cus;
+    s.least_steps = 4;
+  } else if (tiles_of(32) * Hk <= 2 * cus + B * Hk && keys <= 2560) {
+    // Prompts whose 32-row tiles all run at once: four waves on the keys of each.  512 tokens, D=64, 8 heads 6.8 us, 10.4 with
+    // tiles of 128 rows; 2048 tokens 15 and 26; D=128, 32 / 8 heads, 512 tokens 11.2 and 13.5 (1024 tokens, beyond the line,
+    // 26 and 22; 8192 tokens, 2 heads, 81 and 63 in parts).
+    s.waves = 4;
+  } else {
+    // Parts where the tiles leave compute units without work: 4096 tokens, one head, 26 us, 61 whole; 8192, 2 heads, 64 and
+    // 117; 812 new tokens after 22000, 32 / 8 heads, 197 and 307 (2000 after 10000, beyond the line, 377 and 347).
+    s.waves = 0;
+    if (tiles_of(128) * Hk <= (capacity != 0 ? 3 * cus / 2 : cus) && keys > 2560) wanted = 3 * cus;
+    s.least_steps = 8;
+  }
+  const int64_t tiles = tiles_of(s.rows());
+  const bool parts = wanted != 0;
   s.share = parts ? float((wanted + Hk - 1) / Hk) : 0.f;
   // (the sum of what every tile is over a whole number of parts; one more workgroup, so that there is always one
   // without a unit, which clears rows behind the last sequence)

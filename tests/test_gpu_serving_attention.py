@@ -157,6 +157,34 @@ def test_paged_many_sequences_and_long_ones(gpu_device, dtype):
         _compare(o, lse, q, [(at[b], lens[b], *keys[b]) for b in range(len(lens))], True, 0.0, dtype, str(kv[:3]))
 
 
+@pytest.mark.parametrize("lens,kv", [([1, 6, 3], [50, 6, 90]), ([200, 90], [200, 300])])
+def test_values_that_are_no_numbers_behind_a_row(gpu_device, lens, kv):
+    """Infinities and NaN in K and V of later keys of the same sequence reach no row that does not attend them."""
+    gen = torch.Generator().manual_seed(7)
+    dtype, Hq, Hk, D, page = torch.bfloat16, 4, 2, 64, 16
+    q, (kp, vp), table, kv_lens, cu, keys = _paged(gen, gpu_device, dtype, lens, kv, Hq, Hk, D, page)
+    clean = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu)
+    at = offsets(lens)
+    for b, n in enumerate(lens):
+        if n < 2:
+            continue
+        last = kv[b] - 1 - n // 4  # this key and what is behind it is spoilt
+        for pos in range(last, kv[b]):
+            pg = int(table[b, pos // page])
+            vp[pg, :, pos % page, ::3] = float("inf") if pos % 2 else float("nan")
+            if pos % 3 == 0:
+                kp[pg, :, pos % page] = float("nan")
+    dirty = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu)
+    for b, n in enumerate(lens):
+        first_bad = n - 1 - n // 4 if n >= 2 else n
+        a = at[b]
+        # (a row may be summed in another order once a neighbour is spoilt)
+        diff = (clean[a:a + first_bad].float() - dirty[a:a + first_bad].float()).abs()
+        assert bool((diff <= 4 * torch.finfo(dtype).eps).all()), b
+        if n >= 2:
+            assert not bool(torch.isfinite(dirty[a + first_bad:a + n, :, 0]).any())  # (an infinity alone stays one)
+
+
 def test_bad_pages_do_not_fault_and_far_pages_are_read(gpu_device):
     dtype, Hk, D, page = torch.float16, 8, 128, 64
     num = (1 << 31) // (Hk * D * page) + 2  # more than 2^31 elements

@@ -151,25 +151,30 @@ PROGRAM = r"""
 using namespace omni_attn;
 // What the kernels count on the device, over the sequences that come in: tokens, keys.
 int main() {
-  int B, Hk, G, paged;
-  while (scanf("%d %d %d %d", &B, &Hk, &G, &paged) == 4) {
+  int B, Hk, G, capacity;
+  while (scanf("%d %d %d %d", &B, &Hk, &G, &capacity) == 4) {
     std::vector<long long> n(B), kv(B);
     long long T = 0;
     for (int b = 0; b < B; ++b) {
       if (scanf("%lld %lld", &n[b], &kv[b]) != 2) return 1;
       T += n[b];
     }
-    const ServePlan s = plan_serve(T, B, Hk, G, paged != 0, 256);
+    const ServePlan s = plan_serve(T, B, Hk, G, capacity, 256);
     const long long M = s.rows();
     long long units = 0, part = 0;
     if (s.share > 0.f) {
       float all = 0.f;
       for (int b = 0; b < B; ++b) all += float((n[b] * G + M - 1) / M) * float((kv[b] + 63) / 64);
       part = (long long)std::ceil(all / s.share);
-      if (part < 2) part = 2;
+      if (part < s.least_steps) part = s.least_steps;
     }
     for (int b = 0; b < B; ++b) {
-      const long long steps = (kv[b] + 63) / 64, parts = part == 0 || steps <= part ? 1 : (steps + part - 1) / part;
+      const long long steps = (kv[b] + 63) / 64;
+      long long parts = part == 0 || steps <= part ? 1 : (steps + part - 1) / part;
+      if (parts > 1) {  // as even as whole steps allow
+        const long long each = (steps + parts - 1) / parts;
+        parts = (steps + each - 1) / each;
+      }
       units += (n[b] * G + M - 1) / M * parts;
     }
     long long at_head = 0;
@@ -179,7 +184,7 @@ int main() {
       if (at_head < s.units) at_head = -1;
       if (at_head < 0) break;
     }
-    printf("%lld %lld %lld %d\n", units, (long long)s.units, at_head, int(s.share > 0.f));
+    printf("%lld %lld %lld %d %d\n", units, (long long)s.units, at_head, int(s.share > 0.f), s.waves);
   }
 }
 """
@@ -200,12 +205,13 @@ def test_every_unit_has_a_place(tmp_path):
         kv = [m + rng.randint(0, int(math.exp(rng.uniform(0, 11)))) if paged else m for m in n]
         if sum(n) == 0:
             n[0] = kv[0] = 1
-        lines.append(f"{B} {Hk} {G} {int(paged)} " + " ".join(f"{a} {b}" for a, b in zip(n, kv)))
+        capacity = max(kv) + rng.choice([0, 100, 10 ** 5]) if paged else 0
+        lines.append(f"{B} {Hk} {G} {capacity} " + " ".join(f"{a} {b}" for a, b in zip(n, kv)))
     out = subprocess.run([exe], input="\n".join(lines), stdout=subprocess.PIPE, text=True, check=True).stdout.split("\n")
     assert len(out) == len(lines) + 1
     seen = set()
     for line, given in zip(out, lines):
-        units, room, at_head, parts = map(int, line.split())
-        seen.add(parts)
+        units, room, at_head, parts, waves = map(int, line.split())
+        seen.add((parts, waves))
         assert units <= (room if parts else room - 1) and at_head >= room, given[:200]
-    assert seen == {0, 1}
+    assert seen == {(0, 0), (1, 0), (0, 1), (0, 4), (1, 4)}
