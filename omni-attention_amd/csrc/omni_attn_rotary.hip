@@ -57,7 +57,7 @@ struct RotaryBwdParams {
   RotaryParams r;  // in: the incoming gradients, out: the outgoing ones
   const uint16_t *xq, *xk;
   RowStrides xq_at, xk_at;
-  float* partial;  // [blocks, 2, D]
+  float* partial;  // [2, blocks, D]
 };
 
 template <bool BF16>
@@ -290,49 +290,14 @@ __global__ void __launch_bounds__(kBlockWaves * 64) cache_append_kernel(AppendPa
   const uint16_t* kin = p.k.in + token * p.k.in_at.row;
   const uint16_t* vin = ap.v + token * ap.v_at.row;
   uint16_t* qout = p.q.out + token * p.q.out_at.row;
-  // the token's sequence: as many as end at or before it come first
-  // (a lane looks at every per-th first, then at those between)
-  const int per = (ap.sequences + 63) / 64;
-  int b = 0;
-  if (per > 1) {
-    const int64_t last = int64_t(lane + 1) * per;  // end of the lane's sequences
-    b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(last <= ap.sequences && ap.cu[last <= ap.sequences ? last : 0] <= token)) * per;
-  }
-  const int from = b;
-  for (int j0 = 0; j0 < per * 64 && from + j0 < ap.sequences && j0 < (per > 1 ? per : 64); j0 += 64) {
-    const int j = from + j0 + lane;
-    const bool in = j < ap.sequences && (per == 1 || j0 + lane < per);
-    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && ap.cu[1 + (in ? j : 0)] <= token));
-  }
-  int64_t position = -1;
-  uint16_t *krow = nullptr, *vrow = nullptr;
-  bool owned = false;
-  if (b < ap.sequences && token >= ap.cu[b] && token < ap.cu[b + 1]) {
-    owned = true;
-    position = int64_t(ap.kv_lens[b]) - ap.cu[b + 1] + token;
-    const int64_t in_table = position >> ap.page_shift;
-    if (position >= 0 && in_table < ap.max_pages) {
-      const int page = ap.page_table[int64_t(b) * ap.max_pages + in_table];
-      if (page >= 0 && page < ap.num_pages) {
-        const int64_t row = ((int64_t(page) * p.k.heads) << ap.page_shift) + (position & ((1 << ap.page_shift) - 1));
-        krow = ap.k_pages + row * p.D;
-        vrow = ap.v_pages + row * p.D;
-      }
-    }
-  }
-  const int64_t head_step = int64_t(p.D) << ap.page_shift;
   const int qk = p.q.heads + p.k.heads, rows = qk + p.k.heads;
-  float wqa[V], wqb[V], wka[V], wkb[V], c[V], sn[V];
-  load_weight<BF16, V, INTER>(p.q.weight, p.weight32, at, wqa, wqb);
-  load_weight<BF16, V, INTER>(p.k.weight, p.weight32, at, wka, wkb);
-  load_turn<V>(p, p.positions ? position_of(p, token) : position, at, c, sn);
-  for (int r0 = slot; r0 - slot < rows; r0 += kRowsInFlight * slots) {
-    Bits<V> x[kRowsInFlight], y[kRowsInFlight];
+  Bits<V> x[kRowsInFlight], y[kRowsInFlight];
+  auto request = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < kRowsInFlight; ++i) {
       const int r = r0 + i * slots;
       x[i] = y[i] = Bits<V>{};
-      if (r < rows && at.live && owned) {
+      if (r < rows && at.live) {
         const uint16_t* in = r < p.q.heads ? qin + r * p.q.in_at.h
                              : r < qk      ? kin + (r - p.q.heads) * p.k.in_at.h
                                            : vin + (r - qk) * ap.v_at.h;
@@ -340,6 +305,49 @@ __global__ void __launch_bounds__(kBlockWaves * 64) cache_append_kernel(AppendPa
         y[i] = load_bits<V>(in + at.second);
       }
     }
+  };
+  // The token's sequence: as many as end at or before it come first.  A lane looks at every per-th end, then at those
+  // between.  The first ends are asked for before the rows, the rest of the look-up goes through scalar loads: it does
+  // not wait for the rows, which are on their way meanwhile.
+  const int per = (ap.sequences + 63) / 64;
+  const int64_t last = int64_t(lane + 1) * per;
+  const int end = ap.cu[last <= ap.sequences ? last : 0];
+  __builtin_amdgcn_sched_barrier(0);
+  request(slot);
+  __builtin_amdgcn_sched_barrier(0);
+  int b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(last <= ap.sequences && end <= token)) * per;
+  for (int j0 = 0, from = b; per > 1 && j0 < per && from + j0 < ap.sequences; j0 += 64) {
+    const int j = from + j0 + lane;
+    const bool in = j < ap.sequences && j0 + lane < per;
+    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && ap.cu[1 + (in ? j : 0)] <= token));
+  }
+  int64_t position = -1;
+  uint16_t *krow = nullptr, *vrow = nullptr;
+  bool owned = false;
+  if (b < ap.sequences) {
+    const int first = load_uniform(ap.cu + b), behind = load_uniform(ap.cu + b + 1);
+    const int64_t keys = load_uniform(ap.kv_lens + b);
+    if (token >= first && token < behind) {
+      owned = true;
+      position = keys - behind + token;
+      const int64_t in_table = position >> ap.page_shift;
+      if (position >= 0 && in_table < ap.max_pages) {
+        const int page = load_uniform(ap.page_table + int64_t(b) * ap.max_pages + in_table);
+        if (page >= 0 && page < ap.num_pages) {
+          const int64_t row = ((int64_t(page) * p.k.heads) << ap.page_shift) + (position & ((1 << ap.page_shift) - 1));
+          krow = ap.k_pages + row * p.D;
+          vrow = ap.v_pages + row * p.D;
+        }
+      }
+    }
+  }
+  const int64_t head_step = int64_t(p.D) << ap.page_shift;
+  float wqa[V], wqb[V], wka[V], wkb[V], c[V], sn[V];
+  load_turn<V>(p, p.positions ? position_of(p, token) : position, at, c, sn);
+  load_weight<BF16, V, INTER>(p.q.weight, p.weight32, at, wqa, wqb);
+  load_weight<BF16, V, INTER>(p.k.weight, p.weight32, at, wka, wkb);
+  for (int r0 = slot; r0 - slot < rows; r0 += kRowsInFlight * slots) {
+    if (r0 != slot) request(r0);
 #pragma unroll
     for (int i = 0; i < kRowsInFlight; ++i) {
       const int r = r0 + i * slots;
@@ -373,137 +381,143 @@ __global__ void __launch_bounds__(kBlockWaves * 64) cache_append_kernel(AppendPa
   }
 }
 
-// Gradients.  A wave walks tokens wave, wave + waves, ...; its lanes keep their dimensions' sums of dw in
-// registers, a block's four waves add theirs up in LDS and write one row of `partial`.
+constexpr int kBackV = 4;  // (of 8: 144 registers and three waves per SIMD for 88 and five, 53 us for 51)
+
+// Gradients of one side: queries (blockIdx.y 0) or keys.  A wave walks the tokens, several at a time where there are
+// fewer heads than it has rows; its lanes keep their dimensions' sums of dw in registers, a block's four waves add theirs
+// up in LDS and write one row of `partial`.  (Both sides in one wave: weights and sums of both, 171 registers and two
+// waves per SIMD; 2 x 4096 tokens, 32 / 8 heads, D=128: 67 us, 51 so, 4.9 TB/s.)
 template <bool BF16, int V, bool INTER>
 __global__ void __launch_bounds__(kBlockWaves * 64) qk_rotary_bwd_kernel(RotaryBwdParams bp) {
   constexpr int kRows = 2;
   const RotaryParams& p = bp.r;
+  const bool is_k = blockIdx.y != 0;
+  const Heads& io = is_k ? p.k : p.q;
+  const uint16_t* xs = is_k ? bp.xk : bp.xq;
+  const RowStrides& x_at = is_k ? bp.xk_at : bp.xq_at;
+  const bool norm = io.weight != nullptr;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slots = 64 / p.lanes_per_row, slot = lane / p.lanes_per_row;
+  int head_slots = 1;  // rows of a token that a wave has at a time
+  while (head_slots < slots && head_slots < io.heads) head_slots <<= 1;
+  const int tokens_at_once = slots / head_slots;
   const Part<V> at = part_of<V, INTER>(lane % p.lanes_per_row, p.D, p.rot);
-  const int rows = p.q.heads + p.k.heads;
-  float wqa[V], wqb[V], wka[V], wkb[V];
-  load_weight<BF16, V, INTER>(p.q.weight, p.weight32, at, wqa, wqb);
-  load_weight<BF16, V, INTER>(p.k.weight, p.weight32, at, wka, wkb);
-  float gq[2][V] = {}, gk[2][V] = {};
-  for (int64_t token = int64_t(blockIdx.x) * kBlockWaves + wv; token < p.tokens; token += int64_t(gridDim.x) * kBlockWaves) {
+  float wa[V], wb[V];
+  load_weight<BF16, V, INTER>(io.weight, p.weight32, at, wa, wb);
+  float gw[2][V] = {};
+  const int64_t stride = int64_t(gridDim.x) * kBlockWaves * tokens_at_once;
+  for (int64_t t0 = (int64_t(blockIdx.x) * kBlockWaves + wv) * tokens_at_once; t0 < p.tokens; t0 += stride) {
+    const int64_t mine = t0 + slot / head_slots;
+    const bool has = mine < p.tokens && at.live;
+    const int64_t token = mine < p.tokens ? mine : p.tokens - 1;
     const int64_t b = token / p.S, s = token - b * p.S;
-    const int64_t q0 = b * p.q.in_at.b + s * p.q.in_at.row, k0 = b * p.k.in_at.b + s * p.k.in_at.row;
-    const int64_t xq0 = b * bp.xq_at.b + s * bp.xq_at.row, xk0 = b * bp.xk_at.b + s * bp.xk_at.row;
-    const int64_t qo = b * p.q.out_at.b + s * p.q.out_at.row, ko = b * p.k.out_at.b + s * p.k.out_at.row;
+    const uint16_t* in = io.in + b * io.in_at.b + s * io.in_at.row;
+    const uint16_t* xin = xs + b * x_at.b + s * x_at.row;
+    uint16_t* out = io.out + b * io.out_at.b + s * io.out_at.row;
     float c[V], sn[V];
     load_turn<V>(p, position_of(p, b * p.pos_b + s), at, c, sn);
-    for (int r0 = slot; r0 - slot < rows; r0 += kRows * slots) {
+    for (int h0 = 0; h0 < io.heads; h0 += kRows * head_slots) {
       Bits<V> dx[kRows], dy[kRows], x[kRows], y[kRows];
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
-        const int r = r0 + i * slots;
-        const bool is_q = r < p.q.heads;
+        const int h = h0 + i * head_slots + (slot & (head_slots - 1));
         dx[i] = dy[i] = x[i] = y[i] = Bits<V>{};
-        if (r < rows && at.live) {
-          const uint16_t* in = is_q ? p.q.in + q0 + r * p.q.in_at.h : p.k.in + k0 + (r - p.q.heads) * p.k.in_at.h;
-          dx[i] = load_bits<V>(in + at.first);
-          dy[i] = load_bits<V>(in + at.second);
-          if ((is_q ? p.q.weight : p.k.weight) != nullptr) {
-            const uint16_t* xin = is_q ? bp.xq + xq0 + r * bp.xq_at.h : bp.xk + xk0 + (r - p.q.heads) * bp.xk_at.h;
-            x[i] = load_bits<V>(xin + at.first);
-            y[i] = load_bits<V>(xin + at.second);
+        if (h < io.heads && has) {
+          dx[i] = load_bits<V>(in + h * io.in_at.h + at.first);
+          dy[i] = load_bits<V>(in + h * io.in_at.h + at.second);
+          if (norm) {
+            x[i] = load_bits<V>(xin + h * x_at.h + at.first);
+            y[i] = load_bits<V>(xin + h * x_at.h + at.second);
           }
         }
       }
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
-        const int r = r0 + i * slots;
-        if (r - slot >= rows) break;
-        const bool is_q = r < p.q.heads, norm = (is_q ? p.q.weight : p.k.weight) != nullptr;
-        float da[V], db[V], a[V], bb[V];
+        if (h0 + i * head_slots >= io.heads) break;  // (the same for all lanes: the sums cross them)
+        const int h = h0 + i * head_slots + (slot & (head_slots - 1));
+        const bool row = h < io.heads && has;
+        float da[V], db[V];
         to_pairs<BF16, V, INTER>(dx[i], dy[i], da, db);
-        to_pairs<BF16, V, INTER>(x[i], y[i], a, bb);
-        float squares = 0.f, dots = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {  // (s carries the sign of the inverse rotation)
           const float ga = __builtin_fmaf(-db[j], sn[j], da[j] * c[j]), gb = __builtin_fmaf(da[j], sn[j], db[j] * c[j]);
           da[j] = ga;
           db[j] = gb;
-          squares = __builtin_fmaf(a[j], a[j], __builtin_fmaf(bb[j], bb[j], squares));
-          const float wa = is_q ? wqa[j] : wka[j], wb = is_q ? wqb[j] : wkb[j];
-          dots = __builtin_fmaf(ga * wa, a[j], __builtin_fmaf(gb * wb, bb[j], dots));
         }
-        squares = row_sum(squares, p.lanes_per_row);
-        dots = row_sum(dots, p.lanes_per_row);
         if (norm) {
+          float a[V], bb[V], squares = 0.f, dots = 0.f;
+          to_pairs<BF16, V, INTER>(x[i], y[i], a, bb);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            squares = __builtin_fmaf(a[j], a[j], __builtin_fmaf(bb[j], bb[j], squares));
+            dots = __builtin_fmaf(da[j] * wa[j], a[j], __builtin_fmaf(db[j] * wb[j], bb[j], dots));
+          }
+          squares = row_sum(squares, p.lanes_per_row);
+          dots = row_sum(dots, p.lanes_per_row);
           const float rs = 1.f / __builtin_sqrtf(squares / float(p.D) + p.eps);
           const float pull = dots * rs * rs / float(p.D);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const float wa = is_q ? wqa[j] : wka[j], wb = is_q ? wqb[j] : wkb[j];
-            const float ta = r < rows ? da[j] * a[j] * rs : 0.f, tb = r < rows ? db[j] * bb[j] * rs : 0.f;
-            gq[0][j] += is_q ? ta : 0.f;
-            gq[1][j] += is_q ? tb : 0.f;
-            gk[0][j] += is_q ? 0.f : ta;
-            gk[1][j] += is_q ? 0.f : tb;
-            da[j] = rs * __builtin_fmaf(-a[j], pull, da[j] * wa);
-            db[j] = rs * __builtin_fmaf(-bb[j], pull, db[j] * wb);
+            gw[0][j] += row ? da[j] * a[j] * rs : 0.f;
+            gw[1][j] += row ? db[j] * bb[j] * rs : 0.f;
+            da[j] = rs * __builtin_fmaf(-a[j], pull, da[j] * wa[j]);
+            db[j] = rs * __builtin_fmaf(-bb[j], pull, db[j] * wb[j]);
           }
         }
-        if (r < rows && at.live) {
-          uint16_t* out = is_q ? p.q.out + qo + r * p.q.out_at.h : p.k.out + ko + (r - p.q.heads) * p.k.out_at.h;
+        if (row) {
           from_pairs<BF16, V, INTER>(da, db, dx[i], dy[i]);
-          store_bits<V>(out + at.first, dx[i]);
-          store_bits<V>(out + at.second, dy[i]);
+          store_bits<V>(out + h * io.out_at.h + at.first, dx[i]);
+          store_bits<V>(out + h * io.out_at.h + at.second, dy[i]);
         }
       }
     }
   }
   if (bp.partial == nullptr) return;
-  __shared__ float sums[kBlockWaves][2][256];
+  __shared__ float sums[kBlockWaves][256];
+#pragma unroll
   for (int j = 0; j < V; ++j)
+#pragma unroll
     for (int h = 0; h < 2; ++h)
-      for (int m = p.lanes_per_row; m < 64; m <<= 1) {
-        gq[h][j] += __shfl_xor(gq[h][j], m);
-        gk[h][j] += __shfl_xor(gk[h][j], m);
-      }
+      for (int m = p.lanes_per_row; m < 64; m <<= 1) gw[h][j] += __shfl_xor(gw[h][j], m);
   if (slot == 0 && at.live) {
+#pragma unroll
     for (int j = 0; j < V; ++j) {
       const int ia = INTER ? at.first + 2 * j : at.first + j, ib = INTER ? ia + 1 : at.second + j;
-      sums[wv][0][ia] = gq[0][j];
-      sums[wv][0][ib] = gq[1][j];
-      sums[wv][1][ia] = gk[0][j];
-      sums[wv][1][ib] = gk[1][j];
+      sums[wv][ia] = gw[0][j];
+      sums[wv][ib] = gw[1][j];
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.D; i += kBlockWaves * 64) {
-    const int which = i >= p.D, d = i - which * p.D;
+  for (int d = threadIdx.x; d < p.D; d += kBlockWaves * 64) {
     float t = 0.f;
-    for (int w = 0; w < kBlockWaves; ++w) t += sums[w][which][d];
-    bp.partial[int64_t(blockIdx.x) * 2 * p.D + i] = t;
+#pragma unroll
+    for (int w = 0; w < kBlockWaves; ++w) t += sums[w][d];
+    bp.partial[(int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * p.D + d] = t;
   }
 }
 
-// dw of 16 dimensions per block: 16 row lanes each, in 64 bits, added up in a fixed order.
+// dw of 16 dimensions per block: 16 row lanes each, in 64 bits, added up in a fixed order.  blockIdx.y: the side.
 __global__ void __launch_bounds__(256) rotary_weight_grad_kernel(const float* partial, int blocks, int D, void* dwq,
                                                                  void* dwk, int weight32, int bf16) {
   __shared__ double sums[16][17];
-  const int d = threadIdx.x & 15, part = threadIdx.x >> 4;
-  const int column = blockIdx.x * 16 + d;
-  double t = 0;
-  if (column < 2 * D)
-    for (int i = part; i < blocks; i += 16) t += double(partial[int64_t(i) * 2 * D + column]);
-  sums[part][d] = t;
-  __syncthreads();
-  if (part != 0 || column >= 2 * D) return;
-  for (int i = 1; i < 16; ++i) t += sums[i][d];
-  const int which = column >= D, at = column - which * D;
-  void* out = which ? dwk : dwq;
+  void* out = blockIdx.y ? dwk : dwq;
   if (out == nullptr) return;
+  const int part = threadIdx.x >> 4, column = blockIdx.x * 16 + (threadIdx.x & 15);
+  double t = 0;
+  if (column < D) {
+#pragma unroll 8
+    for (int i = part; i < blocks; i += 16) t += double(partial[(int64_t(blockIdx.y) * blocks + i) * D + column]);
+  }
+  sums[part][threadIdx.x & 15] = t;
+  __syncthreads();
+  if (part != 0 || column >= D) return;
+  for (int i = 1; i < 16; ++i) t += sums[i][threadIdx.x & 15];
   if (weight32) {
-    static_cast<float*>(out)[at] = float(t);
+    static_cast<float*>(out)[column] = float(t);
   } else if (bf16) {
-    static_cast<uint16_t*>(out)[at] = __builtin_bit_cast(uint16_t, __bf16(float(t)));
+    static_cast<uint16_t*>(out)[column] = __builtin_bit_cast(uint16_t, __bf16(float(t)));
   } else {
-    static_cast<uint16_t*>(out)[at] = __builtin_bit_cast(uint16_t, _Float16(float(t)));
+    static_cast<uint16_t*>(out)[column] = __builtin_bit_cast(uint16_t, _Float16(float(t)));
   }
 }
 
@@ -554,9 +568,9 @@ template <bool BF16, int V, bool INTER>
 void launch_append(const AppendParams& p, unsigned blocks, hipStream_t stream) {
   hipLaunchKernelGGL((cache_append_kernel<BF16, V, INTER>), dim3(blocks), dim3(kBlockWaves * 64), 0, stream, p);
 }
-template <bool BF16, int V, bool INTER>
+template <bool BF16, bool INTER>
 void launch_backward(const RotaryBwdParams& p, unsigned blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((qk_rotary_bwd_kernel<BF16, V, INTER>), dim3(blocks), dim3(kBlockWaves * 64), 0, stream, p);
+  hipLaunchKernelGGL((qk_rotary_bwd_kernel<BF16, kBackV, INTER>), dim3(blocks, 2), dim3(kBlockWaves * 64), 0, stream, p);
 }
 #define OMNI_ROTARY_INSTANCE(launch, bf16, V, inter, ...)                                                   \
   do {                                                                                                      \
@@ -579,7 +593,7 @@ int launched() {
 // Blocks of the backward's first launch, and so rows of its partial sums.
 int backward_blocks(long long tokens) {
   const long long blocks = (tokens + kBlockWaves - 1) / kBlockWaves;
-  return int(blocks < 1024 ? blocks : 1024);
+  return int(blocks < 768 ? blocks : 768);
 }
 
 }  // namespace
@@ -685,20 +699,22 @@ extern "C" int omni_attn_qk_rotary_bwd_gfx950(
   p.table_rows = table_rows;
   p.eps = eps;
   p.sign = -1.f;
-  const int V = vector_width(wide, D, rotary_dim);
+  const bool turn_only = !q_weight_or_null && !k_weight_or_null;
+  const int V = turn_only ? vector_width(wide, D, rotary_dim) : kBackV;
   const bool bf16 = dtype == OMNI_ATTN_DTYPE_BF16;
   deal_rows(p, V, Hq + Hk);
-  if (!q_weight_or_null && !k_weight_or_null) {  // the inverse rotation alone
+  if (turn_only) {  // the inverse rotation alone
     const long long blocks = (p.tokens * p.waves_per_token + kBlockWaves - 1) / kBlockWaves;
     if (blocks > 0x7fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
     OMNI_ROTARY_INSTANCE(launch_forward, bf16, V, interleaved, p, unsigned(blocks), static_cast<hipStream_t>(stream));
     return launched();
   }
   const int blocks = backward_blocks(p.tokens);
-  OMNI_ROTARY_INSTANCE(launch_backward, bf16, V, interleaved, bp, unsigned(blocks), static_cast<hipStream_t>(stream));
+  (bf16 ? (interleaved ? launch_backward<true, true> : launch_backward<true, false>)
+        : (interleaved ? launch_backward<false, true> : launch_backward<false, false>))(bp, unsigned(blocks), static_cast<hipStream_t>(stream));
   if (const int rc = launched()) return rc;
   if (!weights) return OMNI_ATTN_OK;
-  hipLaunchKernelGGL(rotary_weight_grad_kernel, dim3((2 * D + 15) / 16), dim3(256), 0, static_cast<hipStream_t>(stream),
+  hipLaunchKernelGGL(rotary_weight_grad_kernel, dim3((D + 15) / 16, 2), dim3(256), 0, static_cast<hipStream_t>(stream),
                      static_cast<const float*>(workspace), blocks, D, dq_weight_or_null, dk_weight_or_null, weights_f32,
                      int(bf16));
   return launched();
