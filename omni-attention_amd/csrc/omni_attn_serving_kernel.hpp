@@ -60,16 +60,27 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
-__device__ __forceinline__ float wave_sum(float x) {
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
-  return x;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_zero(float x) {  // another lane's x, or 0 where there is none
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
 }
-__device__ __forceinline__ int wave_max(int x) {
-  for (int m = 1; m < 64; m <<= 1) {
-    const int y = __shfl_xor(x, m);
-    x = x > y ? x : y;
-  }
-  return __builtin_amdgcn_readfirstlane(x);
+__device__ __forceinline__ float wave_sum(float x) {
+  x += dpp_zero<0x111, 0xf>(x);
+  x += dpp_zero<0x112, 0xf>(x);
+  x += dpp_zero<0x114, 0xf>(x);
+  x += dpp_zero<0x118, 0xf>(x);
+  x += dpp_zero<0x142, 0xa>(x);
+  x += dpp_zero<0x143, 0xc>(x);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_max(int x) {
+  const int y = __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+  return x > y ? x : y;
+}
+__device__ __forceinline__ int wave_max(int x) {  // x >= 0
+  x = dpp_max<0x118, 0xf>(dpp_max<0x114, 0xf>(dpp_max<0x112, 0xf>(dpp_max<0x111, 0xf>(x))));
+  return __builtin_amdgcn_readlane(dpp_max<0x143, 0xc>(dpp_max<0x142, 0xa>(x)), 63);
 }
 
 struct Sequence {
@@ -99,18 +110,27 @@ __device__ __forceinline__ int tiles_of(const ServeParams& p, const Sequence& s)
 }
 __device__ __forceinline__ int steps_of(int keys) { return (keys + kStepKeys - 1) / kStepKeys; }
 
-// The sequences of a batch: a lane has p.per_lane neighbours, of up to 64 sequences one, which stays in registers.
+// The sequences of a batch: a lane has p.per_lane neighbours.  Up to eight of them stay in registers, asked for together.
 struct Batch {
-  Sequence own;
-  __device__ __forceinline__ Batch(const ServeParams& p, int lane) : own(sequence_of(p, lane)) {}
+  static constexpr int kKept = 8;
+  Sequence own[kKept];
+  __device__ __forceinline__ Batch(const ServeParams& p, int lane) {
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) own[i] = Sequence{0, 0, 0};
+    own[0] = sequence_of(p, lane * p.per_lane);
+    if (p.per_lane > 1) {
+#pragma unroll
+      for (int i = 1; i < kKept; ++i) own[i] = sequence_of(p, i < p.per_lane ? lane * p.per_lane + i : p.B);
+    }
+  }
   // f(sequence) summed over a lane's sequences.
   template <class F>
   __device__ __forceinline__ auto sum(const ServeParams& p, int lane, F&& f) const {
-    auto all = f(own);
+    auto all = f(own[0]);
     if (p.per_lane > 1) {
-      all = f(sequence_of(p, lane * p.per_lane));
-#pragma unroll 4
-      for (int i = 1; i < p.per_lane; ++i) all += f(sequence_of(p, lane * p.per_lane + i));
+#pragma unroll
+      for (int i = 1; i < kKept; ++i) all += f(own[i]);
+      for (int i = kKept; i < p.per_lane; ++i) all += f(sequence_of(p, lane * p.per_lane + i));
     }
     return all;
   }
@@ -130,7 +150,7 @@ __device__ __forceinline__ Place place_of(const ServeParams& p, const Batch& bat
   if (beyond == 0) return Place{{}, -1, __builtin_amdgcn_readlane(end, 63)};
   const int at = __builtin_ctzll(beyond);
   rank -= __builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(mine, at);
-  if (p.per_lane == 1) return Place{pick(batch.own, at), at, rank};
+  if (p.per_lane == 1) return Place{pick(batch.own[0], at), at, rank};
   for (int i0 = 0;; i0 += 64) {  // (one of the lane's sequences has it)
     const int i = i0 + lane;
     const Sequence s = sequence_of(p, i < p.per_lane ? at * p.per_lane + i : p.B);
@@ -198,7 +218,7 @@ __device__ __forceinline__ Unit find_tile(const ServeParams& p, const Batch& bat
     if (at.b < 0) return Unit{{}, 0, 0, at.in, 0, 0, 1, false, false};
     return Unit{at.seq, at.b, tiles_of<M>(p, at.seq) - 1 - at.in, 0, kAll, 0, 1, false, true};
   }
-  const Sequence& s = batch.own;
+  const Sequence& s = batch.own[0];
   const int most = wave_max(s.n > 0 ? steps_of(s.kv) : 0);
   int unit = 0;  // log2 of the steps of a level
   while ((most >> unit) > 15) ++unit;
@@ -1013,7 +1033,7 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
 #pragma unroll
       for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 1, from + STEP, 0, r1, r1);
     }
-    wait_loads();
+    wait_loads_but<NCH>();  // K(1) may be under way
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < KS; ++s)
