@@ -404,6 +404,16 @@ int omni_attn_packed_gfx950(const void* q, const void* k, const void* v, omni_at
                             omni_attn_strides v_at, void* o, float* lse_or_null, const int32_t* cu_seqlens,
                             void* workspace, size_t workspace_bytes, int tokens, int sequences, int Hq, int Hk, int D,
                             int causal, int dtype, float softcap, void* stream);
+/* Gradients of omni_attn_packed_gfx950, from the o and lse that it wrote and dout [tokens, Hq, D] at strides like q's:
+ * dq [tokens, Hq, D], dk and dv [tokens, Hk, D], contiguous, written completely (zeros behind the last sequence).  Two
+ * kernels, nothing added up across workgroups: the same bits every time.  q, k, v and dout are taken to be finite.  The
+ * workspace holds a float per row of q. */
+size_t omni_attn_packed_bwd_workspace_bytes(int tokens, int Hq);
+int omni_attn_packed_bwd_gfx950(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                                const float* lse, omni_attn_strides q_at, omni_attn_strides k_at, omni_attn_strides v_at,
+                                omni_attn_strides dout_at, void* dq, void* dk, void* dv, const int32_t* cu_seqlens,
+                                void* workspace, size_t workspace_bytes, int tokens, int sequences, int Hq, int Hk, int D,
+                                int causal, int dtype, float softcap, void* stream);
 size_t omni_attn_paged_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D, int page_size, int max_pages);
 int omni_attn_paged_gfx950(const void* q, omni_attn_strides q_at, const void* k_pages, const void* v_pages, void* o,
                            float* lse_or_null, const int32_t* page_table, const int32_t* kv_lens,

@@ -52,7 +52,7 @@ RESOURCES_JSON = os.path.join(OBJ, "kernel_resources.json")
 # The backward kernels and the forward with split lists keep scalar values in spare vector lanes here
 # and there (SGPR spills, no memory behind them): for them only scratch memory and spilled vector registers fail the build.
 MIN_WAVES_PER_SIMD = {"fwd_kernel": 2, "fwd_ksplit": 2, "bwd_dq_kernel": 2, "bwd_dq_short": 2, "bwd_dq_ksplit": 2,
-                      "bwd_dkdv_kernel": 2, "bwd_dkdv_split": 2, "fwd_generic_": 2, "serve_tile": 2, "serve_few": 2,
+                      "bwd_dkdv_kernel": 2, "bwd_dkdv_split": 2, "fwd_generic_": 2, "serve_tile": 2, "serve_few": 2, "serve_dq": 2, "serve_dkdv": 2,
                       "qk_rotary_kernel": 3, "cache_append_kernel": 3, "qk_rotary_bwd": 2}
 SGPR_SPILLS_ALLOWED = ("bwd_dq_", "bwd_dkdv_", "fwd_ksplit", "fwd_generic_", "serve_", "qk_rotary_bwd")
 # For the generic kernel scratch memory is what counts.  Forms that read rows at any alignment (E1E) have some: up to 32 columns
@@ -155,6 +155,12 @@ def build_capi(jobs):
         cmds.append([HIPCC] + DEVICE_FLAGS + [
             "-DOMNI_INST_BF16=%d" % bf, "-DOMNI_INST_D=%d" % d,
             "-c", os.path.join(CSRC, "omni_attn_serving_inst.hip"), "-o", obj])
+    for bf, d in INSTANCES:
+        obj = os.path.join(OBJ, "serving_bwd_inst_%s_d%d.o" % ("bf16" if bf else "f16", d))
+        objs.append(obj)
+        cmds.append([HIPCC] + DEVICE_FLAGS + [
+            "-DOMNI_INST_BF16=%d" % bf, "-DOMNI_INST_D=%d" % d,
+            "-c", os.path.join(CSRC, "omni_attn_serving_bwd_inst.hip"), "-o", obj])
     for src in ("omni_attn_capi", "omni_attn_probe", "omni_attn_mask_pack", "omni_attn_mask_build", "omni_attn_fwd_generic",
                 "omni_attn_rotary", "omni_attn_serving"):
         obj = os.path.join(OBJ, src + ".o")

@@ -356,6 +356,68 @@ pybind11::object result(Tensor out, Tensor lse, bool want_lse) {
   return pybind11::cast(std::move(out));
 }
 
+struct Packed {
+  Tensor cu;
+  bool causal = true;
+  double softcap = 0;
+};
+// q, k and v become the tensors the kernel has read (copies where it could not read them in place).
+Tensor attend_packed(Tensor& q, Tensor& k, Tensor& v, const Packed& m, Tensor* lse) {
+  const int64_t T = q.size(0), B = m.cu.size(0) - 1, Hq = q.size(1), Hk = k.size(1), D = q.size(2);
+  const auto f32 = q.options().dtype(torch::kFloat32);
+  if (T == 0 || B == 0) {
+    if (lse) *lse = torch::full({T, Hq}, -std::numeric_limits<float>::infinity(), f32);
+    return torch::zeros({T, Hq, D}, q.options());
+  }
+  q = in_rows(q, 8);
+  k = in_rows(k, 8);
+  v = in_rows(v, 8);
+  Tensor out = torch::empty({T, Hq, D}, q.options()), workspace;
+  if (lse) *lse = torch::empty({T, Hq}, f32);
+  const size_t bytes = omni_attn_packed_workspace_bytes(int(T), int(B), int(Hq), int(Hk), int(D));
+  if (bytes) workspace = torch::empty({int64_t((bytes + 3) / 4)}, f32);
+  const int rc = omni_attn_packed_gfx950(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides_of(q), strides_of(k), strides_of(v),
+                                         out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr, m.cu.data_ptr<int32_t>(),
+                                         bytes ? workspace.data_ptr() : nullptr, bytes, int(T), int(B), int(Hq), int(Hk), int(D),
+                                         m.causal, dtype_of(q), float(m.softcap), stream_of(q));
+  if (rc != OMNI_ATTN_OK) fail(rc);
+  return out;
+}
+
+class PackedFunction : public torch::autograd::Function<PackedFunction> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, Tensor q, Tensor k, Tensor v, const Packed& m) {
+    Tensor lse;
+    Tensor out = attend_packed(q, k, v, m, &lse);
+    ctx->save_for_backward({q, k, v, out, lse, m.cu});
+    ctx->saved_data["causal"] = m.causal;
+    ctx->saved_data["softcap"] = m.softcap;
+    ctx->mark_non_differentiable({lse});
+    return {out, lse};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (at::GradMode::is_enabled())
+      throw std::runtime_error("omni_attention_packed: gradients of its gradients are not implemented");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &cu = saved[5];
+    const int64_t T = q.size(0), B = cu.size(0) - 1, Hq = q.size(1), Hk = k.size(1), D = q.size(2);
+    c10::DeviceGuard guard(q.device());
+    if (T == 0 || B == 0) return {torch::zeros_like(q), torch::zeros_like(k), torch::zeros_like(v), Tensor()};
+    const Tensor dout = in_rows(grads[0], 8);
+    Tensor dq = torch::empty({T, Hq, D}, q.options()), dk = torch::empty({T, Hk, D}, q.options()), dv = torch::empty({T, Hk, D}, q.options());
+    const size_t bytes = omni_attn_packed_bwd_workspace_bytes(int(T), int(Hq));
+    Tensor workspace = torch::empty({int64_t(bytes / 4)}, lse.options());
+    const int rc = omni_attn_packed_bwd_gfx950(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), strides_of(q), strides_of(k),
+        strides_of(v), strides_of(dout), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu.data_ptr<int32_t>(), workspace.data_ptr(),
+        bytes, int(T), int(B), int(Hq), int(Hk), int(D), ctx->saved_data["causal"].toBool(), dtype_of(q),
+        float(ctx->saved_data["softcap"].toDouble()), stream_of(q));
+    if (rc != OMNI_ATTN_OK) fail(rc);
+    return {dq, dk, dv, Tensor()};
+  }
+};
+
 pybind11::object omni_attn_packed(Tensor q, Tensor k, Tensor v, Tensor cu, bool causal, double softcap, bool want_lse) {
   check_operand(q, "query", q);
   check_operand(k, "key", q);
@@ -366,31 +428,16 @@ pybind11::object omni_attn_packed(Tensor q, Tensor k, Tensor v, Tensor cu, bool 
   check_int32(cu, "cu_seqlens", q, 1);
   require(cu.size(0) >= 1, "cu_seqlens must have one entry more than there are sequences");
   check_softcap(softcap);
-  check_no_grad({q, k, v}, "omni_attention_packed");
-  at::NoGradGuard no_grad;
+  require((cu.size(0) - 1) * k.size(1) <= 0x3fffffff, "too many sequences");
   c10::DeviceGuard guard(q.device());
-  const int64_t T = q.size(0), B = cu.size(0) - 1, Hq = q.size(1), Hk = k.size(1), D = q.size(2);
-  require(B * Hk <= 0x3fffffff, "too many sequences");
-  const bool some = T != 0 && B != 0;
-  Tensor out = some ? torch::empty({T, Hq, D}, q.options()) : torch::zeros({T, Hq, D}, q.options()), lse;
-  if (want_lse) {
-    const auto f32 = q.options().dtype(torch::kFloat32);
-    lse = some ? torch::empty({T, Hq}, f32) : torch::full({T, Hq}, -std::numeric_limits<float>::infinity(), f32);
+  const Packed m{cu.contiguous(), causal, softcap};
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+    auto out = PackedFunction::apply(q, k, v, m);
+    return result(std::move(out[0]), std::move(out[1]), want_lse);
   }
-  if (some) {
-    q = in_rows(q, 8);
-    k = in_rows(k, 8);
-    v = in_rows(v, 8);
-    cu = cu.contiguous();
-    const size_t bytes = omni_attn_packed_workspace_bytes(int(T), int(B), int(Hq), int(Hk), int(D));
-    Tensor workspace;
-    if (bytes) workspace = torch::empty({int64_t((bytes + 3) / 4)}, q.options().dtype(torch::kFloat32));
-    const int rc = omni_attn_packed_gfx950(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides_of(q), strides_of(k), strides_of(v),
-                                           out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, cu.data_ptr<int32_t>(),
-                                           bytes ? workspace.data_ptr() : nullptr, bytes, int(T), int(B), int(Hq), int(Hk),
-                                           int(D), causal, dtype_of(q), float(softcap), stream_of(q));
-    if (rc != OMNI_ATTN_OK) fail(rc);
-  }
+  at::NoGradGuard no_grad;
+  Tensor lse;
+  Tensor out = attend_packed(q, k, v, m, want_lse ? &lse : nullptr);
   return result(std::move(out), std::move(lse), want_lse);
 }
 

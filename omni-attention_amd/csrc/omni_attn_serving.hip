@@ -1,5 +1,6 @@
 // C ABI of the attention of packed sequences: checks, the plan of the launch, instance dispatch.
 #include "../../include/omni_attn_gfx950.h"
+#include "omni_attn_serving_bwd_kernel.hpp"
 #include "omni_attn_serving_kernel.hpp"
 #include "omni_attn_serving_plan.hpp"
 
@@ -18,6 +19,15 @@ template <> int launch_serve<false, 128>(const ServeParams&, int, unsigned, hipS
 template <> int launch_serve<true, 32>(const ServeParams&, int, unsigned, hipStream_t);
 template <> int launch_serve<true, 64>(const ServeParams&, int, unsigned, hipStream_t);
 template <> int launch_serve<true, 128>(const ServeParams&, int, unsigned, hipStream_t);
+
+template <bool BF16, int D>
+int launch_serve_bwd(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
+template <> int launch_serve_bwd<false, 32>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
+template <> int launch_serve_bwd<false, 64>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
+template <> int launch_serve_bwd<false, 128>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
+template <> int launch_serve_bwd<true, 32>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
+template <> int launch_serve_bwd<true, 64>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
+template <> int launch_serve_bwd<true, 128>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
 
 namespace {
 
@@ -141,6 +151,96 @@ extern "C" int omni_attn_packed_gfx950(const void* q, const void* k, const void*
   p.Hk = Hk;
   p.causal = causal != 0;
   return serve(p, Hq, D, workspace, workspace_bytes, dtype, softcap, stream);
+}
+
+extern "C" size_t omni_attn_packed_bwd_workspace_bytes(int tokens, int Hq) {
+  return tokens <= 0 || Hq <= 0 ? 0 : size_t(tokens) * size_t(Hq) * sizeof(float);
+}
+
+extern "C" int omni_attn_packed_bwd_gfx950(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                                           const float* lse, omni_attn_strides q_at, omni_attn_strides k_at,
+                                           omni_attn_strides v_at, omni_attn_strides dout_at, void* dq, void* dk, void* dv,
+                                           const int32_t* cu_seqlens, void* workspace, size_t workspace_bytes, int tokens,
+                                           int sequences, int Hq, int Hk, int D, int causal, int dtype, float softcap,
+                                           void* stream) {
+  using namespace omni_attn;
+  if (!q || !k || !v || !o || !dout || !lse || !dq || !dk || !dv || !cu_seqlens) return OMNI_ATTN_ERR_NULL_POINTER;
+  for (const void* x : {q, k, v, o, dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
+    if (misaligned(x, 16)) return OMNI_ATTN_ERR_MISALIGNED;
+  if (misaligned(lse, 4) || misaligned(cu_seqlens, 4) || misaligned(workspace, 4)) return OMNI_ATTN_ERR_MISALIGNED;
+  if (const int rc = check_sizes(tokens, sequences, Hq, Hk, D)) return rc;
+  const int G = Hq / Hk;
+  for (const omni_attn_strides* at : {&q_at, &k_at, &v_at, &dout_at}) {
+    if (const int rc = check_rows(*at)) return rc;
+    // (the rows of a step, 64 of them, lie within 3 GiB)
+    if (at->head > (1LL << 30) || 66 * at->row + G * at->head > 0x5f000000LL) return OMNI_ATTN_ERR_TOO_LARGE;
+  }
+  if (!(softcap >= 0.f) || std::isinf(softcap)) return OMNI_ATTN_ERR_BAD_SHAPE;
+  if (dtype != OMNI_ATTN_DTYPE_F16 && dtype != OMNI_ATTN_DTYPE_BF16) return OMNI_ATTN_ERR_UNSUPPORTED_DTYPE;
+  if (!workspace || workspace_bytes < omni_attn_packed_bwd_workspace_bytes(tokens, Hq)) return OMNI_ATTN_ERR_WORKSPACE;
+  ServeBwdParams b{};
+  ServeParams& p = b.s;
+  int cus = 0;
+  if (const int e = device_units(&p.n_xcd, &cus)) {
+    record_hip_error(e);
+    return OMNI_ATTN_ERR_LAUNCH;
+  }
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.q_row = q_at.row;
+  p.q_head = q_at.head;
+  p.k_at = {0, k_at.head, uint32_t(k_at.row)};
+  p.v_at = {0, v_at.head, uint32_t(v_at.row)};
+  p.o = static_cast<uint16_t*>(dq);  // (the rows that are cleared)
+  p.cu = cu_seqlens;
+  p.B = sequences;
+  p.T = tokens;
+  p.Hk = Hk;
+  p.per_lane = (sequences + 63) / 64;
+  p.heads = fast_div(uint32_t(Hk));
+  p.causal = causal != 0;
+  p.softcap = softcap;
+  p.cap_c2 = softcap > 0.f ? float(2.0 * 1.4426950408889634 / (std::sqrt(double(D)) * double(softcap))) : 0.f;
+  p.sl2 = softcap > 0.f ? float(1.4426950408889634) : float(1.4426950408889634 / std::sqrt(double(D)));
+  b.dout = static_cast<const uint16_t*>(dout);
+  b.dout_row = dout_at.row;
+  b.dout_head = dout_at.head;
+  b.out = static_cast<const uint16_t*>(o);
+  b.lse = lse;
+  b.delta = static_cast<float*>(workspace);
+  b.dq = static_cast<uint16_t*>(dq);
+  b.dk = static_cast<uint16_t*>(dk);
+  b.dv = static_cast<uint16_t*>(dv);
+  b.G = G;
+  b.group = fast_div(uint32_t(G));
+  b.scale = float(1.0 / std::sqrt(double(D)));
+  b.cap_l2 = float(1.4426950408889634 * double(softcap));
+  // one unit more than there can be tiles, of rows and of keys: it clears what lies behind the last sequence
+  ServeBwdParams rows = b, keys = b;
+  rows.s.G = G;
+  rows.s.group = b.group;
+  keys.s.G = 1;
+  keys.s.group = fast_div(1);
+  const int64_t row_units = int64_t(tokens) * G / 128 + sequences + 1, key_units = int64_t(tokens) / 128 + sequences + 1;
+  const int64_t row_blocks = serve_blocks(row_units, Hk, p.n_xcd), key_blocks = serve_blocks(key_units, Hk, p.n_xcd);
+  if (row_blocks > 0x7fffffffLL || key_blocks > 0x7fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
+  rows.s.units = int(row_units);
+  keys.s.units = int(key_units);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool bf = dtype == OMNI_ATTN_DTYPE_BF16;
+  const unsigned nr = unsigned(row_blocks), nk = unsigned(key_blocks);
+  int e;
+  switch (D) {
+    case 32: e = bf ? launch_serve_bwd<true, 32>(rows, nr, keys, nk, s) : launch_serve_bwd<false, 32>(rows, nr, keys, nk, s); break;
+    case 64: e = bf ? launch_serve_bwd<true, 64>(rows, nr, keys, nk, s) : launch_serve_bwd<false, 64>(rows, nr, keys, nk, s); break;
+    default: e = bf ? launch_serve_bwd<true, 128>(rows, nr, keys, nk, s) : launch_serve_bwd<false, 128>(rows, nr, keys, nk, s); break;
+  }
+  if (e != 0) {
+    record_hip_error(e);
+    return OMNI_ATTN_ERR_LAUNCH;
+  }
+  return OMNI_ATTN_OK;
 }
 
 extern "C" int omni_attn_paged_gfx950(const void* q, omni_attn_strides q_at, const void* k_pages, const void* v_pages,

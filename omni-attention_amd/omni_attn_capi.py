@@ -39,6 +39,8 @@ EXPORTED_SYMBOLS = (
     "omni_attn_cache_append_gfx950",
     "omni_attn_packed_workspace_bytes",
     "omni_attn_packed_gfx950",
+    "omni_attn_packed_bwd_workspace_bytes",
+    "omni_attn_packed_bwd_gfx950",
     "omni_attn_paged_workspace_bytes",
     "omni_attn_paged_gfx950",
     "omni_attn_mfma_peak_probe_gfx950",

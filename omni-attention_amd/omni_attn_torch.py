@@ -889,8 +889,8 @@ def omni_attention_packed(query: Tensor, key: Tensor, value: Tensor, cu_seqlens:
     (head h reads key head h // (heads // kv_heads)), fp16 / bf16, head_dim 32, 64 or 128; cu_seqlens as in
     ``omni_cache_append``.  ``causal``: a token attends itself and those before it; else its whole sequence.  ``softcap``
     as in ``omni_attention``.  Returns [tokens, heads, head_dim], with ``return_lse`` also the fp32 logsumexp
-    [tokens, heads].  Tokens behind the last sequence get zeros (-inf).  Not differentiable; for training, padded
-    batches go through ``omni_attention``."""
+    [tokens, heads].  Tokens behind the last sequence get zeros (-inf).  Differentiable in query, key and value (not
+    through the logsumexp)."""
     return _load_extension().omni_attn_packed(query, key, value, cu_seqlens, bool(causal), float(softcap), bool(return_lse))
 
 
