@@ -21,13 +21,13 @@ template <> int launch_serve<true, 64>(const ServeParams&, int, unsigned, hipStr
 template <> int launch_serve<true, 128>(const ServeParams&, int, unsigned, hipStream_t);
 
 template <bool BF16, int D>
-int launch_serve_bwd(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
-template <> int launch_serve_bwd<false, 32>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
-template <> int launch_serve_bwd<false, 64>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
-template <> int launch_serve_bwd<false, 128>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
-template <> int launch_serve_bwd<true, 32>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
-template <> int launch_serve_bwd<true, 64>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
-template <> int launch_serve_bwd<true, 128>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, hipStream_t);
+int launch_serve_bwd(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, int, hipStream_t);
+template <> int launch_serve_bwd<false, 32>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, int, hipStream_t);
+template <> int launch_serve_bwd<false, 64>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, int, hipStream_t);
+template <> int launch_serve_bwd<false, 128>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, int, hipStream_t);
+template <> int launch_serve_bwd<true, 32>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, int, hipStream_t);
+template <> int launch_serve_bwd<true, 64>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, int, hipStream_t);
+template <> int launch_serve_bwd<true, 128>(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, int, hipStream_t);
 
 namespace {
 
@@ -229,12 +229,17 @@ extern "C" int omni_attn_packed_bwd_gfx950(const void* q, const void* k, const v
   keys.s.units = int(key_units);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool bf = dtype == OMNI_ATTN_DTYPE_BF16;
+  // Two groups of waves share a tile of keys where query heads share key heads (a tile then has the rows of all of them,
+  // and its walk is what a launch ends with: 12 prompts of 128 - 3020 tokens, 32 / 8 heads, D=128, gradients 815 us with
+  // one group, 608 with two; 2 x 4096 tokens 1185 and 980), or where there are few tiles; else one (2 x 4096 tokens, 32 /
+  // 32 heads 990 us, 1034 with two; 4 x 2048, 16 / 16, D=64 182 and 201).
+  const int groups = G > 1 || key_units * Hk <= 2 * cus ? 2 : 1;
   const unsigned nr = unsigned(row_blocks), nk = unsigned(key_blocks);
   int e;
   switch (D) {
-    case 32: e = bf ? launch_serve_bwd<true, 32>(rows, nr, keys, nk, s) : launch_serve_bwd<false, 32>(rows, nr, keys, nk, s); break;
-    case 64: e = bf ? launch_serve_bwd<true, 64>(rows, nr, keys, nk, s) : launch_serve_bwd<false, 64>(rows, nr, keys, nk, s); break;
-    default: e = bf ? launch_serve_bwd<true, 128>(rows, nr, keys, nk, s) : launch_serve_bwd<false, 128>(rows, nr, keys, nk, s); break;
+    case 32: e = bf ? launch_serve_bwd<true, 32>(rows, nr, keys, nk, groups, s) : launch_serve_bwd<false, 32>(rows, nr, keys, nk, groups, s); break;
+    case 64: e = bf ? launch_serve_bwd<true, 64>(rows, nr, keys, nk, groups, s) : launch_serve_bwd<false, 64>(rows, nr, keys, nk, groups, s); break;
+    default: e = bf ? launch_serve_bwd<true, 128>(rows, nr, keys, nk, groups, s) : launch_serve_bwd<false, 128>(rows, nr, keys, nk, groups, s); break;
   }
   if (e != 0) {
     record_hip_error(e);

@@ -13,7 +13,7 @@ namespace omni_attn {
 namespace {
 
 template <auto Kernel>
-int launch(const ServeBwdParams& p, unsigned blocks, size_t lds, hipStream_t stream) {
+int launch(const ServeBwdParams& p, unsigned blocks, unsigned threads, size_t lds, hipStream_t stream) {
   static std::atomic<bool> lds_limit_set[kMaxDevices];
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
@@ -26,25 +26,30 @@ int launch(const ServeBwdParams& p, unsigned blocks, size_t lds, hipStream_t str
   }
   ServeBwdParams params = p;
   void* args[] = {&params};
-  return int(hipLaunchKernel(reinterpret_cast<const void*>(Kernel), dim3(blocks), dim3(256), args, lds, stream));
+  return int(hipLaunchKernel(reinterpret_cast<const void*>(Kernel), dim3(blocks), dim3(threads), args, lds, stream));
 }
 
 }  // namespace
 
 template <bool BF16, int D>
-int launch_serve_bwd(const ServeBwdParams& dq, unsigned dq_blocks, const ServeBwdParams& dkdv, unsigned dkdv_blocks, hipStream_t stream);
+int launch_serve_bwd(const ServeBwdParams& dq, unsigned dq_blocks, const ServeBwdParams& dkdv, unsigned dkdv_blocks, int groups,
+                     hipStream_t stream);
 
+// groups: of four waves, that share a tile of keys.
 template <>
 int launch_serve_bwd<OMNI_INST_BF16 != 0, OMNI_INST_D>(const ServeBwdParams& dq, unsigned dq_blocks, const ServeBwdParams& dkdv,
-                                                       unsigned dkdv_blocks, hipStream_t stream) {
+                                                       unsigned dkdv_blocks, int groups, hipStream_t stream) {
   constexpr bool BF = OMNI_INST_BF16 != 0;
   constexpr int D = OMNI_INST_D;
   const bool cap = dq.s.softcap > 0.f;
-  const int e = cap ? launch<serve_dq_kernel<BF, D, true>>(dq, dq_blocks, kServeDqLdsBytes<D>, stream)
-                    : launch<serve_dq_kernel<BF, D, false>>(dq, dq_blocks, kServeDqLdsBytes<D>, stream);
+  const int e = cap ? launch<serve_dq_kernel<BF, D, true>>(dq, dq_blocks, 256, kServeDqLdsBytes<D>, stream)
+                    : launch<serve_dq_kernel<BF, D, false>>(dq, dq_blocks, 256, kServeDqLdsBytes<D>, stream);
   if (e != 0) return e;
-  return cap ? launch<serve_dkdv_kernel<BF, D, true>>(dkdv, dkdv_blocks, kServeDkdvLdsBytes<D>, stream)
-             : launch<serve_dkdv_kernel<BF, D, false>>(dkdv, dkdv_blocks, kServeDkdvLdsBytes<D>, stream);
+  if (groups == 2)
+    return cap ? launch<serve_dkdv_kernel<BF, D, true, 2>>(dkdv, dkdv_blocks, 512, kServeDkdvLdsBytes<D, 2>, stream)
+               : launch<serve_dkdv_kernel<BF, D, false, 2>>(dkdv, dkdv_blocks, 512, kServeDkdvLdsBytes<D, 2>, stream);
+  return cap ? launch<serve_dkdv_kernel<BF, D, true, 1>>(dkdv, dkdv_blocks, 256, kServeDkdvLdsBytes<D, 1>, stream)
+             : launch<serve_dkdv_kernel<BF, D, false, 1>>(dkdv, dkdv_blocks, 256, kServeDkdvLdsBytes<D, 1>, stream);
 }
 
 }  // namespace omni_attn

@@ -38,7 +38,9 @@ constexpr size_t kServeDqLdsBytes = size_t(2) * 2 * kStepKeys * D * 2;
 template <int D>
 constexpr int kDkdvStep = D == 128 ? 32 : 64;
 template <int D>
-constexpr size_t kServeDkdvLdsBytes = size_t(2) * (2 * kDkdvStep<D> * D * 2 + 2 * kDkdvStep<D> * 4) + (D == 128 ? 128 * D * 2 : 0);
+constexpr size_t kDkdvGroupBytes = size_t(2) * (2 * kDkdvStep<D> * D * 2 + 2 * kDkdvStep<D> * 4);  // two sets of tiles
+template <int D, int KG>
+constexpr size_t kServeDkdvLdsBytes = KG * kDkdvGroupBytes<D> + (D == 128 ? 128 * D * 2 : 0);
 
 // 32 rows of a wave, transposed accumulators x factor, as whole rows; at(row): where a row goes, null: nowhere.
 template <bool BF16, int D, class At>
@@ -185,15 +187,17 @@ __global__ void __launch_bounds__(256, 2) serve_dq_kernel(const ServeBwdParams b
   });
 }
 
-template <bool BF16, int D, bool CAP>
-__global__ void __launch_bounds__(256, 2) serve_dkdv_kernel(const ServeBwdParams b) {
+// KG groups of four waves share the rows of a tile (group i takes the steps i, i + KG, ... of its walk) and add up at the
+// end.
+template <bool BF16, int D, bool CAP, int KG>
+__global__ void __launch_bounds__(256 * KG, 2) serve_dkdv_kernel(const ServeBwdParams b) {
   constexpr int M = 128, STEP = kDkdvStep<D>, KS = D / 16, DT = D / 32, TILE = STEP * D, CPR = D / 8;
   constexpr uint32_t SET = 2u * TILE * 2u + 2u * STEP * 4u;  // Q, dO, -LSE, -delta of a step
   const ServeParams& p = b.s;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
-  const uint32_t lds = lds_offset_of(lds_raw);
-  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c = lane & 31;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x & 255, lane = tid & 63, g = lane >> 5, c = lane & 31;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 8));
+  const uint32_t lds = lds_offset_of(lds_raw) + uint32_t(kg) * uint32_t(kDkdvGroupBytes<D>);
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(256, 2) serve_dkdv_kernel(const ServeBwdParams
     int used = p.cu[p.B];
     used = used < 0 ? 0 : used;
     for (int64_t t = int64_t(used) + (rank - u.step0); t < p.T; t += p.units - u.step0)
-      for (int i = tid; i < D / 8; i += 256) {
+      for (int i = threadIdx.x; i < D / 8; i += 256 * KG) {
         const int64_t at = (t * p.Hk + head) * D + i * 8;
         *reinterpret_cast<u32x4_t*>(b.dk + at) = u32x4_t{0u, 0u, 0u, 0u};
         *reinterpret_cast<u32x4_t*>(b.dv + at) = u32x4_t{0u, 0u, 0u, 0u};
@@ -219,7 +223,7 @@ __global__ void __launch_bounds__(256, 2) serve_dkdv_kernel(const ServeBwdParams
 
   constexpr bool V_IN_LDS = D == 128;
   u32x4_t kf[KS], vf[V_IN_LDS ? 1 : KS];
-  const uint32_t own_v = lds + 2u * SET + uint32_t(w) * (32u * D * 2u);
+  const uint32_t own_v = lds_offset_of(lds_raw) + uint32_t(KG * kDkdvGroupBytes<D>) + uint32_t(w) * (32u * D * 2u);  // (of both groups)
   {
     const int64_t t = int64_t(u.seq.first) + (key < n ? key : n - 1);
     const uint16_t* k = p.k + t * p.k_at.row + head * p.k_at.h;
@@ -239,8 +243,8 @@ __global__ void __launch_bounds__(256, 2) serve_dkdv_kernel(const ServeBwdParams
   // do their LSE and delta: they add nothing.
   constexpr int ROW_STRIDE = 256 / CPR, NCH = STEP / ROW_STRIDE;
   constexpr uint32_t kNowhere = 0xc0000000u, kSpan = 0xbfffffffu;  // behind the resources; a step's rows lie within 3 GiB
-  auto issue = [&](int it) {
-    const uint32_t at = lds + uint32_t(it & 1) * SET;
+  auto issue = [&](int it, int set) {
+    const uint32_t at = lds + uint32_t(set) * SET;
     const int r0 = it * STEP, tok0 = int(divide(uint32_t(r0), b.group));
     const int64_t t0 = int64_t(u.seq.first) + tok0;
     const i32x4_t rq = make_buffer_resource(p.q + t0 * p.q_row + int64_t(head * b.G) * p.q_head, kSpan);
@@ -269,12 +273,15 @@ __global__ void __launch_bounds__(256, 2) serve_dkdv_kernel(const ServeBwdParams
   const uint32_t row_lane = bwd_row_lane<D>(g, c), tr_lane = bwd_tr_lane<D>(g, c, 0);
   const float to_start = CAP ? -1.4426950408889634f : -1.4426950408889634f / p.sl2;
   const int key_rows = p.causal ? key * b.G : 0;  // the first row that attends the lane's key
-  issue(step_first);
-  for (int it = step_first; it < nsteps; ++it) {
+  if (step_first + kg < nsteps) issue(step_first + kg, 0);
+  int set = 0;
+  for (int it0 = step_first; it0 < nsteps; it0 += KG, set ^= 1) {
+    const int it = it0 + kg;
     wait_loads();
     __syncthreads();
-    if (it + 1 < nsteps) issue(it + 1);
-    const uint32_t tQ = lds + uint32_t(it & 1) * SET, tD = tQ + TILE * 2u, stats = tD + TILE * 2u;
+    if (it + KG < nsteps) issue(it + KG, set ^ 1);
+    if (KG > 1 && it >= nsteps) break;  // (the last round of the second group: no barrier of the walk comes behind it)
+    const uint32_t tQ = lds + uint32_t(set) * SET, tD = tQ + TILE * 2u, stats = tD + TILE * 2u;
     const int r0 = it * STEP;
     const bool whole = r0 >= whole_from;
 #pragma unroll 1
@@ -346,16 +353,51 @@ __global__ void __launch_bounds__(256, 2) serve_dkdv_kernel(const ServeBwdParams
           dk[dt] = mfma_32x32x16<BF16>(lds_tr_frag<D>(tQ + tr_lane, 64u * dt, (32u * t + 16u * s2) * D * 2u), pb[s2], dk[dt]);
     }
   }
-  __syncthreads();
-  uint16_t* stage = reinterpret_cast<uint16_t*>(lds_raw) + w * 32 * D;
   const auto place = [&](uint16_t* base) {
     return [=](int r) -> uint16_t* {
       return key0 + r < n ? base + ((int64_t(u.seq.first) + key0 + r) * p.Hk + head) * D : nullptr;
     };
   };
-  serve_store_grad<BF16, D>(dk, b.scale, stage, lane, place(b.dk));
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wave stages both in one place)
-  serve_store_grad<BF16, D>(dv, 1.f, stage, lane, place(b.dv));
+  uint16_t* stage = reinterpret_cast<uint16_t*>(lds_raw) + (4 * kg + w) * 32 * D;
+  if constexpr (KG == 1) {
+    __syncthreads();
+    serve_store_grad<BF16, D>(dk, b.scale, stage, lane, place(b.dk));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wave stages both in one place)
+    serve_store_grad<BF16, D>(dv, 1.f, stage, lane, place(b.dv));
+    return;
+  }
+  // The first group gets the other's dK and stores it, the second one dV.
+  constexpr int PIECES = DT * 4;  // 4-register pieces of a lane's sums
+  static_assert(size_t(4) * 64 * PIECES * 16 <= 2 * kDkdvGroupBytes<D> && KG <= 2, "the tiles' place holds the sums of four waves");
+  auto piece_at = [&](int piece) { return reinterpret_cast<f32x4_t*>(lds_raw) + (w * PIECES + piece) * 64 + lane; };
+  auto give = [&](const f32x16_t (&x)[DT]) {
+    static_for<PIECES>([&](auto pc) {
+      constexpr int i = decltype(pc)::value, dt = i / 4, r = 4 * (i % 4);
+      *piece_at(i) = f32x4_t{x[dt][r], x[dt][r + 1], x[dt][r + 2], x[dt][r + 3]};
+    });
+  };
+  auto take = [&](f32x16_t (&x)[DT]) {
+    static_for<PIECES>([&](auto pc) {
+      constexpr int i = decltype(pc)::value, dt = i / 4, r = 4 * (i % 4);
+      const f32x4_t y = *piece_at(i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[dt][r + j] += y[j];
+    });
+  };
+  __syncthreads();
+  if (kg == 1) give(dk);
+  __syncthreads();
+  if (kg == 0) take(dk);
+  __syncthreads();
+  if (kg == 0) give(dv);
+  __syncthreads();
+  if (kg == 1) take(dv);
+  __syncthreads();
+  if (kg == 0) {
+    serve_store_grad<BF16, D>(dk, b.scale, stage, lane, place(b.dk));
+  } else {
+    serve_store_grad<BF16, D>(dv, 1.f, stage, lane, place(b.dv));
+  }
 }
 
 }  // namespace omni_attn
