@@ -12,13 +12,13 @@ namespace omni_attn {
 int device_units(int* n_xcd, int* cus);
 
 template <bool BF16, int D>
-int launch_serve(const ServeParams& p, int waves, unsigned blocks, hipStream_t stream);
-template <> int launch_serve<false, 32>(const ServeParams&, int, unsigned, hipStream_t);
-template <> int launch_serve<false, 64>(const ServeParams&, int, unsigned, hipStream_t);
-template <> int launch_serve<false, 128>(const ServeParams&, int, unsigned, hipStream_t);
-template <> int launch_serve<true, 32>(const ServeParams&, int, unsigned, hipStream_t);
-template <> int launch_serve<true, 64>(const ServeParams&, int, unsigned, hipStream_t);
-template <> int launch_serve<true, 128>(const ServeParams&, int, unsigned, hipStream_t);
+int launch_serve(const ServeParams& p, int rows, int waves, unsigned blocks, hipStream_t stream);
+template <> int launch_serve<false, 32>(const ServeParams&, int, int, unsigned, hipStream_t);
+template <> int launch_serve<false, 64>(const ServeParams&, int, int, unsigned, hipStream_t);
+template <> int launch_serve<false, 128>(const ServeParams&, int, int, unsigned, hipStream_t);
+template <> int launch_serve<true, 32>(const ServeParams&, int, int, unsigned, hipStream_t);
+template <> int launch_serve<true, 64>(const ServeParams&, int, int, unsigned, hipStream_t);
+template <> int launch_serve<true, 128>(const ServeParams&, int, int, unsigned, hipStream_t);
 
 template <bool BF16, int D>
 int launch_serve_bwd(const ServeBwdParams&, unsigned, const ServeBwdParams&, unsigned, int, hipStream_t);
@@ -78,8 +78,8 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
     if (!workspace || workspace_bytes < plan.workspace_bytes(p.T, p.Hk, D)) return OMNI_ATTN_ERR_WORKSPACE;
     if (misaligned(workspace, 16)) return OMNI_ATTN_ERR_MISALIGNED;
     p.sums = static_cast<float*>(workspace);
-    p.stats = p.sums + plan.units * p.Hk * plan.rows() * D;
-    p.joins = reinterpret_cast<int32_t*>(p.stats + plan.units * p.Hk * plan.rows() * 2);
+    p.stats = p.sums + plan.units * p.Hk * plan.rows * D;
+    p.joins = reinterpret_cast<int32_t*>(p.stats + plan.units * p.Hk * plan.rows * 2);
   }
   p.softcap = softcap;
   p.cap_c2 = softcap > 0.f ? float(2.0 * 1.4426950408889634 / (std::sqrt(double(D)) * double(softcap))) : 0.f;
@@ -89,9 +89,9 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
   const unsigned n = unsigned(blocks);
   int e;
   switch (D) {
-    case 32: e = bf ? launch_serve<true, 32>(p, plan.waves, n, s) : launch_serve<false, 32>(p, plan.waves, n, s); break;
-    case 64: e = bf ? launch_serve<true, 64>(p, plan.waves, n, s) : launch_serve<false, 64>(p, plan.waves, n, s); break;
-    default: e = bf ? launch_serve<true, 128>(p, plan.waves, n, s) : launch_serve<false, 128>(p, plan.waves, n, s); break;
+    case 32: e = bf ? launch_serve<true, 32>(p, plan.rows, plan.waves, n, s) : launch_serve<false, 32>(p, plan.rows, plan.waves, n, s); break;
+    case 64: e = bf ? launch_serve<true, 64>(p, plan.rows, plan.waves, n, s) : launch_serve<false, 64>(p, plan.rows, plan.waves, n, s); break;
+    default: e = bf ? launch_serve<true, 128>(p, plan.rows, plan.waves, n, s) : launch_serve<false, 128>(p, plan.rows, plan.waves, n, s); break;
   }
   if (e != 0) {
     record_hip_error(e);

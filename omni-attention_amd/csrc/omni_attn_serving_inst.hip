@@ -33,19 +33,22 @@ int launch(const ServeParams& p, unsigned blocks, unsigned threads, size_t lds, 
 }  // namespace
 
 template <bool BF16, int D>
-int launch_serve(const ServeParams& p, int waves, unsigned blocks, hipStream_t stream);
+int launch_serve(const ServeParams& p, int rows, int waves, unsigned blocks, hipStream_t stream);
 
-// waves: 128 rows and four waves per unit (0), or 32 rows and so many waves.
+// rows, waves: tiles of 128 or 64 rows (these without parts) and four waves, or of 32 rows and one wave or four.
 template <>
-int launch_serve<OMNI_INST_BF16 != 0, OMNI_INST_D>(const ServeParams& p, int waves, unsigned blocks, hipStream_t stream) {
+int launch_serve<OMNI_INST_BF16 != 0, OMNI_INST_D>(const ServeParams& p, int rows, int waves, unsigned blocks, hipStream_t stream) {
   constexpr bool BF = OMNI_INST_BF16 != 0;
   constexpr int D = OMNI_INST_D;
   constexpr size_t few = kFewLdsBytes<D>;
   const bool paged = p.page_table != nullptr;
   int e;
-  if (waves == 0) {
-    e = paged ? launch<serve_tile_kernel<BF, D, true>>(p, blocks, 256, kTileLdsBytes<D>, stream)
-              : launch<serve_tile_kernel<BF, D, false>>(p, blocks, 256, kTileLdsBytes<D>, stream);
+  if (rows == 128) {
+    e = paged ? launch<serve_tile_kernel<BF, D, true, 128>>(p, blocks, 256, kTileLdsBytes<D, 128>, stream)
+              : launch<serve_tile_kernel<BF, D, false, 128>>(p, blocks, 256, kTileLdsBytes<D, 128>, stream);
+  } else if (rows == 64) {
+    e = paged ? launch<serve_tile_kernel<BF, D, true, 64>>(p, blocks, 256, 2 * kTileLdsBytes<D, 64>, stream)
+              : launch<serve_tile_kernel<BF, D, false, 64>>(p, blocks, 256, 2 * kTileLdsBytes<D, 64>, stream);
   } else if (waves == 1) {
     e = paged ? launch<serve_few_kernel<BF, D, true, 1>>(p, blocks, 64, few, stream)
               : launch<serve_few_kernel<BF, D, false, 1>>(p, blocks, 64, few, stream);
@@ -56,8 +59,8 @@ int launch_serve<OMNI_INST_BF16 != 0, OMNI_INST_D>(const ServeParams& p, int wav
   if (e != 0 || p.share == 0.f) return e;
   const int64_t joined = int64_t(p.T) * ((p.Hk * p.G + kJoinRows<D> - 1) / kJoinRows<D>);
   const unsigned join_blocks = unsigned((joined + 3) / 4);
-  return waves == 0 ? launch<serve_join_kernel<BF, D, 128>>(p, join_blocks, 256, 0, stream)
-                    : launch<serve_join_kernel<BF, D, 32>>(p, join_blocks, 256, 0, stream);
+  return rows == 128 ? launch<serve_join_kernel<BF, D, 128>>(p, join_blocks, 256, 0, stream)
+                     : launch<serve_join_kernel<BF, D, 32>>(p, join_blocks, 256, 0, stream);
 }
 
 }  // namespace omni_attn

@@ -210,7 +210,7 @@ __device__ __forceinline__ Unit find_part(const ServeParams& p, const Batch& bat
 // the last tile of each first.
 template <int M>
 __device__ __forceinline__ Unit find_tile(const ServeParams& p, const Batch& batch, int rank, int lane) {
-  constexpr int kLog = M == 128 ? 7 : 5;
+  constexpr int kLog = M == 128 ? 7 : (M == 64 ? 6 : 5);
   static_assert(M == 1 << kLog, "rows of a tile");
   constexpr int kAll = 0x7fffffff;
   if (p.B == 1 || p.per_lane > 1) {
@@ -510,6 +510,73 @@ __device__ __forceinline__ uint32_t odd_rows(const f32x16_t (&ot)[DT]) {
 
 __device__ __forceinline__ uint32_t live_rows(int rows) { return rows >= 32 ? ~0u : (rows <= 0 ? 0u : (1u << rows) - 1u); }
 
+// KG groups of waves have shared the steps of a tile: every wave's maxima and sums, and its O, go into its own place in LDS
+// (wave_at of its group's bytes, which nobody reads any more); then each group adds up and stores a share of the columns
+// against the common maximum.
+template <int D>
+constexpr size_t kMergeBytes = size_t(32) * D * 4 + 256;  // of a wave
+template <bool BF16, int D, int M, int KG, bool PAGED>
+__device__ __forceinline__ void merge_groups(const ServeParams& p, const Unit& u, int head, int slot, int row0, int rows_all,
+                                             const f32x16_t (&ot)[D / 32], float m_run, float l_run, bool several,
+                                             uint8_t* lds, size_t group_bytes, size_t wave_at, int kg, int from, int to, int lane) {
+  typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+  constexpr int PIECES = D / 8, MINE = PIECES / KG;  // 4-register pieces of a lane's O
+  static_assert(PIECES % KG == 0, "every group has a share");
+  const int c = lane & 31, g = lane >> 5;
+  auto piece_at = [&](int i, int piece) { return reinterpret_cast<f32x4_t*>(lds + i * group_bytes + wave_at) + piece * 64 + lane; };
+  auto stat_at = [&](int i) { return reinterpret_cast<float*>(lds + i * group_bytes + wave_at + 32 * D * 4) + 2 * c; };
+  const float l = pair_sum(l_run);
+  const uint32_t mine_odd = several ? odd_rows<D / 32>(ot) : 0u;
+  if (g == 0) {
+    stat_at(kg)[0] = m_run;
+    stat_at(kg)[1] = mine_odd >> c & 1 ? __builtin_nanf("") : l;
+  }
+  static_for<PIECES>([&](auto pc) {
+    constexpr int piece = decltype(pc)::value, dt = piece / 4, r = 4 * (piece % 4);
+    *piece_at(kg, piece) = f32x4_t{ot[dt][r], ot[dt][r + 1], ot[dt][r + 2], ot[dt][r + 3]};
+  });
+  __syncthreads();
+  float m_all = -INFINITY, l_all = 0.f, scale[KG];
+#pragma unroll
+  for (int i = 0; i < KG; ++i) m_all = fmaxf(m_all, stat_at(i)[0]);
+  const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+#pragma unroll
+  for (int i = 0; i < KG; ++i) {
+    scale[i] = __builtin_amdgcn_exp2f(stat_at(i)[0] - m_ref);
+    l_all += stat_at(i)[1] * scale[i];
+  }
+  const bool live = l_all > 0.f || l_all != l_all;
+  const float inv = u.part ? 1.f : (live ? 1.f / l_all : 0.f);
+  const uint32_t odd = several ? uint32_t(__builtin_amdgcn_ballot_w64(l_all != l_all)) & live_rows(rows_all - row0) : 0u;
+  const bool mine = row0 + c < rows_all && !(odd >> c & 1);
+  const int row = row0 + c < rows_all ? row0 + c : rows_all - 1, token = int(divide(uint32_t(row), p.group));
+  const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (row - token * p.G);
+  const int64_t part_at = (int64_t(slot) * p.Hk + head) * M + (row0 & (M - 1)) + c;
+#pragma unroll
+  for (int n = 0; n < MINE; ++n) {
+    const int piece = kg * MINE + n;
+    f32x4_t x = *piece_at(0, piece) * scale[0];
+#pragma unroll
+    for (int i = 1; i < KG; ++i) x += *piece_at(i, piece) * scale[i];
+    if (!mine) continue;
+    if (u.part) {
+      *reinterpret_cast<f32x4_t*>(p.sums + part_at * D + 8 * piece + 4 * g) = x;
+    } else {
+      const u32x2_t ov = {live ? pack2<BF16>(x[0] * inv, x[1] * inv) : 0u, live ? pack2<BF16>(x[2] * inv, x[3] * inv) : 0u};
+      *reinterpret_cast<u32x2_t*>(p.o + at * D + 8 * piece + 4 * g) = ov;
+    }
+  }
+  if (kg == 0 && g == 0 && mine) {
+    if (u.part) {
+      p.stats[part_at * 2] = m_all;
+      p.stats[part_at * 2 + 1] = l_all;
+    } else if (p.lse != nullptr) {
+      p.lse[at] = live ? (m_all + __builtin_amdgcn_logf(l_all)) * 0.6931471805599453f : -INFINITY;
+    }
+  }
+  if (kg == 0 && odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, slot, row0, odd, from, to, lane);
+}
+
 // ---- few rows ---------------------------------------------------------------------------------------------------
 //
 // Single tokens, a few, and short prompts: tiles of 32 rows.  The work is the reading of K and V: a wave has a K and a V
@@ -520,7 +587,7 @@ __device__ __forceinline__ uint32_t live_rows(int rows) { return rows >= 32 ? ~0
 template <int D>
 constexpr int kFewStep = D == 128 ? 32 : 64;  // keys per step: 16 KiB of K and V
 template <int D>
-constexpr size_t kFewLdsBytes = size_t(2) * kFewStep<D> * D * 2 + 256;  // of a wave: tiles, and room for its rows' statistics
+constexpr size_t kFewLdsBytes = kMergeBytes<D> > size_t(2) * kFewStep<D> * D * 2 ? kMergeBytes<D> : size_t(2) * kFewStep<D> * D * 2;  // of a wave
 
 template <bool BF16, int D, bool PAGED, int KG>
 __global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p) {
@@ -683,111 +750,68 @@ __global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p)
     store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, odd, sK, lane);
     if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
   } else {
-    // Every wave's maxima and sums, then its O against the common maximum, into its own tiles; each wave adds up and
-    // stores a share of the columns.
-    constexpr int PIECES = DT * 4, MINE = PIECES / KG;  // 4-register pieces of a lane's O
-    constexpr size_t kStats = kFewLdsBytes<D> - 256;
-    static_assert(PIECES % KG == 0 && size_t(32) * D * 4 <= kStats, "merge layout");
-    typedef __attribute__((ext_vector_type(4))) float f32x4_t;
-    auto piece_at = [&](int i, int piece) { return reinterpret_cast<f32x4_t*>(lds_raw + i * kFewLdsBytes<D>) + piece * 64 + lane; };
-    auto stat_at = [&](int i) { return reinterpret_cast<float*>(lds_raw + i * kFewLdsBytes<D> + kStats) + 2 * c; };
-    const float l = pair_sum(l_run);
-    const uint32_t mine_odd = several ? odd_rows<DT>(ot) : 0u;
-    if (g == 0) {
-      stat_at(kg)[0] = m_run;
-      stat_at(kg)[1] = mine_odd >> c & 1 ? __builtin_nanf("") : l;
-    }
-    static_for<PIECES>([&](auto pc) {
-      constexpr int piece = decltype(pc)::value, dt = piece / 4, r = 4 * (piece % 4);
-      *piece_at(kg, piece) = f32x4_t{ot[dt][r], ot[dt][r + 1], ot[dt][r + 2], ot[dt][r + 3]};
-    });
-    __syncthreads();
-    float m_all = -INFINITY, l_all = 0.f, scale[KG];
-#pragma unroll
-    for (int i = 0; i < KG; ++i) m_all = fmaxf(m_all, stat_at(i)[0]);
-    const float m_ref = m_all == -INFINITY ? 0.f : m_all;
-#pragma unroll
-    for (int i = 0; i < KG; ++i) {
-      scale[i] = __builtin_amdgcn_exp2f(stat_at(i)[0] - m_ref);
-      l_all += stat_at(i)[1] * scale[i];
-    }
-    const bool live = l_all > 0.f || l_all != l_all;
-    const float inv = u.part ? 1.f : (live ? 1.f / l_all : 0.f);
-    const uint32_t odd = several ? uint32_t(__builtin_amdgcn_ballot_w64(l_all != l_all)) & live_rows(rows_all - row0) : 0u;
-    const bool mine = row0 + c < rows_all && !(odd >> c & 1);
-    const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (row - token * p.G);
-    const int64_t part_at = (int64_t(rank) * p.Hk + head) * M + c;
-#pragma unroll
-    for (int n = 0; n < MINE; ++n) {
-      const int piece = kg * MINE + n;
-      f32x4_t x = *piece_at(0, piece) * scale[0];
-#pragma unroll
-      for (int i = 1; i < KG; ++i) x += *piece_at(i, piece) * scale[i];
-      if (!mine) continue;
-      if (u.part) {
-        *reinterpret_cast<f32x4_t*>(p.sums + part_at * D + 8 * piece + 4 * g) = x;
-      } else {
-        const u32x2_t ov = {live ? pack2<BF16>(x[0] * inv, x[1] * inv) : 0u, live ? pack2<BF16>(x[2] * inv, x[3] * inv) : 0u};
-        *reinterpret_cast<u32x2_t*>(p.o + at * D + 8 * piece + 4 * g) = ov;
-      }
-    }
-    if (kg == 0 && g == 0 && mine) {
-      if (u.part) {
-        p.stats[part_at * 2] = m_all;
-        p.stats[part_at * 2 + 1] = l_all;
-      } else if (p.lse != nullptr) {
-        p.lse[at] = live ? (m_all + __builtin_amdgcn_logf(l_all)) * 0.6931471805599453f : -INFINITY;
-      }
-    }
-    if (kg == 0 && odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
+    merge_groups<BF16, D, M, KG, PAGED>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, several, lds_raw,
+                                        kFewLdsBytes<D>, 0, kg, from, to, lane);
   }
 }
 
 // ---- many rows: four waves per unit -------------------------------------------------------------------------------
 //
-// A tile of 128 rows, 32 per wave, walks its keys in steps of 64, software-pipelined like the block-sparse forward:
-// iteration i issues the matrix instructions of S^T(i + 1) and of O^T += V^T P^T(i - 1) in slots, and between
+// A tile of M rows, 32 per wave, walks its keys in steps, software-pipelined like the block-sparse forward: iteration i issues the matrix instructions of S^T(i + 1) and of O^T += V^T P^T(i - 1) in slots, and between
 // them the softmax of step i, the operand fetches and the loads of K(i + 2) and V(i).  The exponentials' reference
 // stays where it is as long as the row sums do not outgrow it.
+// M = 128: four waves, steps of 64 keys.  M = 64: two groups of two waves share the steps (group i takes the steps i, i + 2,
+// ...) and add up at the end: half the walk, for launches that a few tiles' walks are long for; steps of 32 keys at
+// head_dim 128, so that two workgroups share a compute unit there too.
 
-template <int D>
-constexpr size_t kTileLdsBytes = size_t(2) * 2 * kStepKeys * D * 2;
+template <int D, int M>
+constexpr int kTileStep = M == 64 && D == 128 ? 32 : 64;
+// Of a group: two sets of K and V, or its waves' sums.
+template <int D, int M>
+constexpr size_t kTileLdsBytes = M == 64 && 2 * kMergeBytes<D> > size_t(8) * kTileStep<D, M> * D ? 2 * kMergeBytes<D>
+                                                                                             : size_t(8) * kTileStep<D, M> * D;
 
-template <bool BF16, int D, bool PAGED>
+template <bool BF16, int D, bool PAGED, int M>
 __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p) {
-  constexpr int M = 128, STEP = kStepKeys, NTL = 2, KS = D / 16, DT = D / 32, CPR = D / 8, TILE = STEP * D;
+  constexpr int KG = 128 / M, W = M / 32, STEP = kTileStep<D, M>, NTL = STEP / 32, KS = D / 16, DT = D / 32, CPR = D / 8;
+  constexpr int TILE = STEP * D;
   constexpr int RPC = 64 / CPR;            // rows filled by a wave's load
-  constexpr int ROW_STRIDE = RPC * 4;      // rows between a thread's loads
+  constexpr int ROW_STRIDE = RPC * W;      // rows between a thread's loads
   constexpr int NCH = STEP / ROW_STRIDE;   // loads per thread and tile
   constexpr int KPER = ROW_STRIDE % 16 == 0 ? 1 : 16 / ROW_STRIDE;
   static_assert((KPER * ROW_STRIDE) % 16 == 0 && ROW_STRIDE % 4 == 0 && RPC <= 16, "swizzles repeat over a thread's loads");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
-  uint16_t* sK = reinterpret_cast<uint16_t*>(lds_raw);  // [2][TILE]
-  uint16_t* sV = sK + 2 * TILE;
-  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c = lane & 31;
+  const int tid = threadIdx.x & (64 * W - 1), lane = tid & 63, g = lane >> 5, c = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(int(threadIdx.x) / (64 * W));
+  uint16_t* sK = reinterpret_cast<uint16_t*>(lds_raw + kg * kTileLdsBytes<D, M>);  // [2][TILE]
+  uint16_t* sV = sK + 2 * TILE;
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
   const Unit u = find_unit<M>(p, rank, lane);
   if (!u.found) {
-    if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, tid, 256);
+    if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, threadIdx.x, 256);
     return;
   }
   const int shift = u.seq.kv - u.seq.n;  // a token's position, less its number
   const int rows_all = u.seq.n * p.G, row0 = u.tile * M + 32 * w;
-  tell_joins<M>(p, u, head, rows_all, tid);
+  tell_joins<M>(p, u, head, rows_all, threadIdx.x);
   const int row = row0 + c < rows_all ? row0 + c : rows_all - 1;
   const int token = int(divide(uint32_t(row), p.group));
   const int last_row = u.tile * M + M < rows_all ? u.tile * M + M - 1 : rows_all - 1;
   const int last_key = p.causal ? shift + int(divide(uint32_t(last_row), p.group)) : u.seq.kv - 1;
   const int wave_first = row0 < rows_all ? row0 : rows_all - 1;
   const int first_key = __builtin_amdgcn_readfirstlane(p.causal ? shift + int(divide(uint32_t(wave_first), p.group)) : u.seq.kv - 1);
-  const int from = u.step0 * STEP;
-  int to = u.steps < steps_of(u.seq.kv) - u.step0 ? (u.step0 + u.steps) * STEP : u.seq.kv;
+  const int from = u.step0 * kStepKeys;
+  int to = u.steps < steps_of(u.seq.kv) - u.step0 ? (u.step0 + u.steps) * kStepKeys : u.seq.kv;
   if (to > last_key + 1) to = last_key + 1;  // (keys at or behind `to` are not read)
   to = __builtin_amdgcn_readfirstlane(to);
-  const int nsteps = __builtin_amdgcn_readfirstlane(to > from ? (to - from + STEP - 1) / STEP : 0);
+  // (of each group; where one has a step less than the other its last one lies behind `to`: nothing of it is read, and all
+  // its scores are masked)
+  const int nsteps = __builtin_amdgcn_readfirstlane(to > from ? (to - from + STEP * KG - 1) / (STEP * KG) : 0);
+  constexpr int NEXT = STEP * KG;  // keys from a group's step to its next
+  const int from_kg = from + kg * STEP;
 
   u32x4_t qf[KS];
   {
@@ -829,7 +853,7 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
   auto issue_load = [&](int n, int buf, int k_key0, int v_key0, const i32x4_t& rk, const i32x4_t& rv) {
     const bool is_v = n < NCH;
     const int i = is_v ? n : n - NCH;
-    const uint32_t dst = (is_v ? lds_v0 : lds_k0) + uint32_t(buf) * (TILE * 2u) + uint32_t(i) * 4096u;
+    const uint32_t dst = (is_v ? lds_v0 : lds_k0) + uint32_t(buf) * (TILE * 2u) + uint32_t(i) * (W * 1024u);
     const uint32_t off = is_v ? voff : koff[i % KPER];
     if constexpr (PAGED) {
       const int key = (is_v ? v_key0 : k_key0) + i * ROW_STRIDE + w * RPC;
@@ -989,7 +1013,7 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
   // Steps behind the last one: loads whose rows all lie behind `to` and arrive as zeros.
   auto iteration = [&](auto set_c, auto first_c, int it) {
     constexpr int SET = decltype(set_c)::value;
-    const int key0 = from + it * STEP;
+    const int key0 = from_kg + it * NEXT;
     wait_loads();
     __syncthreads();
     u32x4_t opq[PF];
@@ -1012,8 +1036,8 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
       if (owed & kOwesLook) look(set_c);
     }
     need_window(vwin, kwin, key0);
-    need_window(kwin, vwin, key0 + 2 * STEP);
-    float sum = body(set_c, first_c, key0 + 2 * STEP, key0, opq);
+    need_window(kwin, vwin, key0 + 2 * NEXT);
+    float sum = body(set_c, first_c, key0 + 2 * NEXT, key0, opq);
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= kGrown)) != 0, 0)) {
       owed |= kOwesLook;
       if (__builtin_amdgcn_ballot_w64(!(sum <= kRedo)) != 0) redo(set_c, sum);
@@ -1021,17 +1045,17 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
     l_run += sum;
   };
   if (nsteps > 0) {
-    need_window(kwin, kwin, from);
+    need_window(kwin, kwin, from_kg);
     {
-      const i32x4_t r0 = rows_of(kr, from);
+      const i32x4_t r0 = rows_of(kr, from_kg);
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 0, from, 0, r0, r0);
+      for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 0, from_kg, 0, r0, r0);
     }
-    need_window(kwin, kwin, from + STEP);
+    need_window(kwin, kwin, from_kg + NEXT);
     {
-      const i32x4_t r1 = rows_of(kr, from + STEP);
+      const i32x4_t r1 = rows_of(kr, from_kg + NEXT);
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 1, from + STEP, 0, r1, r1);
+      for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 1, from_kg + NEXT, 0, r1, r1);
     }
     wait_loads_but<NCH>();  // K(1) may be under way
     __syncthreads();
@@ -1063,8 +1087,16 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
       drain(IntC<0>{});
     }
   }
+  const bool several = p.causal && first_key < last_key;  // rows that attend different keys
+  if constexpr (KG > 1) {
+    static_assert(W * kMergeBytes<D> <= kTileLdsBytes<D, M>, "merge layout");
+    __syncthreads();  // (the group's other wave may still read V)
+    merge_groups<BF16, D, M, KG, PAGED>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, several, lds_raw,
+                                        kTileLdsBytes<D, M>, w * kMergeBytes<D>, kg, from, to, lane);
+    return;
+  }
   // (the K tiles are read by nobody any more: a wave stages its rows in a quarter of them)
-  const uint32_t odd = p.causal && first_key < last_key ? odd_rows<DT>(ot) & live_rows(rows_all - row0) : 0u;
+  const uint32_t odd = several ? odd_rows<DT>(ot) & live_rows(rows_all - row0) : 0u;
   store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, odd, sK + w * 32 * D, lane);
   if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
 }

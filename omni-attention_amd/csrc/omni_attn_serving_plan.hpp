@@ -8,13 +8,13 @@
 namespace omni_attn {
 
 struct ServePlan {
-  int waves;       // 0: tiles of 128 rows and four waves; else tiles of 32 rows and so many waves
+  int rows;        // of a tile: 128, 64 or 32
+  int waves;       // of a workgroup: 4, or 1 (tiles of 32 rows)
   float share;     // units per key head that the steps are shared over, 0: whole tiles
   int least_steps; // steps that a part may have in any case
   int64_t units;   // units per key head that there is a place for
-  int rows() const { return waves == 0 ? 128 : 32; }
   size_t workspace_bytes(int64_t T, int Hk, int D) const {  // the parts' rows and statistics, and four words per token
-    return share == 0.f ? 0 : size_t(units) * size_t(Hk) * size_t(rows()) * size_t(D + 2) * sizeof(float) + size_t(T) * 16;
+    return share == 0.f ? 0 : size_t(units) * size_t(Hk) * size_t(rows) * size_t(D + 2) * sizeof(float) + size_t(T) * 16;
   }
 };
 
@@ -23,33 +23,39 @@ struct ServePlan {
 // cache that there may be any number of.
 inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, int64_t capacity, int cus) {
   ServePlan s;
-  const int64_t rows = T * G;
-  const auto tiles_of = [&](int64_t M) { return rows / M + B; };  // at most: every sequence has one that is not full
+  const int64_t all = T * G;
+  s.rows = 32;
+  s.waves = 4;
+  const auto tiles_of = [&](int64_t M) { return all / M + B; };  // at most: every sequence has one that is not full
   const int64_t keys = capacity != 0 ? capacity : T / B;
   int64_t wanted = 0;  // units in all, where tiles are shared by parts
   s.least_steps = 2;
-  if (rows <= 64 * B) {
+  if (all <= 64 * B) {
     // Single tokens, a few.  One wave per tile where keys are few and tiles more than the card holds at a time: D=128, 32 / 8
     // heads, 512 sequences of 30 - 100 keys 34 us, 58 with four waves, 110 with four and parts; 256 of 100 - 300 keys 41, 47
     // and 61; 200 prompts of 60 tokens 24 and 41.  Else four waves and parts: 8 tokens after 2000 keys 22 us, 34 with whole
     // tiles, 106 with one wave; after 60000 keys 345, 900 and 3232; 64 tokens after 500 - 1500 keys 50 us, 44 with whole tiles
     // (lengths are not known here).  Twice as many units or half as many: within 3 %.
-    s.waves = (keys <= 512 && tiles_of(32) * Hk > 4 * cus) || (capacity == 0 && keys <= 128) ? 1 : 4;
+    if ((keys <= 512 && tiles_of(32) * Hk > 4 * cus) || (capacity == 0 && keys <= 128)) s.waves = 1;
     if (s.waves == 4 && keys > 512) wanted = 4 * cus;
     s.least_steps = 4;
   } else if (tiles_of(32) * Hk <= 2 * cus + B * Hk && keys <= 2560) {
     // Prompts whose 32-row tiles all run at once: four waves on the keys of each.  512 tokens, D=64, 8 heads 6.8 us, 10.4 with
     // tiles of 128 rows; 2048 tokens 15 and 26; D=128, 32 / 8 heads, 512 tokens 11.2 and 13.5 (1024 tokens, beyond the line,
     // 26 and 22; 8192 tokens, 2 heads, 81 and 63 in parts).
-    s.waves = 4;
   } else {
     // Parts where the tiles leave compute units without work: 4096 tokens, one head, 26 us, 61 whole; 8192, 2 heads, 64 and
     // 117; 812 new tokens after 22000, 32 / 8 heads, 197 and 307 (2000 after 10000, beyond the line, 377 and 347).
-    s.waves = 0;
+    s.rows = 128;
     if (tiles_of(128) * Hk <= (capacity != 0 ? 3 * cus / 2 : cus) && keys > 2560) wanted = 3 * cus;
+    // Tiles of 64 rows and two groups of waves where there are fewer tiles of 128 than the card holds at a time, and their
+    // walks are not short: 9 prompts of 35 - 1047 tokens, D=64, 16 heads, capped scores 20 us, 26 with 128 rows; 4 x 1157
+    // tokens, 8 heads 23.6 and 27.5; 1024 tokens, D=128, 32 / 8 heads 19.3 and 22.1 (beyond the line: 2048 tokens 46.4 and
+    // 44.7; 4 x 512 25.8 and 19.5; 16 x 100 tokens, D=64, 16 heads 8.2 and 7.6).
+    if (wanted == 0 && (2 * all / 128 + B) * Hk <= 7 * cus / 2 && keys >= 256 && keys <= 2560) s.rows = 64;
     s.least_steps = 8;
   }
-  const int64_t tiles = tiles_of(s.rows());
+  const int64_t tiles = tiles_of(s.rows);
   const bool parts = wanted != 0;
   s.share = parts ? float((wanted + Hk - 1) / Hk) : 0.f;
   // (the sum of what every tile is over a whole number of parts; one more workgroup, so that there is always one

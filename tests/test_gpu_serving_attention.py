@@ -68,13 +68,15 @@ def test_packed(gpu_device, dtype, D, lens, Hq, Hk, causal, softcap):
 @pytest.mark.parametrize("lens,Hq,Hk,D", [
     ([1500, 2048, 700, 33, 128, 1], 32, 8, 128),   # tiles, whole: their order goes by length
     ([1024] * 3, 16, 16, 64), ([2000, 100], 24, 24, 32),
-    ([40] * 330, 8, 8, 64)])                       # few rows, whole
-def test_packed_whole_tiles(gpu_device, dtype, lens, Hq, Hk, D):
+    ([40] * 330, 8, 8, 64),                        # few rows, whole
+    ([1300], 16, 16, 128), ([700, 0, 900, 64], 32, 8, 64), ([1500], 12, 12, 32)])  # two groups of waves on tiles of 64 rows
+@pytest.mark.parametrize("causal,softcap", [(True, 0.0), (False, 20.0)])
+def test_packed_whole_tiles(gpu_device, dtype, lens, Hq, Hk, D, causal, softcap):
     gen = torch.Generator().manual_seed(Hq)
     q, k, v, cu = _packed(gen, gpu_device, dtype, lens, Hq, Hk, D, behind=300)
-    o, lse = oat.omni_attention_packed(q, k, v, cu, return_lse=True)
+    o, lse = oat.omni_attention_packed(q, k, v, cu, causal=causal, softcap=softcap, return_lse=True)
     at = offsets(lens)
-    _compare(o, lse, q, [(a, b - a, k[a:b], v[a:b]) for a, b in zip(at, at[1:])], True, 0.0, dtype, "whole")
+    _compare(o, lse, q, [(a, b - a, k[a:b], v[a:b]) for a, b in zip(at, at[1:])], causal, softcap, dtype, "whole")
 
 
 def test_packed_rows_of_a_fused_projection(gpu_device):
@@ -137,6 +139,7 @@ def _paged(gen, device, dtype, lens, kv, Hq, Hk, D, page, behind=2, spare=2):
     ([1] * 7, [1, 15, 16, 17, 500, 64, 1111], 8, 2, True, 0.0), ([1, 0, 1, 1], [90, 33, 0, 5], 4, 1, True, 20.0),
     ([3, 1, 8], [3, 130, 77], 6, 2, True, 0.0), ([5, 2], [5, 300], 4, 4, False, 0.0),
     ([70, 200, 1], [1500, 200, 40], 8, 2, True, 0.0), ([130], [900], 2, 1, False, 30.0),
+    ([600, 500], [900, 700], 16, 8, True, 0.0), ([600, 1, 500], [600, 0, 1000], 8, 8, False, 20.0),
     ([4, 40], [2, 30], 2, 2, True, 0.0)])  # (fewer keys than tokens: the first tokens have none)
 def test_paged(gpu_device, dtype, D, page, lens, kv, Hq, Hk, causal, softcap):
     gen = torch.Generator().manual_seed(page + D + len(lens))
@@ -157,11 +160,13 @@ def test_paged_many_sequences_and_long_ones(gpu_device, dtype):
         _compare(o, lse, q, [(at[b], lens[b], *keys[b]) for b in range(len(lens))], True, 0.0, dtype, str(kv[:3]))
 
 
-@pytest.mark.parametrize("lens,kv", [([1, 6, 3], [50, 6, 90]), ([200, 90], [200, 300])])
-def test_values_that_are_no_numbers_behind_a_row(gpu_device, lens, kv):
+@pytest.mark.parametrize("lens,kv,Hq,Hk,D", [([1, 6, 3], [50, 6, 90], 4, 2, 64), ([200, 90], [200, 300], 4, 2, 64),
+                                             ([600, 500], [900, 700], 16, 8, 128), ([7] * 200, [60] * 200, 8, 8, 32),
+                                             ([400], [6000], 4, 1, 128), ([9, 2], [5000, 700], 8, 2, 128)])
+def test_values_that_are_no_numbers_behind_a_row(gpu_device, lens, kv, Hq, Hk, D):
     """Infinities and NaN in K and V of later keys of the same sequence reach no row that does not attend them."""
     gen = torch.Generator().manual_seed(7)
-    dtype, Hq, Hk, D, page = torch.bfloat16, 4, 2, 64, 16
+    dtype, page = torch.bfloat16, 16
     q, (kp, vp), table, kv_lens, cu, keys = _paged(gen, gpu_device, dtype, lens, kv, Hq, Hk, D, page)
     clean = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu)
     at = offsets(lens)
@@ -169,11 +174,12 @@ def test_values_that_are_no_numbers_behind_a_row(gpu_device, lens, kv):
         if n < 2:
             continue
         last = kv[b] - 1 - n // 4  # this key and what is behind it is spoilt
-        for pos in range(last, kv[b]):
-            pg = int(table[b, pos // page])
-            vp[pg, :, pos % page, ::3] = float("inf") if pos % 2 else float("nan")
-            if pos % 3 == 0:
-                kp[pg, :, pos % page] = float("nan")
+        pos = torch.arange(last, kv[b], device=gpu_device)
+        pg = table[b][pos // page].long()
+        bad = torch.where(pos % 2 == 1, float("inf"), float("nan")).to(dtype)
+        vp[pg, :, pos % page, ::3] = bad.view(-1, 1, 1).expand(-1, Hk, len(range(0, D, 3)))
+        third = pos[pos % 3 == 0]
+        kp[table[b][third // page].long(), :, third % page] = float("nan")
     dirty = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu)
     for b, n in enumerate(lens):
         first_bad = n - 1 - n // 4 if n >= 2 else n

@@ -160,7 +160,7 @@ int main() {
       T += n[b];
     }
     const ServePlan s = plan_serve(T, B, Hk, G, capacity, 256);
-    const long long M = s.rows();
+    const long long M = s.rows;
     long long units = 0, part = 0;
     if (s.share > 0.f) {
       float all = 0.f;
@@ -184,7 +184,7 @@ int main() {
       if (at_head < s.units) at_head = -1;
       if (at_head < 0) break;
     }
-    printf("%lld %lld %lld %d %d\n", units, (long long)s.units, at_head, int(s.share > 0.f), s.waves);
+    printf("%lld %lld %lld %d %d %d\n", units, (long long)s.units, at_head, int(s.share > 0.f), s.rows, s.waves);
   }
 }
 """
@@ -211,7 +211,7 @@ def test_every_unit_has_a_place(tmp_path):
     assert len(out) == len(lines) + 1
     seen = set()
     for line, given in zip(out, lines):
-        units, room, at_head, parts, waves = map(int, line.split())
-        seen.add((parts, waves))
+        units, room, at_head, parts, rows, waves = map(int, line.split())
+        seen.add((parts, rows, waves))
         assert units <= (room if parts else room - 1) and at_head >= room, given[:200]
-    assert seen == {(0, 0), (1, 0), (0, 1), (0, 4), (1, 4)}
+    assert seen == {(0, 128, 4), (1, 128, 4), (0, 64, 4), (0, 32, 1), (0, 32, 4), (1, 32, 4)}
