@@ -50,7 +50,7 @@ enum omni_attn_status {
   OMNI_ATTN_ERR_TOO_LARGE = 7,         /* a tensor exceeds 2^31-1 elements per (b,h) slab */
   OMNI_ATTN_ERR_MISALIGNED = 8,        /* q, k, v, o or partial masks not 16-byte aligned, or a
                                           32-bit array not 4-byte aligned */
-  OMNI_ATTN_ERR_WORKSPACE = 9,         /* workspace smaller than omni_attn_bwd_workspace_bytes() */
+  OMNI_ATTN_ERR_WORKSPACE = 9,         /* workspace smaller than the entry point's _workspace_bytes() */
   OMNI_ATTN_ERR_SCRATCH_LIMIT = 10     /* omni_attn_bwd_noalloc_gfx950: B * H * S_pad beyond its
                                           built-in scratch (omni_attn_bwd_noalloc_max_rows()) */
 };
@@ -360,7 +360,7 @@ int omni_attn_qk_rotary_bwd_gfx950(const void* dq_out, const void* dk_out, const
 
 /*
  * New tokens of a batch of sequences enter a paged cache.  Sequence b has the tokens cu_seqlens[b] ..
- * cu_seqlens[b + 1] - 1 (cu_seqlens [sequences + 1] int32) and kv_lens[b] keys with them: token i of it is at position
+ * cu_seqlens[b + 1] - 1 (cu_seqlens [sequences + 1] int32: 0 first, not decreasing) and kv_lens[b] keys with them: token i is at position
  * pos = kv_lens[b] - cu_seqlens[b + 1] + i, in row pos % page_size of page page_table[b, pos / page_size].
  *
  *   k, v       [tokens, Hk, D] at (head, row) strides as above.  k is normed and rotated as above on the way, v goes

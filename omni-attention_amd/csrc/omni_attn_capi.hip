@@ -519,7 +519,7 @@ extern "C" const char* omni_attn_status_string(int status) {
     case OMNI_ATTN_ERR_LAUNCH: return "HIP kernel launch failed";
     case OMNI_ATTN_ERR_TOO_LARGE: return "tensor too large for 32-bit slab indexing";
     case OMNI_ATTN_ERR_MISALIGNED: return "misaligned pointer: q, k, v, o and partial masks need 16 bytes, 32-bit arrays 4";
-    case OMNI_ATTN_ERR_WORKSPACE: return "workspace too small (see omni_attn_bwd_workspace_bytes)";
+    case OMNI_ATTN_ERR_WORKSPACE: return "workspace too small (see the entry point's _workspace_bytes function)";
     case OMNI_ATTN_ERR_SCRATCH_LIMIT:
       return "B * H * S_pad exceeds the built-in scratch of omni_attn_bwd_noalloc_gfx950 (4 194 304 rows); "
              "use omni_attn_bwd_gfx950 with a workspace";

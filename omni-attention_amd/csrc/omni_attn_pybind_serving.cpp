@@ -52,16 +52,12 @@ void check_no_grad(std::initializer_list<Tensor> tensors, const char* op) {
       refuse(std::string(op) + " is not differentiable: call it under torch.no_grad()");
 }
 
-// Rows that the kernels read in place: whole pieces of `piece` elements.  Others are copied.
+// Rows that the kernels read in place: whole pieces of `piece` elements, up to 2^24 apart ([B, H, S, D]: 2^31).  Others are
+// copied.
 Tensor in_rows(const Tensor& t, int64_t piece) {
   bool ok = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & uintptr_t(2 * piece - 1)) == 0;
-  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && t.stride(i) >= 0 && t.stride(i) % piece == 0 && t.stride(i) <= (1 << 24);
-  // (the first dimension of [B, H, S, D] may be any distance apart)
-  if (!ok && t.dim() == 4 && t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & uintptr_t(2 * piece - 1)) == 0) {
-    ok = true;
-    for (int64_t i = 0; i < 3; ++i) ok = ok && t.stride(i) >= 0 && t.stride(i) % piece == 0;
-    ok = ok && t.stride(2) <= 0x7fffffff;
-  }
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && t.stride(i) >= 0 && t.stride(i) % piece == 0;
+  ok = ok && (t.dim() == 3 ? t.stride(0) <= (1 << 24) && t.stride(1) <= (1 << 30) : t.stride(2) <= 0x7fffffff);
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 Tensor aligned(const Tensor& t) {  // contiguous and on a 16-byte boundary
@@ -319,6 +315,9 @@ pybind11::object omni_attn_cache_append(Tensor k, Tensor v, Tensor k_pages, Tens
     k = in_rows(k, 4);
     v = in_rows(v, 4);
     if (q.defined()) q = in_rows(q, 4);
+    // (what autograd has saved of the pages is no longer theirs; refuses what may not be written)
+    k_pages.unsafeGetTensorImpl()->bump_version();
+    v_pages.unsafeGetTensorImpl()->bump_version();
     const omni_attn_strides none{0, 0, 0};
     const bool turns = r.table.defined();
     const int rc = omni_attn_cache_append_gfx950(
@@ -331,8 +330,6 @@ pybind11::object omni_attn_cache_append(Tensor k, Tensor v, Tensor k_pages, Tens
         int(page_table.size(1)), turns ? int(r.table.size(1)) : 0, turns ? int(r.table.size(0)) : 0, float(r.eps), r.interleaved,
         dtype_of(k), stream_of(k));
     if (rc != OMNI_ATTN_OK) fail(rc);
-    k_pages.unsafeGetTensorImpl()->bump_version();
-    v_pages.unsafeGetTensorImpl()->bump_version();
   } else if (q_out.defined()) {
     q_out.zero_();
   }

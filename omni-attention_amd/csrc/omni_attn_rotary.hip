@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kBlockWaves * 64) cache_append_kernel(AppendPa
   uint16_t *krow = nullptr, *vrow = nullptr;
   bool owned = false;
   if (b < ap.sequences) {
-    const int first = load_uniform(ap.cu + b), behind = load_uniform(ap.cu + b + 1);
+    const int first = b == 0 ? 0 : load_uniform(ap.cu + b), behind = load_uniform(ap.cu + b + 1);
     const int64_t keys = load_uniform(ap.kv_lens + b);
     if (token >= first && token < behind) {
       owned = true;

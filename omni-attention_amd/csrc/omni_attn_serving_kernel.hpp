@@ -86,11 +86,12 @@ __device__ __forceinline__ int wave_max(int x) {  // x >= 0
 struct Sequence {
   int first, n, kv;  // first token, tokens, keys
 };
-// (offsets that run backwards or beyond the tokens, and lengths beyond the page table, are cut)
+// (the first offset counts as 0; offsets that run backwards or beyond the tokens, and lengths beyond the page table, are
+// cut)
 __device__ __forceinline__ Sequence sequence_of(const ServeParams& p, int b) {
   Sequence s = {0, 0, 0};
   if (b < p.B) {
-    int from = p.cu[b], to = p.cu[b + 1];
+    int from = b == 0 ? 0 : p.cu[b], to = p.cu[b + 1];
     from = from < 0 ? 0 : (from > p.T ? p.T : from);
     to = to < from ? from : (to > p.T ? p.T : to);
     s.first = from;

@@ -869,8 +869,8 @@ def omni_cache_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages
                  two from 16
     page_table   [sequences, max_pages] int32: the pages of each sequence, in order
     kv_lens      [sequences] int32: keys of each sequence, the new ones included
-    cu_seqlens   [sequences + 1] int32: sequence b has the tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1, the last of
-                 them at position kv_lens[b] - 1
+    cu_seqlens   [sequences + 1] int32, 0 first and not decreasing: sequence b has the tokens cu_seqlens[b] ..
+                 cu_seqlens[b + 1] - 1, the last of them at position kv_lens[b] - 1
     positions    [tokens] table rows to rotate by, where they are not the places in the sequence
 
     Tokens whose page number or position lies outside the cache are not written, and no row but the new tokens' is.

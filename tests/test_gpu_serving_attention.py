@@ -107,6 +107,23 @@ def test_packed_agrees_with_the_block_sparse_operator(gpu_device):
     assert (got.float() - ref.float()).abs().max().item() <= 4 * 4 * torch.finfo(dtype).eps / 2
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,Hq,Hk,D", [([200], 4, 2, 64), ([1300], 16, 16, 128), ([1500, 2048, 700], 32, 8, 128), ([9] * 40, 8, 8, 32)])
+def test_scores_that_outgrow_their_reference(gpu_device, dtype, lens, Hq, Hk, D):
+    """Scores that grow along the keys, in steps and within a step, shrink, and jump at a single key."""
+    gen = torch.Generator().manual_seed(13)
+    q, k, v, cu = _packed(gen, gpu_device, dtype, lens, Hq, Hk, D)
+    position = torch.cat([torch.arange(n) for n in lens] + [torch.zeros(2, dtype=torch.long)]).to(gpu_device)
+    towards = torch.randn(D, generator=gen).to(gpu_device)
+    size = 0.02 * position.float() * torch.where(position % 97 == 50, 6.0, 1.0) * torch.where(position > 1000, 0.3, 1.0)
+    k = (k.float() + size.clamp(max=25.0).view(-1, 1, 1) * towards / towards.norm()).to(dtype)
+    q = (q.float() + 4 * towards / towards.norm()).to(dtype)
+    at = offsets(lens)
+    for softcap in (0.0, 30.0):
+        o, lse = oat.omni_attention_packed(q, k, v, cu, softcap=softcap, return_lse=True)
+        _compare(o, lse, q, [(a, b - a, k[a:b], v[a:b]) for a, b in zip(at, at[1:])], True, softcap, dtype, "growing")
+
+
 def _paged(gen, device, dtype, lens, kv, Hq, Hk, D, page, behind=2, spare=2):
     T = sum(lens) + behind
     q = torch.randn(T, Hq, D, generator=gen).to(device=device, dtype=dtype)
@@ -258,3 +275,62 @@ def test_graph_replay_with_other_lengths_and_another_stream(gpu_device):
         for out in outs:
             for a, b in zip(out, eager):
                 assert torch.equal(a, b), rep
+
+
+def test_two_streams_at_once(gpu_device):
+    """Calls that run at the same time have workspaces of their own."""
+    gen = torch.Generator().manual_seed(14)
+    dtype, lens, kv, Hq, Hk, D = torch.bfloat16, [1, 1, 3], [9000, 700, 4000], 8, 2, 128
+    made = [_paged(gen, gpu_device, dtype, lens, kv, Hq, Hk, D, 32) for _ in range(2)]
+    call = lambda m: oat.omni_attention_paged(m[0], m[1][0], m[1][1], m[2], m[3], m[4], return_lse=True)
+    want = [call(m) for m in made]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=gpu_device) for _ in made]
+    for rep in range(5):
+        got = []
+        for stream, m in zip(streams, made):
+            with torch.cuda.stream(stream):
+                got.append([call(m) for _ in range(4)])
+        torch.cuda.synchronize()
+        for w, calls in zip(want, got):
+            for c in calls:
+                assert torch.equal(c[0], w[0]) and torch.equal(c[1], w[1]), rep
+
+
+def test_refusals_on_the_gpu(gpu_device):
+    gen = torch.Generator().manual_seed(15)
+    q, (kp, vp), table, kv_lens, cu, _ = _paged(gen, gpu_device, torch.float16, [1, 2], [20, 30], 4, 2, 64, 16)
+    paged = lambda **x: oat.omni_attention_paged(*[x.get(n, d) for n, d in (("q", q), ("kp", kp), ("vp", vp), ("table", table), ("kv", kv_lens), ("cu", cu))],
+                                                 softcap=x.get("softcap", 0.0))
+    rows = q[:, :2].contiguous()
+    append = lambda **x: oat.omni_cache_append(x.get("k", rows), rows, x.get("kp", kp), vp, table, kv_lens, cu, **x.get("more", {}))
+    packed = lambda **x: oat.omni_attention_packed(x.get("q", q), x.get("k", rows), x.get("v", rows), x.get("cu", cu))
+    angles = oat.omni_rotary_table(64, 40, device=gpu_device)
+    for call, match in (
+            (lambda: paged(q=q.float()), "float16"), (lambda: paged(q=q.bfloat16()), "dtype"), (lambda: paged(q=q[:, :3]), "multiple"),
+            (lambda: paged(q=q[:, :, :48]), "head_dim"), (lambda: paged(kp=kp[:, :, :12].contiguous(), vp=vp[:, :, :12].contiguous()), "page_size"),
+            (lambda: paged(kp=kp[:, :, :8].contiguous(), vp=vp[:, :, :8].contiguous()), "page_size"),
+            (lambda: paged(kp=kp.transpose(1, 2), vp=vp.transpose(1, 2)), "contiguous"), (lambda: paged(table=table.long()), "int32"),
+            (lambda: paged(kv=kv_lens[:1]), "cu_seqlens"), (lambda: paged(cu=cu.cpu()), "device"), (lambda: paged(table=table[:1]), "row per"),
+            (lambda: paged(softcap=-1.0), "softcap"), (lambda: paged(softcap=float("nan")), "softcap"), (lambda: paged(q=q.cpu()), "GPU"),
+            (lambda: paged(q=q.detach().requires_grad_()), "no_grad"), (lambda: append(k=rows.detach().requires_grad_()), "no_grad"),
+            (lambda: append(more=dict(query_norm=torch.ones(64, dtype=torch.float16, device=gpu_device))), "query"),
+            (lambda: append(more=dict(positions=cu[:1])), "table"), (lambda: append(more=dict(table=angles[:, :12])), "rotary_dim"),
+            (lambda: append(more=dict(table=angles.double())), "float32"), (lambda: append(more=dict(table=angles, positions=cu)), "one entry"),
+            (lambda: append(k=rows[:, :1]), "kv_heads"), (lambda: packed(k=rows[:1]), "kv_heads"), (lambda: packed(cu=cu[:0]), "entry"),
+            (lambda: packed(v=rows.bfloat16()), "dtype"),
+            (lambda: oat.omni_qk_rotary(q, rows, cu, angles), "one entry"), (lambda: oat.omni_qk_rotary(q, rows[:1], cu, angles), "tokens"),
+            (lambda: oat.omni_qk_rotary(q[..., :60], rows[..., :60], torch.zeros(5, dtype=torch.int64, device=gpu_device), angles), "head_dim"),
+            (lambda: oat.omni_qk_rotary(q, rows, torch.zeros(5, device=gpu_device), angles), "int32"),
+            (lambda: oat.omni_qk_rotary(q, rows, torch.zeros(5, dtype=torch.int64, device=gpu_device), angles, eps=-1.0), "eps"),
+            (lambda: oat.omni_qk_rotary(q, rows, torch.zeros(5, dtype=torch.int64, device=gpu_device), angles,
+                                        key_norm=torch.ones(32, dtype=torch.float16, device=gpu_device)), "key_norm")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    with torch.inference_mode():  # pages made here may be written here
+        inside = kp.clone(), vp.clone()
+        oat.omni_cache_append(rows, rows, *inside, table, kv_lens, cu)
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        oat.omni_cache_append(rows, rows, *inside, table, kv_lens, cu)
+    with torch.no_grad():
+        paged(q=q.detach().requires_grad_())
