@@ -71,9 +71,11 @@ omni_attn_strides strides_of(const Tensor& t) {
 }
 // A result in the memory order of its operand (a projection's [B, S, H, D] seen as [B, H, S, D] stays that).
 Tensor result_like(const Tensor& t) {
-  if (t.dim() == 4 && t.stride(1) < t.stride(2))
-    return torch::empty({t.size(0), t.size(2), t.size(1), t.size(3)}, t.options()).transpose(1, 2);
-  return torch::empty(t.sizes(), t.options());
+  if (t.dim() == 4 && t.stride(1) < t.stride(2)) {
+    const int64_t B = t.size(0), H = t.size(1), S = t.size(2), D = t.size(3);
+    return at::empty_strided({B, H, S, D}, {S * H * D, D, H * D, 1}, t.options());
+  }
+  return at::empty(t.sizes(), t.options());
 }
 
 // ---- norm and rotation ------------------------------------------------------------------------------
@@ -146,18 +148,14 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     const Tensor wq = query_norm.value_or(Tensor()), wk = key_norm.value_or(Tensor());
     r.wq = wq;
     r.wk = wk;
-    ctx->saved_data["want_wq"] = wq.defined() && wq.requires_grad();
-    ctx->saved_data["want_wk"] = wk.defined() && wk.requires_grad();
     q = in_rows(q, 4);
     k = in_rows(k, 4);
     auto out = rotate(q, k, r);
-    // a rotation alone needs no inputs for its gradient
+    // (a rotation alone needs no inputs for its gradient)
     ctx->save_for_backward({wq.defined() ? q : Tensor(), wk.defined() ? k : Tensor(), r.positions, r.table, wq, wk});
     ctx->saved_data["eps"] = r.eps;
-    ctx->saved_data["interleaved"] = r.interleaved;
-    ctx->saved_data["pos_b"] = r.pos_b;
-    ctx->saved_data["q_like"] = std::vector<int64_t>(q.sizes().begin(), q.sizes().end());
-    ctx->saved_data["k_like"] = std::vector<int64_t>(k.sizes().begin(), k.sizes().end());
+    ctx->saved_data["how"] = r.pos_b * 8 + int64_t(r.interleaved) * 4 + int64_t(wq.defined() && wq.requires_grad()) * 2 +
+                             int64_t(wk.defined() && wk.requires_grad());
     return {out.first, out.second};
   }
 
@@ -172,18 +170,14 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     r.wq = saved[4];
     r.wk = saved[5];
     r.eps = ctx->saved_data["eps"].toDouble();
-    r.interleaved = ctx->saved_data["interleaved"].toBool();
-    r.pos_b = ctx->saved_data["pos_b"].toInt();
-    const std::vector<int64_t> q_size = ctx->saved_data["q_like"].toIntVector(), k_size = ctx->saved_data["k_like"].toIntVector();
-    Tensor dqo = grads[0], dko = grads[1];
+    const int64_t how = ctx->saved_data["how"].toInt();
+    r.interleaved = (how & 4) != 0;
+    r.pos_b = how >> 3;
     c10::DeviceGuard guard(r.table.device());
-    // (an output that nothing was computed from has no gradient)
-    if (!dqo.defined()) dqo = torch::zeros(q_size, dko.options());
-    if (!dko.defined()) dko = torch::zeros(k_size, dqo.options());
-    dqo = in_rows(dqo, 4);
-    dko = in_rows(dko, 4);
+    // (the gradient of an output that nothing was computed from comes as zeros)
+    const Tensor dqo = in_rows(grads[0], 4), dko = in_rows(grads[1], 4);
     Tensor dq = result_like(dqo), dk = result_like(dko);
-    const bool want_wq = ctx->saved_data["want_wq"].toBool(), want_wk = ctx->saved_data["want_wk"].toBool();
+    const bool want_wq = (how & 2) != 0, want_wk = (how & 1) != 0;
     Tensor dwq, dwk, workspace;
     const bool flat = dqo.dim() == 3;
     const int64_t B = flat ? 1 : dqo.size(0), S = flat ? dqo.size(0) : dqo.size(2), D = dqo.size(-1);
