@@ -337,7 +337,7 @@ void check_heads(const Tensor& q, int64_t Hk, int64_t D) {
   if (D != 32 && D != 64 && D != 128)
     refuse("Unsupported head_dim=" + std::to_string(D) + ". Supported values: 32, 64, 128.");
   require(q.size(1) >= 1 && Hk >= 1 && q.size(1) % Hk == 0, "the number of query heads must be a multiple of the key heads'");
-  require(q.size(0) * q.size(1) <= 0x3fffffff, "query has too many rows");
+  require(q.size(1) <= 65536 && q.size(0) * q.size(1) <= 0x3fffffff, "query has too many rows");
 }
 void check_softcap(double softcap) {
   if (!(softcap >= 0) || std::isinf(softcap)) refuse("softcap must be 0 (off) or positive and finite");

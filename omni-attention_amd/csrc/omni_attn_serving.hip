@@ -44,8 +44,8 @@ int check_rows(const omni_attn_strides& at) {
 int check_sizes(int T, int B, int Hq, int Hk, int D) {
   if (D != 32 && D != 64 && D != 128) return OMNI_ATTN_ERR_UNSUPPORTED_HEAD_DIM;
   if (T <= 0 || B <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk != 0) return OMNI_ATTN_ERR_BAD_SHAPE;
-  // (rows of a key head, and rows in all, are numbered with an int)
-  if ((long long)T * Hq > 0x3fffffffLL || (long long)B * Hk > 0x3fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
+  // (rows of a key head, and rows in all, are numbered with an int; a wave's rows lie within 32-bit offsets)
+  if (Hq > 65536 || (long long)T * Hq > 0x3fffffffLL || (long long)B * Hk > 0x3fffffffLL) return OMNI_ATTN_ERR_TOO_LARGE;
   return OMNI_ATTN_OK;
 }
 

@@ -228,9 +228,9 @@ __device__ __forceinline__ Unit find_tile(const ServeParams& p, const Batch& bat
   auto long_tiles = [&](int steps) {
     if (steps <= 0) return tiles;
     if (!p.causal) return steps_of(s.kv) >= steps ? tiles : 0;
-    const int64_t token = int64_t(kStepKeys) * (steps - 1) - (s.kv - s.n);  // first token whose keys reach so far
-    if (token >= s.n) return 0;
-    return token <= 0 ? tiles : tiles - int((token * p.G) >> kLog);
+    const int token = kStepKeys * (steps - 1) - (s.kv - s.n);  // first token whose keys reach so far
+    const int row = (token < s.n ? token : s.n) * p.G;
+    return token >= s.n ? 0 : (token <= 0 ? tiles : tiles - (row >> kLog));
   };
   const int all = wave_sum(tiles);
   if (all <= rank) return Unit{{}, 0, 0, all, 0, 0, 1, false, false};
@@ -399,16 +399,20 @@ __device__ __forceinline__ void store_rows(const ServeParams& p, const Unit& u, 
       *reinterpret_cast<u32x2_t*>(stage + c * D + ((4 * dt + r4) ^ k_swizzle<D>(c)) * 8 + 4 * g) = ov;
     }
   constexpr int CPR = D / 8, RPS = 64 / CPR;
-  const int pch = lane % CPR;
+  // (rows of o: the wave's first token and head, and 32-bit offsets from there)
+  const int pch = lane % CPR, token0 = __builtin_amdgcn_readfirstlane(int(divide(uint32_t(row0), p.group)));
+  uint16_t* const o = p.o + (int64_t(u.seq.first + token0) * p.Hk + head) * p.G * D;
+  const uint32_t token_step = uint32_t(p.Hk * p.G - p.G) * D;
 #pragma unroll
   for (int i = 0; i < 32 / RPS; ++i) {
     const int row = i * RPS + lane / CPR;
     const u32x4_t val = *reinterpret_cast<const u32x4_t*>(stage + row * D + pch * 8);
     const int r = row0 + row;
     if (r < rows_all && !(skip >> row & 1)) {
-      const int token = int(divide(uint32_t(r), p.group));
-      const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (r - token * p.G);
-      *reinterpret_cast<u32x4_t*>(p.o + at * D + (pch ^ k_swizzle<D>(row)) * 8) = val;
+      // (token - token0) heads of all groups and r - token G of this one: r - token0 G of this one, and the tokens' rest
+      const uint32_t token = divide(uint32_t(r), p.group) - uint32_t(token0);
+      const uint32_t at = token * token_step + uint32_t(r - token0 * p.G) * D + uint32_t(pch ^ k_swizzle<D>(row)) * 8u;
+      *reinterpret_cast<u32x4_t*>(o + at) = val;
     }
   }
   if (p.lse != nullptr && g == 0 && row0 + c < rows_all && !(skip >> c & 1)) {

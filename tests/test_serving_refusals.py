@@ -102,8 +102,27 @@ def test_attention_codes():
         assert paged(**bad) == 2, bad
     assert packed(D=96) == 3 and paged(D=256) == 3
     assert packed(dtype=3) == 5
-    assert packed(T=1 << 29) == 7 and paged(width=1 << 27) == 7 and packed(at=Strides(0, 128, 1 << 30)) == 7
+    assert packed(T=1 << 29) == 7 and packed(T=1, Hq=1 << 18) == 7 and paged(width=1 << 27) == 7 and packed(at=Strides(0, 128, 1 << 30)) == 7
     assert packed(q=ctypes.c_void_p(4104)) == 8 and packed(at=Strides(0, 124, 1024)) == 8
+
+
+def test_packed_backward_codes():
+    lib = omni_attn_capi.load_library()
+    f = lib.omni_attn_packed_bwd_gfx950
+
+    def call(q=ONE, dq=ONE, lse=ONE, at=AT, ws=ONE, size=1 << 20, T=4, B=1, Hq=4, Hk=2, D=64, dtype=0, cap=0.0):
+        return f(q, ONE, ONE, ONE, ONE, lse, at, AT, AT, AT, dq, ONE, ONE, ONE, ws, ctypes.c_size_t(size), T, B, Hq, Hk, D, 1, dtype,
+                 ctypes.c_float(cap), NULL)
+
+    assert call(q=NULL) == 1 and call(dq=NULL) == 1 and call(lse=NULL) == 1
+    for bad in (dict(T=0), dict(B=0), dict(Hq=3), dict(cap=-1.0), dict(cap=float("nan"))):
+        assert call(**bad) == 2, bad
+    assert call(D=96) == 3 and call(dtype=2) == 5
+    assert call(at=Strides(0, 128, 1 << 25)) == 7 and call(at=Strides(0, 1 << 30, 1024)) == 7
+    assert call(dq=ctypes.c_void_p(4104)) == 8 and call(at=Strides(0, 124, 1024)) == 8
+    assert call(ws=NULL) == 9 and call(size=60) == 9
+    lib.omni_attn_packed_bwd_workspace_bytes.restype = ctypes.c_size_t
+    assert lib.omni_attn_packed_bwd_workspace_bytes(4, 4) == 64 and lib.omni_attn_packed_bwd_workspace_bytes(0, 4) == 0
 
 
 @pytest.mark.parametrize("rot,scaling,factor", [(64, None, 1.0), (8, "linear", 4.0), (128, "ntk", 8.0), (128, "yarn", 16.0), (32, "yarn", 1.0)])
