@@ -394,8 +394,8 @@ __device__ __forceinline__ void store_rows(const ServeParams& p, const Unit& u, 
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       u32x2_t ov;
-      ov[0] = pack2<BF16>(live ? ot[dt][4 * r4 + 0] * inv : 0.f, live ? ot[dt][4 * r4 + 1] * inv : 0.f);
-      ov[1] = pack2<BF16>(live ? ot[dt][4 * r4 + 2] * inv : 0.f, live ? ot[dt][4 * r4 + 3] * inv : 0.f);
+      ov[0] = pack2<BF16>(ot[dt][4 * r4 + 0] * inv, ot[dt][4 * r4 + 1] * inv);
+      ov[1] = pack2<BF16>(ot[dt][4 * r4 + 2] * inv, ot[dt][4 * r4 + 3] * inv);
       *reinterpret_cast<u32x2_t*>(stage + c * D + ((4 * dt + r4) ^ k_swizzle<D>(c)) * 8 + 4 * g) = ov;
     }
   constexpr int CPR = D / 8, RPS = 64 / CPR;
@@ -895,18 +895,8 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
 
   const f32x16_t zero16 = {};
   f32x16_t ot[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) ot[dt] = zero16;
-  f32x16_t st[2][NTL];
+  f32x16_t st[2][NTL];   // (written by the first products, and the first softmax)
   u32x4_t pb[2][NTL][2];
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int t = 0; t < NTL; ++t) {
-      st[a][t] = zero16;
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) pb[a][t][s2] = u32x4_t{0u, 0u, 0u, 0u};
-    }
   float m_run = -INFINITY, m_ref = 0.f, l_run = 0.f, alpha_pending = 1.f;
   constexpr uint32_t kOwesRescale = 1, kOwesLook = 2;
   uint32_t owed = kOwesLook;
@@ -1062,6 +1052,12 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
 #pragma unroll
       for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 1, from_kg + NEXT, 0, r1, r1);
     }
+  }
+  // (while the first tiles are on their way)
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) ot[dt] = zero16;
+  if (nsteps > 0) {
     wait_loads_but<NCH>();  // K(1) may be under way
     __syncthreads();
 #pragma unroll
