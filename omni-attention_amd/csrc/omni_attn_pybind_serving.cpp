@@ -60,6 +60,11 @@ Tensor in_rows(const Tensor& t, int64_t piece) {
   ok = ok && (t.dim() == 3 ? t.stride(0) <= (1 << 24) && t.stride(1) <= (1 << 30) : t.stride(2) <= 0x7fffffff);
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
+// ... for the gradients of packed sequences, too: a step's rows, of every head, within 3 GiB.
+Tensor in_near_rows(const Tensor& t) {
+  const Tensor r = in_rows(t, 8);
+  return 66 * r.stride(0) + r.size(1) * r.stride(1) <= 0x5f000000 ? r : r.clone(at::MemoryFormat::Contiguous);
+}
 Tensor aligned(const Tensor& t) {  // contiguous and on a 16-byte boundary
   if (t.is_contiguous() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) return t;
   return t.clone(at::MemoryFormat::Contiguous);
@@ -379,6 +384,9 @@ class PackedFunction : public torch::autograd::Function<PackedFunction> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, Tensor q, Tensor k, Tensor v, const Packed& m) {
     Tensor lse;
+    q = in_near_rows(q);
+    k = in_near_rows(k);
+    v = in_near_rows(v);
     Tensor out = attend_packed(q, k, v, m, &lse);
     ctx->save_for_backward({q, k, v, out, lse, m.cu});
     ctx->saved_data["causal"] = m.causal;
@@ -395,7 +403,7 @@ class PackedFunction : public torch::autograd::Function<PackedFunction> {
     const int64_t T = q.size(0), B = cu.size(0) - 1, Hq = q.size(1), Hk = k.size(1), D = q.size(2);
     c10::DeviceGuard guard(q.device());
     if (T == 0 || B == 0) return {torch::zeros_like(q), torch::zeros_like(k), torch::zeros_like(v), Tensor()};
-    const Tensor dout = in_rows(grads[0], 8);
+    const Tensor dout = in_near_rows(grads[0]);
     Tensor dq = torch::empty({T, Hq, D}, q.options()), dk = torch::empty({T, Hk, D}, q.options()), dv = torch::empty({T, Hk, D}, q.options());
     const size_t bytes = omni_attn_packed_bwd_workspace_bytes(int(T), int(Hq));
     Tensor workspace = torch::empty({int64_t(bytes / 4)}, lse.options());

@@ -171,3 +171,25 @@ def test_many_tiles_and_a_graph(gpu_device):
         torch.cuda.synchronize()
         for a, b in zip(captured, eager):
             assert torch.equal(a, b), lens
+
+
+def test_heads_that_lie_far_apart(gpu_device):
+    """Heads 2^30 elements from one another: the gradients' steps of rows reach over 3 GiB of them."""
+    gen = torch.Generator().manual_seed(6)
+    dtype, lens, Hq, Hk, D = torch.bfloat16, [70, 30], 2, 1, 32
+    T = sum(lens)
+    q, k, v, do = _inputs(gen, gpu_device, dtype, T, Hq, Hk, D)
+    cu = torch.tensor(offsets(lens), dtype=torch.int32, device=gpu_device)
+    far = torch.zeros((1 << 30) + T * D, dtype=dtype, device=gpu_device).as_strided((T, Hq, D), (D, 1 << 30, 1))
+    near = [t.requires_grad_() for t in (q, k, v)]
+    out = oat.omni_attention_packed(*near, cu)
+    want = torch.autograd.grad(out, near, do)
+    far.copy_(q.detach())
+    leaves = [far.requires_grad_(), k, v]
+    got = torch.autograd.grad(oat.omni_attention_packed(*leaves, cu), leaves, do)
+    with torch.no_grad():
+        assert torch.equal(oat.omni_attention_packed(far, k, v, cu), out)
+        far.copy_(do)
+    again = torch.autograd.grad(oat.omni_attention_packed(*near, cu), near, far.detach())
+    for a, b, c in zip(want, got, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
