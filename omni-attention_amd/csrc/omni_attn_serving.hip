@@ -56,6 +56,40 @@ int check_pages(int num_pages, int page_size, int max_pages) {
   return (long long)max_pages * page_size > 0x3fffffffLL ? OMNI_ATTN_ERR_TOO_LARGE : OMNI_ATTN_OK;
 }
 
+// Counts the units of more sequences than a wave has lanes, in one workgroup.
+template <int M>
+__global__ void __launch_bounds__(1024) serve_count_kernel(const ServeParams p) {
+  __shared__ float steps[16];
+  __shared__ int units[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  float all = 0.f;
+  for (int b = tid; b < p.B; b += 1024) {
+    const Sequence s = sequence_of(p, b);
+    all += float(tiles_of<M>(p, s)) * float(steps_of(s.kv));
+  }
+  all = wave_sum(all);
+  if (lane == 0) steps[w] = all;
+  __syncthreads();
+  all = 0.f;
+  for (int i = 0; i < 16; ++i) all += steps[i];
+  const int most = part_steps(p, all);
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 1024) {
+    const Sequence s = sequence_of(p, b0 + tid);
+    const int end = wave_scan(tiles_of<M>(p, s) * parts_of(s.kv, most).n);
+    if (lane == 63) units[w] = end;
+    __syncthreads();
+    int here = before;
+    for (int i = 0; i < 16; ++i) {
+      if (i < w) here += units[i];
+      before += units[i];
+    }
+    if (b0 + tid < p.B) p.ends[b0 + tid] = here + end;
+    __syncthreads();
+  }
+  if (tid == 0) p.ends[p.B] = most;
+}
+
 int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes, int dtype, float softcap, void* stream) {
   if (!(softcap >= 0.f) || std::isinf(softcap)) return OMNI_ATTN_ERR_BAD_SHAPE;
   if (dtype != OMNI_ATTN_DTYPE_F16 && dtype != OMNI_ATTN_DTYPE_BF16) return OMNI_ATTN_ERR_UNSUPPORTED_DTYPE;
@@ -65,7 +99,6 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
     return OMNI_ATTN_ERR_LAUNCH;
   }
   p.G = Hq / p.Hk;
-  p.per_lane = (p.B + 63) / 64;
   p.group = fast_div(uint32_t(p.G));
   p.heads = fast_div(uint32_t(p.Hk));
   const ServePlan plan = plan_serve(p.T, p.B, p.Hk, p.G, p.page_table != nullptr ? int64_t(p.max_pages) << p.page_shift : 0, cus);
@@ -80,6 +113,7 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
     p.sums = static_cast<float*>(workspace);
     p.stats = p.sums + plan.units * p.Hk * plan.rows * D;
     p.joins = reinterpret_cast<int32_t*>(p.stats + plan.units * p.Hk * plan.rows * 2);
+    p.ends = plan.counted != 0 ? p.joins + int64_t(p.T) * 4 : nullptr;
   }
   p.softcap = softcap;
   p.cap_c2 = softcap > 0.f ? float(2.0 * 1.4426950408889634 / (std::sqrt(double(D)) * double(softcap))) : 0.f;
@@ -87,8 +121,13 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool bf = dtype == OMNI_ATTN_DTYPE_BF16;
   const unsigned n = unsigned(blocks);
-  int e;
-  switch (D) {
+  int e = 0;
+  if (p.ends != nullptr) {
+    if (plan.rows == 128) hipLaunchKernelGGL((serve_count_kernel<128>), dim3(1), dim3(1024), 0, s, p);
+    else hipLaunchKernelGGL((serve_count_kernel<32>), dim3(1), dim3(1024), 0, s, p);
+    e = int(hipGetLastError());
+  }
+  if (e == 0) switch (D) {
     case 32: e = bf ? launch_serve<true, 32>(p, plan.rows, plan.waves, n, s) : launch_serve<false, 32>(p, plan.rows, plan.waves, n, s); break;
     case 64: e = bf ? launch_serve<true, 64>(p, plan.rows, plan.waves, n, s) : launch_serve<false, 64>(p, plan.rows, plan.waves, n, s); break;
     default: e = bf ? launch_serve<true, 128>(p, plan.rows, plan.waves, n, s) : launch_serve<false, 128>(p, plan.rows, plan.waves, n, s); break;
@@ -197,7 +236,6 @@ extern "C" int omni_attn_packed_bwd_gfx950(const void* q, const void* k, const v
   p.B = sequences;
   p.T = tokens;
   p.Hk = Hk;
-  p.per_lane = (sequences + 63) / 64;
   p.heads = fast_div(uint32_t(Hk));
   p.causal = causal != 0;
   p.softcap = softcap;

@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(256 * KG, 2) serve_dkdv_kernel(const ServeBwdP
   if (rank >= p.units) return;
   const Unit u = find_unit<M>(p, rank, lane);
   if (!u.found) {  // keys of tokens behind the last sequence have no gradient
+    if (rank < u.step0) return;
     int used = p.cu[p.B];
     used = used < 0 ? 0 : used;
     for (int64_t t = int64_t(used) + (rank - u.step0); t < p.T; t += p.units - u.step0)

@@ -10,10 +10,9 @@
 // the G heads of a group: the rows of a tile share one key head, so K and V are read once for all of them, a single
 // token fills G rows, and a tile of a prompt has few tokens, so little of its last steps is masked.
 //
-// Work is dealt on the device, because lengths are there: every workgroup reads the lengths (64 sequences per wave at
-// a time) and finds the unit with its number.  A unit is a tile of rows and a range of keys (all of them, or where
-// there are fewer units than the card holds, parts that are equal over the whole batch).  Parts leave their sums
-// and maxima in a workspace, and a second kernel joins them.
+// Work is dealt on the device, because lengths are there: every workgroup finds the unit with its number.  A unit is a
+// tile of rows and a range of keys (all of them, or where there are fewer units than the card holds, parts that are equal
+// over the whole batch).  Parts leave their sums and maxima in a workspace, and a second kernel joins them.
 #pragma once
 
 #include "omni_attn_fwd_kernel.hpp"
@@ -33,7 +32,6 @@ struct ServeParams {
   const int32_t* page_table;  // [B, max_pages]
   int num_pages, max_pages, page_shift;
   int B, T, Hk, G;
-  int per_lane;        // sequences per lane of a wave: B / 64, up
   FastDiv group;       // by G
   FastDiv heads;       // by Hk
   int n_xcd;
@@ -41,6 +39,7 @@ struct ServeParams {
   float share;         // units per key head that the batch's steps are shared over; 0: whole tiles
   int least_steps;     // ... and the steps that a part may have in any case
   int units;           // units per key head that there is a place for
+  int32_t* ends;       // [B + 1] of batches that a kernel of its own counts: units up to and with each sequence; steps of a part
   float* sums;         // [units, Hk, M, D] unscaled O of parts
   float* stats;        // [units, Hk, M, 2] their reference points (log2 domain) and sums of weights
   int32_t* joins;      // [T, 4] of a token: first token and number of parts of its sequence, number of its first unit
@@ -111,59 +110,20 @@ __device__ __forceinline__ int tiles_of(const ServeParams& p, const Sequence& s)
 }
 __device__ __forceinline__ int steps_of(int keys) { return (keys + kStepKeys - 1) / kStepKeys; }
 
-// The sequences of a batch: a lane has p.per_lane neighbours.  Up to eight of them stay in registers, asked for together.
-struct Batch {
-  static constexpr int kKept = 8;
-  Sequence own[kKept];
-  __device__ __forceinline__ Batch(const ServeParams& p, int lane) {
-#pragma unroll
-    for (int i = 0; i < kKept; ++i) own[i] = Sequence{0, 0, 0};
-    own[0] = sequence_of(p, lane * p.per_lane);
-    if (p.per_lane > 1) {
-#pragma unroll
-      for (int i = 1; i < kKept; ++i) own[i] = sequence_of(p, i < p.per_lane ? lane * p.per_lane + i : p.B);
-    }
-  }
-  // f(sequence) summed over a lane's sequences.
-  template <class F>
-  __device__ __forceinline__ auto sum(const ServeParams& p, int lane, F&& f) const {
-    auto all = f(own[0]);
-    if (p.per_lane > 1) {
-#pragma unroll
-      for (int i = 1; i < kKept; ++i) all += f(own[i]);
-      for (int i = kKept; i < p.per_lane; ++i) all += f(sequence_of(p, lane * p.per_lane + i));
-    }
-    return all;
-  }
-};
 __device__ __forceinline__ Sequence pick(const Sequence& s, int lane) {
   return {__builtin_amdgcn_readlane(s.first, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.kv, lane)};
 }
-// Of numbers 0, 1, ... given out to the sequences in order, f(sequence) to each: who has number `rank`.
-struct Place {
-  Sequence seq;
-  int b, in;  // the sequence, and which of its numbers; b -1: nobody's, of `in` that were given out
-};
+// How many of at(1) .. at(n), which do not decrease, are at most `rank`: 64 of them are looked at in a round.
 template <class F>
-__device__ __forceinline__ Place place_of(const ServeParams& p, const Batch& batch, int rank, int lane, F&& f) {
-  const int mine = batch.sum(p, lane, f), end = wave_scan(mine);
-  const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
-  if (beyond == 0) return Place{{}, -1, __builtin_amdgcn_readlane(end, 63)};
-  const int at = __builtin_ctzll(beyond);
-  rank -= __builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(mine, at);
-  if (p.per_lane == 1) return Place{pick(batch.own[0], at), at, rank};
-  for (int i0 = 0;; i0 += 64) {  // (one of the lane's sequences has it)
-    const int i = i0 + lane;
-    const Sequence s = sequence_of(p, i < p.per_lane ? at * p.per_lane + i : p.B);
-    const int n = f(s), last = wave_scan(n);
-    const uint64_t here = __builtin_amdgcn_ballot_w64(last > rank);
-    if (here != 0 || i0 + 64 >= p.per_lane) {
-      const int who = here != 0 ? __builtin_ctzll(here) : 0;
-      return Place{pick(s, who), at * p.per_lane + i0 + who,
-                   rank - (__builtin_amdgcn_readlane(last, who) - __builtin_amdgcn_readlane(n, who))};
-    }
-    rank -= __builtin_amdgcn_readlane(last, 63);
+__device__ __forceinline__ int count_up_to(int n, int rank, int lane, F&& at) {
+  int count = 0;
+  for (int left = n; left > 0;) {
+    const int step = (left + 63) / 64, i = (lane + 1) * step;
+    const int passed = __builtin_popcountll(__builtin_amdgcn_ballot_w64(i <= left && at(i <= left ? count + i : n) <= rank)) * step;
+    count += passed;
+    left = left - passed < step - 1 ? left - passed : step - 1;
   }
+  return count;
 }
 
 // A sequence's keys in parts of at most `most` steps: as few as that takes, as even as whole steps allow.
@@ -176,50 +136,74 @@ __device__ __forceinline__ Parts parts_of(int kv, int most) {
   const int n = int(uint32_t(all + most - 1) / uint32_t(most)), each = int(uint32_t(all + n - 1) / uint32_t(n));
   return {int(uint32_t(all + each - 1) / uint32_t(each)), each};
 }
-// The most steps of a part: the batch's steps over the units that they are shared by.  (The same number in every
-// wave: the same sums in the same order.)
-template <int M>
-__device__ __forceinline__ int part_steps(const ServeParams& p, const Batch& batch, int lane) {
-  const float all = wave_sum(batch.sum(p, lane, [&](const Sequence& s) { return float(tiles_of<M>(p, s)) * float(steps_of(s.kv)); }));
+// The most steps of a part: the batch's steps (of all tiles) over the units that they are shared by.
+__device__ __forceinline__ int part_steps(const ServeParams& p, float all) {
   const float steps = ceilf(all / p.share);
   const int part = steps < 1e9f ? int(steps) : 1000000000;
   return __builtin_amdgcn_readfirstlane(part < p.least_steps ? p.least_steps : part);
 }
 
+constexpr int kAll = 0x7fffffff;
 struct Unit {
   Sequence seq;
   int b, tile;
   int step0, steps;  // range of steps (all that the tile has may be fewer)
   int base, parts;   // (shared by parts) number of the sequence's first unit, parts of each of its tiles
   bool part;         // one of several: its sums are joined later
-  bool found;        // no: step0 is the number of units that there are
+  bool found;        // no: (whole tiles) step0 is the number behind the last unit's (kAll: this number is left out)
 };
 
-// Unit number `rank` of tiles that are shared by parts: sequences in order, tiles in order, parts in order.
+// Unit number `rank` of tiles that are shared by parts: sequences in order, tiles in order, parts in order.  Up to 64
+// sequences, one per lane, are counted by every wave (the same numbers in each: the same sums in the same order); more, by
+// a kernel that goes before (512 single tokens after 500 - 1000 keys, 8 / 1 heads, D=128: 48 us, 54 with every wave counting
+// eight per lane; 4096 of them, 32 / 8 heads, 2.1 ms and 5.7).
 template <int M>
-__device__ __forceinline__ Unit find_part(const ServeParams& p, const Batch& batch, int rank, int lane) {
-  const int most = part_steps<M>(p, batch, lane);
-  const Place at = place_of(p, batch, rank, lane, [&](const Sequence& s) { return tiles_of<M>(p, s) * parts_of(s.kv, most).n; });
-  if (at.b < 0) return Unit{{}, 0, 0, at.in, 0, 0, 0, false, false};
-  const Parts parts = parts_of(at.seq.kv, most);
-  const int tile = int(uint32_t(at.in) / uint32_t(parts.n));
-  return Unit{at.seq, at.b, tile, (at.in - tile * parts.n) * parts.steps, parts.steps, rank - at.in, parts.n, parts.n > 1, true};
+__device__ __forceinline__ Unit find_part(const ServeParams& p, int rank, int lane) {
+  Sequence s;
+  int b, most, in;
+  if (p.ends != nullptr) {
+    most = load_uniform(p.ends + p.B);
+    b = count_up_to(p.B, rank, lane, [&](int i) { return p.ends[i - 1]; });
+    if (b == p.B) return Unit{{}, 0, 0, 0, 0, 0, 0, false, false};
+    s = pick(sequence_of(p, b), 0);
+    in = rank - (b == 0 ? 0 : load_uniform(p.ends + b - 1));
+  } else {
+    const Sequence own = sequence_of(p, lane);
+    const int tiles = tiles_of<M>(p, own);
+    most = part_steps(p, wave_sum(float(tiles) * float(steps_of(own.kv))));
+    const int mine = tiles * parts_of(own.kv, most).n, end = wave_scan(mine);
+    const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
+    if (beyond == 0) return Unit{{}, 0, 0, 0, 0, 0, 0, false, false};
+    b = __builtin_ctzll(beyond);
+    s = pick(own, b);
+    in = rank - (__builtin_amdgcn_readlane(end, b) - __builtin_amdgcn_readlane(mine, b));
+  }
+  const Parts parts = parts_of(s.kv, most);
+  const int tile = int(uint32_t(in) / uint32_t(parts.n));
+  return Unit{s, b, tile, (in - tile * parts.n) * parts.steps, parts.steps, rank - in, parts.n, parts.n > 1, true};
 }
 
 // Unit number `rank` of whole tiles.  Of up to 64 sequences those with most steps come first, so that a launch ends with
-// short ones: steps are compared in sixteen levels, which four rounds of counting find.  More sequences come in order,
-// the last tile of each first.
+// short ones: steps are compared in sixteen levels, which four rounds of counting find.  One sequence, or more than 64, in
+// order, the last tile of each first.  Their numbers need no counting: the tiles of sequence b start at number
+// floor(cu[b] G / M) + b, which leaves room for all that the sequences before it can have, and out one number for some.
 template <int M>
-__device__ __forceinline__ Unit find_tile(const ServeParams& p, const Batch& batch, int rank, int lane) {
+__device__ __forceinline__ Unit find_tile(const ServeParams& p, int rank, int lane) {
   constexpr int kLog = M == 128 ? 7 : (M == 64 ? 6 : 5);
   static_assert(M == 1 << kLog, "rows of a tile");
-  constexpr int kAll = 0x7fffffff;
-  if (p.B == 1 || p.per_lane > 1) {
-    const Place at = place_of(p, batch, rank, lane, [&](const Sequence& s) { return tiles_of<M>(p, s); });
-    if (at.b < 0) return Unit{{}, 0, 0, at.in, 0, 0, 1, false, false};
-    return Unit{at.seq, at.b, tiles_of<M>(p, at.seq) - 1 - at.in, 0, kAll, 0, 1, false, true};
+  if (p.B == 1 || p.B > 64) {
+    const auto start = [&](int b) {
+      int from = b == 0 ? 0 : p.cu[b];
+      from = from < 0 ? 0 : (from > p.T ? p.T : from);
+      return int(uint32_t(from) * uint32_t(p.G) >> kLog) + b;
+    };
+    const int b = count_up_to(p.B, rank, lane, start), first = __builtin_amdgcn_readfirstlane(start(b));
+    if (b == p.B) return Unit{{}, 0, 0, first, 0, 0, 1, false, false};
+    const Sequence s = pick(sequence_of(p, b), 0);
+    const int tile = tiles_of<M>(p, s) - 1 - (rank - first);
+    return Unit{s, b, tile, tile < 0 ? kAll : 0, kAll, 0, 1, false, tile >= 0};
   }
-  const Sequence& s = batch.own[0];
+  const Sequence s = sequence_of(p, lane);
   const int most = wave_max(s.n > 0 ? steps_of(s.kv) : 0);
   int unit = 0;  // log2 of the steps of a level
   while ((most >> unit) > 15) ++unit;
@@ -254,8 +238,7 @@ __device__ __forceinline__ Unit find_tile(const ServeParams& p, const Batch& bat
 }
 template <int M>
 __device__ __forceinline__ Unit find_unit(const ServeParams& p, int rank, int lane) {
-  const Batch batch(p, lane);
-  return p.share > 0.f ? find_part<M>(p, batch, rank, lane) : find_tile<M>(p, batch, rank, lane);
+  return p.share > 0.f ? find_part<M>(p, rank, lane) : find_tile<M>(p, rank, lane);
 }
 
 // Workgroup -> (key head, rank).  Ids go round-robin over the XCDs: the heads are dealt to the XCDs, so that the
@@ -276,10 +259,10 @@ __device__ __forceinline__ void deal_head(const ServeParams& p, int id, int& hea
   }
 }
 
-// Rows of tokens behind the last sequence are zeros: their workgroups are those without a unit, the first of which is
-// number `units`.
+// Rows of tokens behind the last sequence are zeros: their workgroups are those from number `units` on, which have no unit.
 template <int D>
 __device__ void clear_rows(const ServeParams& p, int head, int rank, int units, int ranks, int tid, int threads) {
+  if (rank < units) return;
   int used = p.cu[p.B];
   used = used < 0 ? 0 : used;
   for (int64_t t = int64_t(used) + (rank - units); t < p.T; t += ranks - units) {

@@ -13,8 +13,11 @@ struct ServePlan {
   float share;     // units per key head that the steps are shared over, 0: whole tiles
   int least_steps; // steps that a part may have in any case
   int64_t units;   // units per key head that there is a place for
-  size_t workspace_bytes(int64_t T, int Hk, int D) const {  // the parts' rows and statistics, and four words per token
-    return share == 0.f ? 0 : size_t(units) * size_t(Hk) * size_t(rows) * size_t(D + 2) * sizeof(float) + size_t(T) * 16;
+  int64_t counted; // sequences whose units a kernel of its own counts, or 0
+  // the parts' rows and statistics, four words per token, one per counted sequence and one more
+  size_t workspace_bytes(int64_t T, int Hk, int D) const {
+    if (share == 0.f) return 0;
+    return size_t(units) * size_t(Hk) * size_t(rows) * size_t(D + 2) * sizeof(float) + size_t(T) * 16 + size_t(counted) * 4 + 4;
   }
 };
 
@@ -57,6 +60,7 @@ inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, int64_t capacit
   }
   const int64_t tiles = tiles_of(s.rows);
   const bool parts = wanted != 0;
+  s.counted = parts && B > 64 ? B : 0;
   s.share = parts ? float((wanted + Hk - 1) / Hk) : 0.f;
   // (the sum of what every tile is over a whole number of parts; one more workgroup, so that there is always one
   // without a unit, which clears rows behind the last sequence)

@@ -193,3 +193,24 @@ def test_heads_that_lie_far_apart(gpu_device):
     again = torch.autograd.grad(oat.omni_attention_packed(*near, cu), near, far.detach())
     for a, b, c in zip(want, got, again):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("B,most,Hq,Hk,D", [(70, 300, 4, 2, 64), (4500, 6, 2, 1, 32)])
+def test_thousands_of_sequences(gpu_device, B, most, Hq, Hk, D):
+    gen = torch.Generator().manual_seed(B)
+    dtype = torch.float16
+    lens = torch.randint(0, most, (B,), generator=gen).tolist()
+    lens[0], lens[-1] = 0, 2
+    T = sum(lens) + 40
+    q, k, v, do = _inputs(gen, gpu_device, dtype, T, Hq, Hk, D)
+    cu = torch.tensor(offsets(lens), dtype=torch.int32, device=gpu_device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(oat.omni_attention_packed(*leaves, cu), leaves, do)
+    at = offsets(lens)
+    for a, b in list(zip(at, at[1:]))[::9] + [(at[-2], at[-1])]:
+        if a == b:
+            continue
+        want, bound = _reference(*(t.detach()[a:b] for t in (q, k, v, do)), True, 0.0, dtype)
+        for g, w, e in zip(got, want, bound):
+            assert bool(((g[a:b].double() - w).abs() <= e).all()), (a, b)
+    assert all(bool((g[at[-1]:] == 0).all()) and not bool(torch.isnan(g).any()) for g in got)

@@ -334,3 +334,51 @@ def test_refusals_on_the_gpu(gpu_device):
         oat.omni_cache_append(rows, rows, *inside, table, kv_lens, cu)
     with torch.no_grad():
         paged(q=q.detach().requires_grad_())
+
+
+@pytest.mark.parametrize("B,kv,page,Hq,Hk,D", [(65, 1500, 64, 4, 1, 128), (513, 900, 64, 4, 1, 128), (1100, 700, 128, 8, 2, 64), (4500, 520, 16, 2, 1, 32)])
+def test_paged_thousands_of_sequences(gpu_device, B, kv, page, Hq, Hk, D):
+    """More sequences than the waves count by themselves: parts, tokens that a sequence has none or several of."""
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 4, (B,), generator=gen).tolist()
+    keys = torch.randint(0, kv, (B,), generator=gen).tolist()
+    keys[B // 2] = 8 * kv  # one that is cut into many parts
+    lens[B // 2], lens[-1] = 20, 1
+    dtype = torch.bfloat16
+    q, (kp, vp), table, kv_lens, cu, rows = _paged(gen, gpu_device, dtype, lens, keys, Hq, Hk, D, page, behind=70)
+    o, lse = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu, return_lse=True)
+    at = offsets(lens)
+    looked_at = [b for b in range(B) if b % 5 == 0 or b in (B // 2, B - 1)]
+    _compare(o, lse, q, [(at[b], lens[b], *rows[b]) for b in looked_at], True, 0.0, dtype, str(B))
+    assert not bool(torch.isnan(o).any()) and not bool(torch.isnan(lse).any())  # (no row is left out)
+    assert torch.equal(oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu), o)
+
+
+@pytest.mark.parametrize("B,most,Hq,Hk,D", [(70, 300, 8, 2, 64), (513, 40, 4, 4, 128), (4500, 9, 6, 2, 32)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_thousands_of_sequences(gpu_device, B, most, Hq, Hk, D, causal):
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, most, (B,), generator=gen).tolist()
+    lens[0], lens[-1] = 0, 2
+    dtype = torch.float16
+    q, k, v, cu = _packed(gen, gpu_device, dtype, lens, Hq, Hk, D, behind=100)
+    o, lse = oat.omni_attention_packed(q, k, v, cu, causal=causal, return_lse=True)
+    at = offsets(lens)
+    spans = list(zip(at, at[1:]))
+    _compare(o, lse, q, [(a, b - a, k[a:b], v[a:b]) for a, b in spans[::7] + spans[-1:]], causal, 0.0, dtype, str(B))
+    assert not bool(torch.isnan(o).any()) and not bool(torch.isnan(lse).any())
+    assert torch.equal(oat.omni_attention_packed(q, k, v, cu, causal=causal), o)
+
+
+def test_paged_chunks_of_many_sequences(gpu_device):
+    """Tiles of 128 rows in parts, more sequences than a wave has lanes."""
+    gen = torch.Generator().manual_seed(9)
+    B, Hq, Hk, D, dtype = 70, 4, 1, 64, torch.float16
+    lens = [40 + 3 * b % 50 for b in range(B)]
+    keys = [n + 100 + 211 * b % 3500 for b, n in enumerate(lens)]
+    q, (kp, vp), table, kv_lens, cu, rows = _paged(gen, gpu_device, dtype, lens, keys, Hq, Hk, D, 64)
+    at = offsets(lens)
+    for causal in (True, False):
+        o, lse = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu, causal=causal, return_lse=True)
+        _compare(o, lse, q, [(at[b], lens[b], *rows[b]) for b in range(0, B, 3)] + [(at[-2], lens[-1], *rows[-1])], causal, 0.0, dtype, "chunks")
+        assert not bool(torch.isnan(o).any()) and not bool(torch.isnan(lse).any())
