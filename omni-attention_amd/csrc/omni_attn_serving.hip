@@ -107,6 +107,7 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
   p.share = plan.share;
   p.least_steps = plan.least_steps;
   p.units = int(plan.units);
+  p.places = plan.places;
   if (plan.share != 0.f) {
     if (!workspace || workspace_bytes < plan.workspace_bytes(p.T, p.Hk, D)) return OMNI_ATTN_ERR_WORKSPACE;
     if (misaligned(workspace, 16)) return OMNI_ATTN_ERR_MISALIGNED;

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256, 2) serve_dq_kernel(const ServeBwdParams b
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
-  const Unit u = find_unit<M>(p, rank, lane);
+  const Unit u = find_tile<M>(p, rank, lane);
   if (!u.found) {
     clear_rows<D>(p, head, rank, u.step0, p.units, tid, 256);  // (p.o is dQ here)
     return;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(256 * KG, 2) serve_dkdv_kernel(const ServeBwdP
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
-  const Unit u = find_unit<M>(p, rank, lane);
+  const Unit u = find_tile<M>(p, rank, lane);
   if (!u.found) {  // keys of tokens behind the last sequence have no gradient
     if (rank < u.step0) return;
     int used = p.cu[p.B];

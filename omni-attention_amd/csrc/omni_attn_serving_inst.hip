@@ -41,21 +41,22 @@ int launch_serve<OMNI_INST_BF16 != 0, OMNI_INST_D>(const ServeParams& p, int row
   constexpr bool BF = OMNI_INST_BF16 != 0;
   constexpr int D = OMNI_INST_D;
   constexpr size_t few = kFewLdsBytes<D>;
-  const bool paged = p.page_table != nullptr;
+  const Keys keys = p.page_table == nullptr ? kPacked : ((1 << p.page_shift) >= kPageOfStep ? kPages : kSmallPages);
+#define OMNI_SERVE(kernel, n, threads, lds)                                                        \
+  (keys == kPacked  ? launch<kernel<BF, D, kPacked, n>>(p, blocks, threads, lds, stream)           \
+   : keys == kPages ? launch<kernel<BF, D, kPages, n>>(p, blocks, threads, lds, stream)            \
+                    : launch<kernel<BF, D, kSmallPages, n>>(p, blocks, threads, lds, stream))
   int e;
   if (rows == 128) {
-    e = paged ? launch<serve_tile_kernel<BF, D, true, 128>>(p, blocks, 256, kTileLdsBytes<D, 128>, stream)
-              : launch<serve_tile_kernel<BF, D, false, 128>>(p, blocks, 256, kTileLdsBytes<D, 128>, stream);
+    e = OMNI_SERVE(serve_tile_kernel, 128, 256, (kTileLdsBytes<D, 128>));
   } else if (rows == 64) {
-    e = paged ? launch<serve_tile_kernel<BF, D, true, 64>>(p, blocks, 256, 2 * kTileLdsBytes<D, 64>, stream)
-              : launch<serve_tile_kernel<BF, D, false, 64>>(p, blocks, 256, 2 * kTileLdsBytes<D, 64>, stream);
+    e = OMNI_SERVE(serve_tile_kernel, 64, 256, (2 * kTileLdsBytes<D, 64>));
   } else if (waves == 1) {
-    e = paged ? launch<serve_few_kernel<BF, D, true, 1>>(p, blocks, 64, few, stream)
-              : launch<serve_few_kernel<BF, D, false, 1>>(p, blocks, 64, few, stream);
+    e = OMNI_SERVE(serve_few_kernel, 1, 64, few);
   } else {
-    e = paged ? launch<serve_few_kernel<BF, D, true, 4>>(p, blocks, 256, 4 * few, stream)
-              : launch<serve_few_kernel<BF, D, false, 4>>(p, blocks, 256, 4 * few, stream);
+    e = OMNI_SERVE(serve_few_kernel, 4, 256, 4 * few);
   }
+#undef OMNI_SERVE
   if (e != 0 || p.share == 0.f) return e;
   const int64_t joined = int64_t(p.T) * ((p.Hk * p.G + kJoinRows<D> - 1) / kJoinRows<D>);
   const unsigned join_blocks = unsigned((joined + 3) / 4);

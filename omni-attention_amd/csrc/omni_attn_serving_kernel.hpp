@@ -19,6 +19,11 @@
 
 namespace omni_attn {
 
+// Where keys and values lie: packed, in pages of which a step of the walk reads one, or in smaller ones.  (A page looked up
+// once a step, and not once a load: 8192 tokens, 32 / 8 heads, D=128, 490 us for 532, as fast as packed ones.)
+enum Keys { kPacked, kPages, kSmallPages };
+constexpr int kPageOfStep = 64;  // keys
+
 struct ServeParams {
   const uint16_t* q;  // [T, Hk * G, D] at q_row, q_head
   const uint16_t* k;  // packed [T, Hk, D] at their strides, or pages [num_pages, Hk, page, D]
@@ -38,6 +43,7 @@ struct ServeParams {
   int causal;
   float share;         // units per key head that the batch's steps are shared over; 0: whole tiles
   int least_steps;     // ... and the steps that a part may have in any case
+  int places;          // (tiles of 128 rows) units per key head that run at once
   int units;           // units per key head that there is a place for
   int32_t* ends;       // [B + 1] of batches that a kernel of its own counts: units up to and with each sequence; steps of a part
   float* sums;         // [units, Hk, M, D] unscaled O of parts
@@ -77,7 +83,7 @@ __device__ __forceinline__ int dpp_max(int x) {
   const int y = __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
   return x > y ? x : y;
 }
-__device__ __forceinline__ int wave_max(int x) {  // x >= 0
+__device__ __forceinline__ int wave_max(int x) {
   x = dpp_max<0x118, 0xf>(dpp_max<0x114, 0xf>(dpp_max<0x112, 0xf>(dpp_max<0x111, 0xf>(x))));
   return __builtin_amdgcn_readlane(dpp_max<0x143, 0xc>(dpp_max<0x142, 0xa>(x)), 63);
 }
@@ -144,6 +150,33 @@ __device__ __forceinline__ int part_steps(const ServeParams& p, float all) {
 }
 
 constexpr int kAll = 0x7fffffff;
+// The same for tiles of 128 rows of a few sequences, which take long enough for their last round to count: the longest
+// sequence is cut into 1, 2, ... (a multiple per lane), the others into parts that are no longer, and what ends first
+// is taken: rounds of the units that run at once, each as long as a part and its start and end (about four steps).  Parts
+// lie alike in all tiles of a sequence, so that these read the same keys at a time.  (100 new tokens after 20000 keys, 32 / 8
+// heads, D=128: 60 us, 71 with the batch's steps over 1.5 times the units that run at once, 68 with even runs of steps that go
+// on from tile to tile; 512 and 300 after 15000 and 7000: 202, 207, 209; 812 after 22000: 325, 347, 316.  Packed prompts,
+// where causal tiles have fewer steps than are counted here: 8192 tokens, 2 heads, 72 us and 63 with the shares.)
+constexpr int kWeighed = 16;  // sequences
+template <int M>
+__device__ __forceinline__ int weighed_steps(const ServeParams& p, int tiles, int steps, int lane, int fallback) {
+  constexpr int kEnds = 4;
+  const int longest = wave_max(tiles > 0 ? steps : 0), all_tiles = wave_sum(tiles);
+  if (longest <= p.least_steps) return fallback;
+  const int stride = 1 + int(uint32_t(3 * p.places) / uint32_t(64 * (all_tiles < 1 ? 1 : all_tiles)));
+  const int cut = (lane + 1) * stride;
+  int most = int(uint32_t(longest + cut - 1) / uint32_t(cut));
+  if (most < p.least_steps) most = p.least_steps;
+  int units = 0;
+  for (int b = 0; b < p.B; ++b) units += __builtin_amdgcn_readlane(tiles, b) * parts_of(__builtin_amdgcn_readlane(steps, b) * kStepKeys, most).n;
+  const int rounds = int(uint32_t(units + p.places - 1) / uint32_t(p.places));
+  // (the smallest time, and of the same the longest parts)
+  const int time = units < p.units ? rounds * (most + kEnds) : 0x7fffffff;
+  const int best = -wave_max(-time);
+  if (best == 0x7fffffff) return fallback;
+  return __builtin_amdgcn_readlane(most, __builtin_ctzll(__builtin_amdgcn_ballot_w64(time == best)));
+}
+
 struct Unit {
   Sequence seq;
   int b, tile;
@@ -157,7 +190,7 @@ struct Unit {
 // sequences, one per lane, are counted by every wave (the same numbers in each: the same sums in the same order); more, by
 // a kernel that goes before (512 single tokens after 500 - 1000 keys, 8 / 1 heads, D=128: 48 us, 54 with every wave counting
 // eight per lane; 4096 of them, 32 / 8 heads, 2.1 ms and 5.7).
-template <int M>
+template <int M, bool WEIGH>
 __device__ __forceinline__ Unit find_part(const ServeParams& p, int rank, int lane) {
   Sequence s;
   int b, most, in;
@@ -171,6 +204,7 @@ __device__ __forceinline__ Unit find_part(const ServeParams& p, int rank, int la
     const Sequence own = sequence_of(p, lane);
     const int tiles = tiles_of<M>(p, own);
     most = part_steps(p, wave_sum(float(tiles) * float(steps_of(own.kv))));
+    if (WEIGH && p.B <= kWeighed) most = weighed_steps<M>(p, tiles, steps_of(own.kv), lane, most);
     const int mine = tiles * parts_of(own.kv, most).n, end = wave_scan(mine);
     const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
     if (beyond == 0) return Unit{{}, 0, 0, 0, 0, 0, 0, false, false};
@@ -236,9 +270,9 @@ __device__ __forceinline__ Unit find_tile(const ServeParams& p, int rank, int la
   const int tile = __builtin_amdgcn_readlane(tiles - from + mine, at) - 1 - in;
   return Unit{pick(s, at), at, tile, 0, kAll, 0, 1, false, true};
 }
-template <int M>
+template <int M, bool WEIGH>
 __device__ __forceinline__ Unit find_unit(const ServeParams& p, int rank, int lane) {
-  return p.share > 0.f ? find_part<M>(p, rank, lane) : find_tile<M>(p, rank, lane);
+  return p.share > 0.f ? find_part<M, WEIGH>(p, rank, lane) : find_tile<M>(p, rank, lane);
 }
 
 // Workgroup -> (key head, rank).  Ids go round-robin over the XCDs: the heads are dealt to the XCDs, so that the
@@ -565,6 +599,16 @@ __device__ __forceinline__ void merge_groups(const ServeParams& p, const Unit& u
   if (kg == 0 && odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, slot, row0, odd, from, to, lane);
 }
 
+// Rows from `row` on of the page that a step reads, up to `to`.
+template <int D>
+__device__ __forceinline__ i32x4_t page_rows(const ServeParams& p, const uint16_t* pages, const PageWindow& win, int head, int row, int to) {
+  const int page = __builtin_amdgcn_readlane(win.pages, (row >> p.page_shift) & 63);
+  const int64_t at = (((int64_t(page) * p.Hk + head) << p.page_shift) + (row & ((1 << p.page_shift) - 1))) * D;
+  int left = to - row;
+  left = left < 0 ? 0 : (left > kPageOfStep ? kPageOfStep : left);
+  return make_buffer_resource(pages + at, uint32_t(left) * (D * 2u));
+}
+
 // ---- few rows ---------------------------------------------------------------------------------------------------
 //
 // Single tokens, a few, and short prompts: tiles of 32 rows.  The work is the reading of K and V: a wave has a K and a V
@@ -577,8 +621,9 @@ constexpr int kFewStep = D == 128 ? 32 : 64;  // keys per step: 16 KiB of K and 
 template <int D>
 constexpr size_t kFewLdsBytes = kMergeBytes<D> > size_t(2) * kFewStep<D> * D * 2 ? kMergeBytes<D> : size_t(2) * kFewStep<D> * D * 2;  // of a wave
 
-template <bool BF16, int D, bool PAGED, int KG>
+template <bool BF16, int D, Keys KEYS, int KG>
 __global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p) {
+  constexpr bool PAGED = KEYS != kPacked;
   constexpr int M = 32, STEP = kFewStep<D>, NTL = STEP / 32, KS = D / 16, DT = D / 32, CPR = D / 8;
   constexpr int RPC = 64 / CPR, NCH = STEP / RPC, TILE = STEP * D;  // rows per load, loads per tile
   constexpr int KPER = RPC % 16 == 0 ? 1 : 16 / RPC;
@@ -590,7 +635,7 @@ __global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p)
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
-  const Unit u = find_unit<M>(p, rank, lane);
+  const Unit u = find_unit<M, false>(p, rank, lane);
   if (!u.found) {  // (with parts the joining kernel clears rows behind the last sequence)
     if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, threadIdx.x, 64 * KG);
     return;
@@ -639,11 +684,12 @@ __global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p)
   };
   auto issue = [&](bool is_v, int key0) {
     i32x4_t r;
-    if constexpr (!PAGED) r = is_v ? vr.rows<D>(key0) : kr.rows<D>(key0);
+    if constexpr (KEYS == kPacked) r = is_v ? vr.rows<D>(key0) : kr.rows<D>(key0);
+    if constexpr (KEYS == kPages) r = page_rows<D>(p, is_v ? p.v : p.k, window, head, key0, to);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const uint32_t dst = (is_v ? lds_v : lds_k) + uint32_t(i) * 1024u, off = is_v ? voff : koff[i % KPER];
-      if constexpr (PAGED) {
+      if constexpr (KEYS == kSmallPages) {
         const int key = key0 + i * RPC;
         const int page = __builtin_amdgcn_readlane(window.pages, (key >> p.page_shift) & 63);
         const int64_t at = (((int64_t(page) * p.Hk + head) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * D;
@@ -759,8 +805,9 @@ template <int D, int M>
 constexpr size_t kTileLdsBytes = M == 64 && 2 * kMergeBytes<D> > size_t(8) * kTileStep<D, M> * D ? 2 * kMergeBytes<D>
                                                                                              : size_t(8) * kTileStep<D, M> * D;
 
-template <bool BF16, int D, bool PAGED, int M>
+template <bool BF16, int D, Keys KEYS, int M>
 __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p) {
+  constexpr bool PAGED = KEYS != kPacked;
   constexpr int KG = 128 / M, W = M / 32, STEP = kTileStep<D, M>, NTL = STEP / 32, KS = D / 16, DT = D / 32, CPR = D / 8;
   constexpr int TILE = STEP * D;
   constexpr int RPC = 64 / CPR;            // rows filled by a wave's load
@@ -777,7 +824,7 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
-  const Unit u = find_unit<M>(p, rank, lane);
+  const Unit u = find_unit<M, M == 128 && PAGED>(p, rank, lane);
   if (!u.found) {
     if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, threadIdx.x, 256);
     return;
@@ -808,7 +855,7 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(at + 16 * s + 8 * g);
   }
 
-  const int ld_row = PAGED ? lane / CPR : tid / CPR, ld_pch = tid % CPR, sw_row = tid / CPR;
+  const int ld_row = KEYS == kSmallPages ? lane / CPR : tid / CPR, ld_pch = tid % CPR, sw_row = tid / CPR;
   PackedRows kr, vr;
   PageWindow kwin{0, -1}, vwin{0, -1};
   uint32_t kpitch = D * 2, vpitch = D * 2;
@@ -837,13 +884,13 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
       }
     }
   };
-  // Load n of a tile pair: n < NCH part n of V, else of K.  rk, rv: (packed) the rows from the step's first on.
+  // Load n of a tile pair: n < NCH part n of V, else of K.  rk, rv: (but for small pages) the rows from the step's first on.
   auto issue_load = [&](int n, int buf, int k_key0, int v_key0, const i32x4_t& rk, const i32x4_t& rv) {
     const bool is_v = n < NCH;
     const int i = is_v ? n : n - NCH;
     const uint32_t dst = (is_v ? lds_v0 : lds_k0) + uint32_t(buf) * (TILE * 2u) + uint32_t(i) * (W * 1024u);
     const uint32_t off = is_v ? voff : koff[i % KPER];
-    if constexpr (PAGED) {
+    if constexpr (KEYS == kSmallPages) {
       const int key = (is_v ? v_key0 : k_key0) + i * ROW_STRIDE + w * RPC;
       const int page = __builtin_amdgcn_readlane(is_v ? vwin.pages : kwin.pages, (key >> p.page_shift) & 63);
       const int64_t at = (((int64_t(page) * p.Hk + head) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * D;
@@ -854,11 +901,13 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
       buffer_to_lds_b128(is_v ? rv : rk, off, uint32_t(i * ROW_STRIDE) * (is_v ? vpitch : kpitch), dst);
     }
   };
-  auto rows_of = [&](const PackedRows& r, int key0) {
-    if constexpr (PAGED) {
-      return i32x4_t{};
+  auto rows_of = [&](bool is_v, int key0) {
+    if constexpr (KEYS == kPacked) {
+      return (is_v ? vr : kr).template rows<D>(key0);
+    } else if constexpr (KEYS == kPages) {
+      return page_rows<D>(p, is_v ? p.v : p.k, is_v ? vwin : kwin, head, key0, to);
     } else {
-      return r.template rows<D>(key0);
+      return i32x4_t{};
     }
   };
 
@@ -956,7 +1005,7 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
     constexpr int NPR = 8 * NTL;
     const uint16_t* tK = sK + (SET ^ 1) * TILE;
     const uint16_t* tV = sV + (SET ^ 1) * TILE;
-    const i32x4_t rk = rows_of(kr, k_key0), rv = rows_of(vr, v_key0);
+    const i32x4_t rk = rows_of(false, k_key0), rv = rows_of(true, v_key0);
     float rs0, rs1;
     __builtin_amdgcn_s_setprio(1);
     static_for<NS>([&](auto jc) {
@@ -1025,13 +1074,13 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
   if (nsteps > 0) {
     need_window(kwin, kwin, from_kg);
     {
-      const i32x4_t r0 = rows_of(kr, from_kg);
+      const i32x4_t r0 = rows_of(false, from_kg);
 #pragma unroll
       for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 0, from_kg, 0, r0, r0);
     }
     need_window(kwin, kwin, from_kg + NEXT);
     {
-      const i32x4_t r1 = rows_of(kr, from_kg + NEXT);
+      const i32x4_t r1 = rows_of(false, from_kg + NEXT);
 #pragma unroll
       for (int i = 0; i < NCH; ++i) issue_load(NCH + i, 1, from_kg + NEXT, 0, r1, r1);
     }

@@ -12,6 +12,7 @@ struct ServePlan {
   int waves;       // of a workgroup: 4, or 1 (tiles of 32 rows)
   float share;     // units per key head that the steps are shared over, 0: whole tiles
   int least_steps; // steps that a part may have in any case
+  int places;      // units per key head that run at once (tiles of 128 rows, two to a compute unit)
   int64_t units;   // units per key head that there is a place for
   int64_t counted; // sequences whose units a kernel of its own counts, or 0
   // the parts' rows and statistics, four words per token, one per counted sequence and one more
@@ -48,9 +49,10 @@ inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, int64_t capacit
     // 26 and 22; 8192 tokens, 2 heads, 81 and 63 in parts).
   } else {
     // Parts where the tiles leave compute units without work: 4096 tokens, one head, 26 us, 61 whole; 8192, 2 heads, 64 and
-    // 117; 812 new tokens after 22000, 32 / 8 heads, 197 and 307 (2000 after 10000, beyond the line, 377 and 347).
+    // 117; 512 and 300 new tokens after 15000 and 7000, 32 / 8 heads, D=128, 188 and 307; 4096 after 10000, 8 heads, D=64, 132
+    // and 156 (1500 after 6000, 32 / 8 heads, beyond the line, 198 and 170).
     s.rows = 128;
-    if (tiles_of(128) * Hk <= (capacity != 0 ? 3 * cus / 2 : cus) && keys > 2560) wanted = 3 * cus;
+    if (tiles_of(128) * Hk <= (capacity != 0 ? 5 * cus / 4 : cus) && keys > 2560) wanted = 3 * cus;
     // Tiles of 64 rows and two groups of waves where there are fewer tiles of 128 than the card holds at a time, and their
     // walks are not short: 9 prompts of 35 - 1047 tokens, D=64, 16 heads, capped scores 20 us, 26 with 128 rows; 4 x 1157
     // tokens, 8 heads 23.6 and 27.5; 1024 tokens, D=128, 32 / 8 heads 19.3 and 22.1 (beyond the line: 2048 tokens 46.4 and
@@ -64,7 +66,9 @@ inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, int64_t capacit
   s.share = parts ? float((wanted + Hk - 1) / Hk) : 0.f;
   // (the sum of what every tile is over a whole number of parts; one more workgroup, so that there is always one
   // without a unit, which clears rows behind the last sequence)
+  s.places = 2 * cus >= Hk ? 2 * cus / Hk : 1;
   s.units = tiles + 1 + (parts ? int64_t(s.share) + 1 : 0);
+  if (parts && s.rows == 128) s.units += 3 * s.places / 2;  // (three rounds of them)
   return s;
 }
 

@@ -382,3 +382,34 @@ def test_paged_chunks_of_many_sequences(gpu_device):
         o, lse = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu, causal=causal, return_lse=True)
         _compare(o, lse, q, [(at[b], lens[b], *rows[b]) for b in range(0, B, 3)] + [(at[-2], lens[-1], *rows[-1])], causal, 0.0, dtype, "chunks")
         assert not bool(torch.isnan(o).any()) and not bool(torch.isnan(lse).any())
+
+
+@pytest.mark.parametrize("B,Hq,Hk,D,softcap", [(30, 4, 1, 128, 0.0), (85, 4, 1, 128, 0.0), (40, 8, 2, 64, 20.0), (64, 5, 1, 32, 0.0)])
+def test_parts_of_uneven_sequences(gpu_device, B, Hq, Hk, D, softcap):
+    """Tiles of 128 rows, one sequence cut into many parts and the others into few or none; heads of a token in two tiles;
+    sequences without tokens and without keys among them."""
+    gen = torch.Generator().manual_seed(B + D)
+    dtype = torch.bfloat16
+    lens = [0 if b % 7 == 3 else 60 + 5 * b % 70 for b in range(B)]
+    keys = [0 if b % 11 == 5 else lens[b] + 37 * b % 230 for b in range(B)]
+    keys[B // 2] = 3500
+    q, (kp, vp), table, kv_lens, cu, rows = _paged(gen, gpu_device, dtype, lens, keys, Hq, Hk, D, 64, behind=130)
+    at = offsets(lens)
+    for causal in (True, False):
+        o, lse = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu, causal=causal, softcap=softcap, return_lse=True)
+        _compare(o, lse, q, [(at[b], lens[b], *rows[b]) for b in range(B)], causal, softcap, dtype, "parts")
+        assert torch.equal(oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu, causal=causal, softcap=softcap), o)
+
+
+@pytest.mark.parametrize("lens,cached,Hq,Hk,D", [([100], [20000], 8, 1, 128), ([512, 300], [3000, 1401], 8, 2, 64),
+                                                 ([40, 300, 7, 0, 200], [6000, 0, 2500, 900, 64], 3, 1, 32), ([33] * 16, [1000 + 700 * b for b in range(16)], 8, 1, 64)])
+@pytest.mark.parametrize("page", [32, 64])
+def test_chunks_in_weighed_parts(gpu_device, lens, cached, Hq, Hk, D, page):
+    gen = torch.Generator().manual_seed(D + page)
+    dtype = torch.float16
+    keys = [n + m for n, m in zip(lens, cached)]
+    q, (kp, vp), table, kv_lens, cu, rows = _paged(gen, gpu_device, dtype, lens, keys, Hq, Hk, D, page, behind=3)
+    at = offsets(lens)
+    for causal in (True, False):
+        o, lse = oat.omni_attention_paged(q, kp, vp, table, kv_lens, cu, causal=causal, return_lse=True)
+        _compare(o, lse, q, [(at[b], lens[b], *rows[b]) for b in range(len(lens))], causal, 0.0, dtype, "weighed")
