@@ -621,31 +621,22 @@ constexpr int kFewStep = D == 128 ? 32 : 64;  // keys per step: 16 KiB of K and 
 template <int D>
 constexpr size_t kFewLdsBytes = kMergeBytes<D> > size_t(2) * kFewStep<D> * D * 2 ? kMergeBytes<D> : size_t(2) * kFewStep<D> * D * 2;  // of a wave
 
-template <bool BF16, int D, Keys KEYS, int KG>
-__global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p) {
+// The rows from row0 on of a unit, by one wave, or by KG of which this is number kg.  LDS: bytes of a wave from lds on.
+template <bool BF16, int D, Keys KEYS, int M, int KG, int STEP, size_t LDS>
+__device__ __forceinline__ void few_rows(const ServeParams& p, const Unit& u, int head, int rank, int row0, int kg, uint8_t* lds, int lane) {
   constexpr bool PAGED = KEYS != kPacked;
-  constexpr int M = 32, STEP = kFewStep<D>, NTL = STEP / 32, KS = D / 16, DT = D / 32, CPR = D / 8;
+  constexpr int NTL = STEP / 32, KS = D / 16, DT = D / 32, CPR = D / 8;
   constexpr int RPC = 64 / CPR, NCH = STEP / RPC, TILE = STEP * D;  // rows per load, loads per tile
   constexpr int KPER = RPC % 16 == 0 ? 1 : 16 / RPC;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
-  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint16_t* sK = reinterpret_cast<uint16_t*>(lds_raw + kg * kFewLdsBytes<D>);
+  static_assert(LDS >= size_t(2) * TILE * 2, "a tile of K and one of V");
+  uint16_t* sK = reinterpret_cast<uint16_t*>(lds + kg * LDS);
   uint16_t* sV = sK + TILE;
-  const int lane = threadIdx.x & 63, g = lane >> 5, c = lane & 31;
-  int head, rank;
-  deal_head(p, blockIdx.x, head, rank);
-  if (rank >= p.units) return;
-  const Unit u = find_unit<M, false>(p, rank, lane);
-  if (!u.found) {  // (with parts the joining kernel clears rows behind the last sequence)
-    if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, threadIdx.x, 64 * KG);
-    return;
-  }
-  const int rows_all = u.seq.n * p.G, row0 = u.tile * M;
-  tell_joins<M>(p, u, head, rows_all, threadIdx.x);
+  const int g = lane >> 5, c = lane & 31;
+  const int rows_all = u.seq.n * p.G;
   const int row = row0 + c < rows_all ? row0 + c : rows_all - 1;
   const int token = int(divide(uint32_t(row), p.group));
   const int limit = p.causal ? u.seq.kv - u.seq.n + token : u.seq.kv - 1;  // the row's last key
-  const int last_row = row0 + M < rows_all ? row0 + M - 1 : rows_all - 1;
+  const int last_row = row0 + 32 < rows_all ? row0 + 31 : rows_all - 1;
   const int last_key = p.causal ? u.seq.kv - u.seq.n + int(divide(uint32_t(last_row), p.group)) : u.seq.kv - 1;
   const int first_key = p.causal ? u.seq.kv - u.seq.n + int(divide(uint32_t(row0), p.group)) : u.seq.kv - 1;
   const int from = u.step0 * kStepKeys;
@@ -784,9 +775,26 @@ __global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p)
     store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, odd, sK, lane);
     if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
   } else {
-    merge_groups<BF16, D, M, KG, PAGED>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, several, lds_raw,
-                                        kFewLdsBytes<D>, 0, kg, from, to, lane);
+    merge_groups<BF16, D, M, KG, PAGED>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, several, lds,
+                                        LDS, 0, kg, from, to, lane);
   }
+}
+
+template <bool BF16, int D, Keys KEYS, int KG>
+__global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p) {
+  constexpr int M = 32;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int head, rank;
+  deal_head(p, blockIdx.x, head, rank);
+  if (rank >= p.units) return;
+  const Unit u = find_unit<M, false>(p, rank, lane);
+  if (!u.found) {  // (with parts the joining kernel clears rows behind the last sequence)
+    if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, threadIdx.x, 64 * KG);
+    return;
+  }
+  tell_joins<M>(p, u, head, u.seq.n * p.G, threadIdx.x);
+  few_rows<BF16, D, KEYS, M, KG, kFewStep<D>, kFewLdsBytes<D>>(p, u, head, rank, u.tile * M, kg, lds_raw, lane);
 }
 
 // ---- many rows: four waves per unit -------------------------------------------------------------------------------
@@ -804,6 +812,12 @@ constexpr int kTileStep = M == 64 && D == 128 ? 32 : 64;
 template <int D, int M>
 constexpr size_t kTileLdsBytes = M == 64 && 2 * kMergeBytes<D> > size_t(8) * kTileStep<D, M> * D ? 2 * kMergeBytes<D>
                                                                                              : size_t(8) * kTileStep<D, M> * D;
+
+// Sequences of so few keys gain nothing from a pipeline over their steps: each wave has its rows' walk to itself and waits for
+// nobody.  32 / 8 heads, D=128: 4096 prompts of 20 - 40 tokens 642 us, 729 in the pipeline; 300 of 40 - 80 tokens 95 and 102;
+// 1000 of 67 - 133 tokens 540 and 545; 1000 of 15 and one of 4000 223 and 246 (300 of 133 - 267, beyond the line, D=64, 16
+// heads 190 and 184).
+constexpr int kShortKeys = 128;
 
 template <bool BF16, int D, Keys KEYS, int M>
 __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p) {
@@ -828,6 +842,14 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
   if (!u.found) {
     if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, threadIdx.x, 256);
     return;
+  }
+  if constexpr (M == 128) {
+    if (p.share == 0.f && u.seq.kv <= kShortKeys) {
+      constexpr size_t kOwn = kTileLdsBytes<D, M> / 4;
+      const int row0 = u.tile * M + 32 * w;
+      if (row0 < u.seq.n * p.G) few_rows<BF16, D, KEYS, M, 1, 32, kOwn>(p, u, head, rank, row0, 0, lds_raw + w * kOwn, lane);
+      return;
+    }
   }
   const int shift = u.seq.kv - u.seq.n;  // a token's position, less its number
   const int rows_all = u.seq.n * p.G, row0 = u.tile * M + 32 * w;
