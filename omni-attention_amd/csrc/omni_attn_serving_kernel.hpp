@@ -43,7 +43,7 @@ struct ServeParams {
   int causal;
   float share;         // units per key head that the batch's steps are shared over; 0: whole tiles
   int least_steps;     // ... and the steps that a part may have in any case
-  int places;          // (tiles of 128 rows) units per key head that run at once
+  int places;          // units per key head that run at once, where tiles are shared
   int units;           // units per key head that there is a place for
   int32_t* ends;       // [B + 1] of batches that a kernel of its own counts: units up to and with each sequence; steps of a part
   float* sums;         // [units, Hk, M, D] unscaled O of parts
@@ -150,14 +150,17 @@ __device__ __forceinline__ int part_steps(const ServeParams& p, float all) {
 }
 
 constexpr int kAll = 0x7fffffff;
-// The same for tiles of 128 rows of a few sequences, which take long enough for their last round to count: the longest
+// The same for a few sequences with many steps over a cache, which take long enough for their last round to count: the longest
 // sequence is cut into 1, 2, ... (a multiple per lane), the others into parts that are no longer, and what ends first
 // is taken: rounds of the units that run at once, each as long as a part and its start and end (about four steps).  Parts
 // lie alike in all tiles of a sequence, so that these read the same keys at a time.  (100 new tokens after 20000 keys, 32 / 8
 // heads, D=128: 60 us, 71 with the batch's steps over 1.5 times the units that run at once, 68 with even runs of steps that go
 // on from tile to tile; 512 and 300 after 15000 and 7000: 202, 207, 209; 812 after 22000: 325, 347, 316.  Packed prompts,
-// where causal tiles have fewer steps than are counted here: 8192 tokens, 2 heads, 72 us and 63 with the shares.)
-constexpr int kWeighed = 16;  // sequences
+// where causal tiles have fewer steps than are counted here: 8192 tokens, 2 heads, 72 us and 63 with the shares.  Single
+// tokens: one after 60000 keys 63 us, 78 with the shares; 4 after 1000 - 8000 28 and 30.5; beyond the lines one after 4000
+// 15.6 and 14.9, 16 after 300 - 16000 50 and 48.5, 60 after 4000 125 and 103.)
+template <int M>
+constexpr int kWeighed = M == 128 ? 16 : 8;  // sequences
 template <int M>
 __device__ __forceinline__ int weighed_steps(const ServeParams& p, int tiles, int steps, int lane, int fallback) {
   constexpr int kEnds = 4;
@@ -203,8 +206,9 @@ __device__ __forceinline__ Unit find_part(const ServeParams& p, int rank, int la
   } else {
     const Sequence own = sequence_of(p, lane);
     const int tiles = tiles_of<M>(p, own);
-    most = part_steps(p, wave_sum(float(tiles) * float(steps_of(own.kv))));
-    if (WEIGH && p.B <= kWeighed) most = weighed_steps<M>(p, tiles, steps_of(own.kv), lane, most);
+    const float all = wave_sum(float(tiles) * float(steps_of(own.kv)));
+    most = part_steps(p, all);
+    if (WEIGH && p.B <= kWeighed<M> && all > 2.f * float(p.places)) most = weighed_steps<M>(p, tiles, steps_of(own.kv), lane, most);
     const int mine = tiles * parts_of(own.kv, most).n, end = wave_scan(mine);
     const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
     if (beyond == 0) return Unit{{}, 0, 0, 0, 0, 0, 0, false, false};
@@ -788,7 +792,7 @@ __global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p)
   int head, rank;
   deal_head(p, blockIdx.x, head, rank);
   if (rank >= p.units) return;
-  const Unit u = find_unit<M, false>(p, rank, lane);
+  const Unit u = find_unit<M, (KEYS != kPacked && KG == 4)>(p, rank, lane);
   if (!u.found) {  // (with parts the joining kernel clears rows behind the last sequence)
     if (p.share == 0.f) clear_rows<D>(p, head, rank, u.step0, p.units, threadIdx.x, 64 * KG);
     return;

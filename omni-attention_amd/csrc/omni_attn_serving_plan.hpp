@@ -12,7 +12,7 @@ struct ServePlan {
   int waves;       // of a workgroup: 4, or 1 (tiles of 32 rows)
   float share;     // units per key head that the steps are shared over, 0: whole tiles
   int least_steps; // steps that a part may have in any case
-  int places;      // units per key head that run at once (tiles of 128 rows, two to a compute unit)
+  int places;      // units per key head that run at once, where tiles are shared (two workgroups to a compute unit)
   int64_t units;   // units per key head that there is a place for
   int64_t counted; // sequences whose units a kernel of its own counts, or 0
   // the parts' rows and statistics, four words per token, one per counted sequence and one more
