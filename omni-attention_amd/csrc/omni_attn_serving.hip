@@ -271,8 +271,12 @@ extern "C" int omni_attn_packed_bwd_gfx950(const void* q, const void* k, const v
   // Two groups of waves share a tile of keys where query heads share key heads (a tile then has the rows of all of them,
   // and its walk is what a launch ends with: 12 prompts of 128 - 3020 tokens, 32 / 8 heads, D=128, gradients 815 us with
   // one group, 608 with two; 2 x 4096 tokens 1185 and 980), or where there are few tiles; else one (2 x 4096 tokens, 32 /
-  // 32 heads 990 us, 1034 with two; 4 x 2048, 16 / 16, D=64 182 and 201).
-  const int groups = G > 1 || key_units * Hk <= 2 * cus ? 2 : 1;
+  // 32 heads 990 us, 1034 with two; 4 x 2048, 16 / 16, D=64 182 and 201).  One, too, for many short sequences, which leave two
+  // groups little to share: 32 / 8 heads, 100 prompts of 400 tokens 894 us, 1092 with two; 300 of 100 455 and 531; 2000 of 30
+  // 927 and 1226 (16 of 1000, beyond the line, 607 and 617; a long prompt among short ones is what this loses by: 500 of 60 and
+  // one of 4000 tokens 1312 and 1138).
+  const bool many_short = tokens <= 512 * int64_t(sequences) && key_units * Hk > 8 * cus;
+  const int groups = (G > 1 && !many_short) || key_units * Hk <= 2 * cus ? 2 : 1;
   const unsigned nr = unsigned(row_blocks), nk = unsigned(key_blocks);
   int e;
   switch (D) {

@@ -890,7 +890,7 @@ def omni_attention_packed(query: Tensor, key: Tensor, value: Tensor, cu_seqlens:
     ``omni_cache_append``.  ``causal``: a token attends itself and those before it; else its whole sequence.  ``softcap``
     as in ``omni_attention``.  Returns [tokens, heads, head_dim], with ``return_lse`` also the fp32 logsumexp
     [tokens, heads].  Tokens behind the last sequence get zeros (-inf).  Differentiable in query, key and value (not
-    through the logsumexp)."""
+    through the logsumexp); the gradients take the operands to be finite."""
     return _load_extension().omni_attn_packed(query, key, value, cu_seqlens, bool(causal), float(softcap), bool(return_lse))
 
 

@@ -214,3 +214,22 @@ def test_thousands_of_sequences(gpu_device, B, most, Hq, Hk, D):
         for g, w, e in zip(got, want, bound):
             assert bool(((g[a:b].double() - w).abs() <= e).all()), (a, b)
     assert all(bool((g[at[-1]:] == 0).all()) and not bool(torch.isnan(g).any()) for g in got)
+
+
+@pytest.mark.parametrize("causal,softcap", [(True, 0.0), (False, 0.0), (True, 15.0)])
+def test_many_short_sequences_of_shared_heads(gpu_device, causal, softcap):
+    """One group of waves on a tile of keys that several query heads share, at head_dim 128."""
+    gen = torch.Generator().manual_seed(8)
+    dtype, B, Hq, Hk, D = torch.bfloat16, 600, 8, 4, 128
+    lens = [1 + 37 * b % 150 for b in range(B)]
+    T = sum(lens) + 3
+    q, k, v, do = _inputs(gen, gpu_device, dtype, T, Hq, Hk, D)
+    cu = torch.tensor(offsets(lens), dtype=torch.int32, device=gpu_device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(oat.omni_attention_packed(*leaves, cu, causal=causal, softcap=softcap), leaves, do)
+    at = offsets(lens)
+    for a, b in list(zip(at, at[1:]))[::17]:
+        want, bound = _reference(*(t.detach()[a:b] for t in (q, k, v, do)), causal, softcap, dtype)
+        for g, w, e in zip(got, want, bound):
+            assert bool(((g[a:b].double() - w).abs() <= e).all()), (a, b)
+    assert all(bool((g[at[-1]:] == 0).all()) and not bool(torch.isnan(g).any()) for g in got)
