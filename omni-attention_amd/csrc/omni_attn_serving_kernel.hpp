@@ -155,7 +155,8 @@ constexpr int kAll = 0x7fffffff;
 // is taken: rounds of the units that run at once, each as long as a part and its start and end (about four steps).  Parts
 // lie alike in all tiles of a sequence, so that these read the same keys at a time.  (100 new tokens after 20000 keys, 32 / 8
 // heads, D=128: 60 us, 71 with the batch's steps over 1.5 times the units that run at once, 68 with even runs of steps that go
-// on from tile to tile; 512 and 300 after 15000 and 7000: 202, 207, 209; 812 after 22000: 325, 347, 316.  Packed prompts,
+// on from tile to tile; 512 and 300 after 15000 and 7000: 202, 207, 209; 812 after 22000: 325, 347, 316; all three with a
+// page looked up for every load, which left 58, 186 and 308 of the first.  Packed prompts,
 // where causal tiles have fewer steps than are counted here: 8192 tokens, 2 heads, 72 us and 63 with the shares.  Single
 // tokens: one after 60000 keys 63 us, 78 with the shares; 4 after 1000 - 8000 28 and 30.5; beyond the lines one after 4000
 // 15.6 and 14.9, 16 after 300 - 16000 50 and 48.5, 60 after 4000 125 and 103.)
