@@ -13,7 +13,7 @@ Four kinds of work:
 
 A case is a dict of plain values:
   op           which of the four
-  lens         tokens of each sequence of the batch ("append": new tokens; "paged": new tokens), "7,120,33"
+  lens         tokens of each sequence of the batch ("append": new tokens; "paged": new tokens)
   cached       ("append", "paged") keys of each sequence that the cache holds before them
   Hq, Hk, D    query heads, key heads, head dimension
   dtype        "float16" or "bfloat16"
@@ -50,14 +50,9 @@ def _ops():
 
 def _case(op, lens, Hq, Hk, D, dtype, cached=(), rot=0, interleaved=False, norm=False, train=False, page=0,
           softcap=0.0, causal=True):
-    return {"op": op, "lens": ",".join(map(str, lens)), "cached": ",".join(map(str, cached)), "Hq": Hq, "Hk": Hk, "D": D,
+    return {"op": op, "lens": [int(n) for n in lens], "cached": [int(n) for n in cached], "Hq": Hq, "Hk": Hk, "D": D,
             "dtype": dtype, "rot": rot, "interleaved": interleaved, "norm": norm, "train": train, "page": page,
             "softcap": softcap, "causal": causal}
-
-
-def _lists(case):
-    """The case with its lengths as lists of numbers."""
-    return dict(case, **{n: [int(x) for x in case[n].split(",")] if case[n] else [] for n in ("lens", "cached")})
 
 
 def _spread(n, low, high, seed):
@@ -152,7 +147,6 @@ def _offsets(lens):
 
 
 def prepare(case, seed):
-    case = _lists(case)
     g = torch.Generator(device="cuda").manual_seed(seed)
     dt, Hq, Hk, D, op = _DT[case["dtype"]], case["Hq"], case["Hk"], case["D"], case["op"]
     lens, cached = case["lens"], case["cached"]
@@ -267,19 +261,19 @@ def _attend(q, k, v, first, case):
     m, Hk = k.shape[0], k.shape[1]
     G = Hq // Hk
     out = torch.empty_like(q)
-    rows = max(1, min(n, (1 << 28) // (Hq * m)))  # (scores of at most 2^28 entries at a time)
-    kh, vh = k.permute(1, 2, 0).contiguous(), v.transpose(0, 1).contiguous()
-    for r0 in range(0, n, rows):
-        qh = q[r0:r0 + rows].view(-1, Hk, G, D).permute(1, 0, 2, 3).reshape(Hk, -1, D)
-        x = torch.bmm(qh, kh).mul_(1.0 / math.sqrt(D))
-        if case["softcap"]:
-            x = x.div_(case["softcap"]).tanh_().mul_(case["softcap"])
-        if case["causal"]:
-            at = first + r0 + torch.arange(qh.shape[1], device=q.device) // G
-            x = x.masked_fill_(torch.arange(m, device=q.device) > at.unsqueeze(1), float("-inf"))
-        x = x.sub_(x.amax(-1, keepdim=True)).exp_()
-        o = torch.bmm(x, vh).div_(x.sum(-1, keepdim=True))
-        out[r0:r0 + rows] = o.view(Hk, -1, G, D).transpose(0, 1).reshape(-1, Hq, D)
+    rows = max(1, min(n, (1 << 27) // (G * m)))  # (scores of at most 2^27 entries at a time)
+    for h in range(Hk):
+        kh, vh = k[:, h].t().contiguous(), v[:, h].contiguous()
+        for r0 in range(0, n, rows):
+            qh = q[r0:r0 + rows, h * G:(h + 1) * G].reshape(-1, D)
+            x = (qh @ kh).mul_(1.0 / math.sqrt(D))
+            if case["softcap"]:
+                x = (x / case["softcap"]).tanh_().mul_(case["softcap"])
+            if case["causal"]:
+                at = first + r0 + torch.arange(qh.shape[0], device=q.device) // G
+                x = x.masked_fill_(torch.arange(m, device=q.device) > at.unsqueeze(1), float("-inf"))
+            x = (x - x.amax(1, keepdim=True)).exp_()
+            out[r0:r0 + rows, h * G:(h + 1) * G] = ((x @ vh) / x.sum(1, keepdim=True)).view(-1, G, D)
     return out
 
 
@@ -339,7 +333,6 @@ def _run_own(s, case):
 # ---- what a pass cannot do without ---------------------------------------------------------------
 
 def work(case):
-    case = _lists(case)
     Hq, Hk, D, rot, lens, cached = (case[n] for n in ("Hq", "Hk", "D", "rot", "lens", "cached"))
     T = sum(lens)
     if case["op"] == "rotary":
@@ -466,7 +459,7 @@ def _exact_attention(q, k, v, first, case):
 
 
 def exact(case, seed):
-    s, case = prepare(case, seed), _lists(case)
+    s = prepare(case, seed)
     with torch.no_grad():
         if case["op"] == "rotary":
             return _exact_rotary(s, case)
