@@ -16,6 +16,7 @@
 #pragma once
 
 #include "omni_attn_fwd_kernel.hpp"
+#include "omni_attn_serving_plan.hpp"
 
 namespace omni_attn {
 
@@ -219,6 +220,8 @@ __device__ __forceinline__ Unit find_part(const ServeParams& p, int rank, int la
   }
   const Parts parts = parts_of(s.kv, most);
   const int tile = int(uint32_t(in) / uint32_t(parts.n));
+  // (counts of overlapping sequences, from offsets that run backwards, may pass 32 bits)
+  if (in < 0 || tile >= tiles_of<M>(p, s)) return Unit{{}, 0, 0, 0, 0, 0, 0, false, false};
   return Unit{s, b, tile, (in - tile * parts.n) * parts.steps, parts.steps, rank - in, parts.n, parts.n > 1, true};
 }
 
@@ -239,7 +242,7 @@ __device__ __forceinline__ Unit find_tile(const ServeParams& p, int rank, int la
     const int b = count_up_to(p.B, rank, lane, start), first = __builtin_amdgcn_readfirstlane(start(b));
     if (b == p.B) return Unit{{}, 0, 0, first, 0, 0, 1, false, false};
     const Sequence s = pick(sequence_of(p, b), 0);
-    const int tile = tiles_of<M>(p, s) - 1 - (rank - first);
+    const int tile = whole_tile(rank, first, tiles_of<M>(p, s));
     return Unit{s, b, tile, tile < 0 ? kAll : 0, kAll, 0, 1, false, tile >= 0};
   }
   const Sequence s = sequence_of(p, lane);

@@ -72,6 +72,11 @@ inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, int64_t capacit
   return s;
 }
 
+// Tile number of unit `rank` of a sequence whose units start at number `first`: the last tile comes first.  -1: the unit is not
+// one of its tiles.  (Offsets that run backwards make a search over their sequences' first units end anywhere, before a
+// sequence's units too: an empty one has no tile then either.)
+constexpr int whole_tile(int rank, int first, int tiles) { return rank < first || rank - first >= tiles ? -1 : tiles - 1 - (rank - first); }
+
 // Workgroups, so that every key head has `units` of them (the dealing gives XCDs whole heads, or heads whole XCDs).
 inline int64_t serve_blocks(int64_t units, int Hk, int n_xcd) {
   if (Hk % n_xcd != 0 && n_xcd % Hk == 0) {
