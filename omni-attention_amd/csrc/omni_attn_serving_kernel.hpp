@@ -447,11 +447,6 @@ __device__ __forceinline__ void store_rows(const ServeParams& p, const Unit& u, 
   }
 }
 
-// Rows whose sums are no numbers, in a unit where rows attend different keys: a weight of zero times a value that is
-// infinite or no number, of a key that the row does not attend, may have made them so.  Such a row (and one that is no
-// number by right) is summed again, over its own keys alone: a lane per key for the scores, a lane per dimensions for
-// the sums.  Slow, and never entered otherwise.  Returns the row's O in the lanes' dimensions (two per lane at
-// head_dim 128), its reference and its sum.
 template <bool BF16, int D, bool PAGED>
 __device__ __forceinline__ const uint16_t* key_row(const ServeParams& p, const Unit& u, int head, int key, bool is_v) {
   if constexpr (PAGED) {
@@ -471,59 +466,145 @@ __device__ __forceinline__ float widen16(uint32_t x) {
     return float(__builtin_bit_cast(_Float16, uint16_t(x)));
   }
 }
+// A step's scores become weights, packed for the second product; the row's maximum is kept exactly, its sums follow.
+template <bool BF16, int NTL, int DT>
+__device__ __forceinline__ void weigh_step(const f32x16_t (&st)[NTL], float sl2, float& m_run, float& l_run, f32x16_t (&ot)[DT],
+                                           u32x4_t (&pb)[NTL][2]) {
+  const float m_new = fmaxf(m_run, max_of<NTL>(st, sl2));
+  if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
+    const float m_old = m_run == -INFINITY ? (m_new == -INFINITY ? 0.f : m_new) : m_run;
+    const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_old - m_new);
+    l_run *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ot[dt][r] *= alpha;
+    m_run = m_new;
+  }
+  const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+  static_for<8 * NTL>([&](auto ic) {
+    constexpr int i = decltype(ic)::value, t = i / 8, r = 2 * (i % 8);
+    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], sl2, -m_ref));
+    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r + 1], sl2, -m_ref));
+    l_run += p0 + p1;
+    pb[t][r >> 3][(r & 7) >> 1] = pack2<BF16>(p0, p1);
+  });
+}
+
+// Rows whose sums are no numbers, in a unit where rows attend different keys: a weight of zero times a value that is
+// infinite or no number, of a key that the row does not attend, may have made them so.  Such rows of a wave (and those that
+// are no numbers by right) are summed again.  Up to the key that the wave's first row attends last nothing is masked, and
+// matrix products do it, from memory without LDS; of the keys behind, as many as the wave has tokens at most, a row adds one at a
+// time those that it attends.  Packed prompts with a value that is no number in the first key, which spoils every row, or in
+// the last, which spoils one: 4096 tokens, 8 / 2 heads, D=128, 0.70 ms, 0.07 without one; 8192 tokens, 8 heads 2.1 and 0.17;
+// 512 tokens, 8 heads, D=64 0.07 and 0.01 (a row at a time over all of its keys, a lane per key: 21, 47 and 2.2 ms).
 template <bool BF16, int D, int M, bool PAGED>
-__device__ void sum_rows_again(const ServeParams& p, const Unit& u, int head, int slot, int row0, uint32_t rows, int from,
+__device__ __forceinline__ void sum_rows_again(const ServeParams& p, const Unit& u, int head, int slot, int row0, uint32_t rows, int from,
                                int to, int lane) {
-  const int shift = u.seq.kv - u.seq.n;
-  for (; rows != 0; rows &= rows - 1) {
-    const int row = row0 + __builtin_ctz(rows), token = int(divide(uint32_t(row), p.group));
-    const int end = shift + token + 1 < to ? shift + token + 1 : to;
-    const uint16_t* q = p.q + int64_t(u.seq.first + token) * p.q_row + int64_t(head * p.G + (row - token * p.G)) * p.q_head;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    const int d = D == 128 ? 2 * lane : (lane < D ? lane : D - 1);
-    for (int key0 = from; key0 < end; key0 += 64) {
-      float x = -INFINITY;
-      if (key0 + lane < end) {
-        const uint16_t* k = key_row<BF16, D, PAGED>(p, u, head, key0 + lane, false);
-        x = 0.f;
-        for (int i = 0; i < D; ++i) x = __builtin_fmaf(widen16<BF16>(q[i]), widen16<BF16>(k[i]), x);
-        if (p.softcap > 0.f)
-          x = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * p.cap_c2) + 1.f), -2.f * p.softcap, p.softcap);
-        x *= p.sl2;
+  typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+  constexpr int KS = D / 16, DT = D / 32, STEP = 32;
+  const int g = lane >> 5, c = lane & 31, shift = u.seq.kv - u.seq.n, rows_all = u.seq.n * p.G;
+  const int row = row0 + c < rows_all ? row0 + c : rows_all - 1, token = int(divide(uint32_t(row), p.group));
+  const int last_row = row0 + 32 < rows_all ? row0 + 31 : rows_all - 1;
+  const int limit = shift + token;  // the row's last key
+  const int first_key = __builtin_amdgcn_readfirstlane(shift + int(divide(uint32_t(row0), p.group)));
+  const int last_key = __builtin_amdgcn_readfirstlane(shift + int(divide(uint32_t(last_row), p.group)));
+  const int common = first_key + 1 < to ? first_key + 1 : to, end = last_key + 1 < to ? last_key + 1 : to;
+  u32x4_t qf[KS];
+  {
+    const uint16_t* at = p.q + int64_t(u.seq.first + token) * p.q_row + int64_t(head * p.G + (row - token * p.G)) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(at + 16 * s + 8 * g);
+  }
+  f32x16_t ot[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) ot[dt] = f32x16_t{};
+  float m_run = -INFINITY, l_run = 0.f;
+  for (int key0 = from; key0 < common; key0 += STEP) {
+    const int key = key0 + c < common ? key0 + c : common - 1;
+    const uint16_t* k = key_row<BF16, D, PAGED>(p, u, head, key, false);
+    const int64_t v = key_row<BF16, D, PAGED>(p, u, head, key, true) - p.v;
+    f32x16_t st[1];
+    st[0] = f32x16_t{};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) st[0] = mfma_32x32x16<BF16>(*reinterpret_cast<const u32x4_t*>(k + 16 * s + 8 * g), qf[s], st[0]);
+    if (p.softcap > 0.f) cap_scores<1>(st, p.softcap, p.cap_c2);
+    if (key0 + STEP > common) mask_scores<1>(st, common - 1 - key0, g);
+    u32x4_t pb[1][2];
+    weigh_step<BF16, 1>(st, p.sl2, m_run, l_run, ot, pb);
+#pragma unroll
+    for (int ts = 0; ts < 2; ++ts) {
+      // the keys 16 ts + 4 g + (0 .. 3) and 8 further on, a dimension per lane
+      int64_t at[8];
+      bool in[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int n = 16 * ts + 4 * g + (i & 3) + 8 * (i >> 2);
+        at[i] = __shfl(v, n) + c;
+        in[i] = key0 + n < common;
       }
-      float most = x;
-      for (int i = 1; i < 64; i <<= 1) most = fmaxf(most, __shfl_xor(most, i));
-      const float m_new = fmaxf(m, most), m_ref = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_ref);
-      const float w = __builtin_amdgcn_exp2f(x - m_ref);
-      l = l * alpha + wave_sum(w);
-      o0 *= alpha;
-      o1 *= alpha;
-      m = m_new;
-      for (int j = 0; j < 64 && key0 + j < end; ++j) {
-        const float wj = __shfl(w, j);
-        const uint16_t* v = key_row<BF16, D, PAGED>(p, u, head, key0 + j, true);
-        o0 = __builtin_fmaf(wj, widen16<BF16>(v[d]), o0);
-        if constexpr (D == 128) o1 = __builtin_fmaf(wj, widen16<BF16>(v[d + 1]), o1);
+      static_for<DT>([&](auto dc) {
+        constexpr int dt = decltype(dc)::value;
+        uint32_t x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = in[i] ? p.v[at[i] + 32 * dt] : 0u;
+        ot[dt] = mfma_32x32x16<BF16>(u32x4_t{x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16}, pb[0][ts], ot[dt]);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    }
+  }
+  for (int key = common < from ? from : common; key < end; ++key) {
+    const uint16_t* k = key_row<BF16, D, PAGED>(p, u, head, key, false);
+    const uint16_t* v = key_row<BF16, D, PAGED>(p, u, head, key, true);
+    float x = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const u32x4_t y = *reinterpret_cast<const u32x4_t*>(k + 16 * s + 8 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x = __builtin_fmaf(widen16<BF16>(qf[s][i] & 0xffffu), widen16<BF16>(y[i] & 0xffffu), x);
+        x = __builtin_fmaf(widen16<BF16>(qf[s][i] >> 16), widen16<BF16>(y[i] >> 16), x);
       }
     }
+    x = pair_sum(x);
+    if (p.softcap > 0.f)
+      x = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * p.cap_c2) + 1.f), -2.f * p.softcap, p.softcap);
+    x *= p.sl2;
+    if (key > limit) continue;
+    const float m_new = fmaxf(m_run, x), m_ref = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_ref), weight = __builtin_amdgcn_exp2f(x - m_ref);
+    l_run = __builtin_fmaf(l_run, alpha, g == 0 ? weight : 0.f);
+    m_run = m_new;
+    static_for<4 * DT>([&](auto ic) {
+      constexpr int dt = decltype(ic)::value / 4, r = 4 * (decltype(ic)::value % 4);
+      const u32x2_t y = *reinterpret_cast<const u32x2_t*>(v + 32 * dt + 2 * r + 4 * g);
+      const float f[4] = {widen16<BF16>(y[0] & 0xffffu), widen16<BF16>(y[0] >> 16), widen16<BF16>(y[1] & 0xffffu), widen16<BF16>(y[1] >> 16)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ot[dt][r + i] = __builtin_fmaf(weight, f[i], ot[dt][r + i] * alpha);
+    });
+  }
+  const float l = pair_sum(l_run);
+  if (!(rows >> c & 1)) return;
+  const bool live = l > 0.f || l != l;
+  const float inv = live ? 1.f / l : 0.f;
+  const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (row - token * p.G);
+  const int64_t part_at = (int64_t(slot) * p.Hk + head) * M + (row & (M - 1));
+  static_for<4 * DT>([&](auto ic) {
+    constexpr int dt = decltype(ic)::value / 4, r = 4 * (decltype(ic)::value % 4);
+    const int d = 32 * dt + 2 * r + 4 * g;
     if (u.part) {
-      const int64_t at = (int64_t(slot) * p.Hk + head) * M + (row & (M - 1));
-      if (lane < D) p.sums[at * D + d] = o0;
-      if constexpr (D == 128) p.sums[at * D + d + 1] = o1;
-      if (lane == 0) {
-        p.stats[at * 2] = m;
-        p.stats[at * 2 + 1] = l;
-      }
-      continue;
+      *reinterpret_cast<f32x4_t*>(p.sums + part_at * D + d) = f32x4_t{ot[dt][r], ot[dt][r + 1], ot[dt][r + 2], ot[dt][r + 3]};
+    } else {
+      const u32x2_t ov = {live ? pack2<BF16>(ot[dt][r] * inv, ot[dt][r + 1] * inv) : 0u, live ? pack2<BF16>(ot[dt][r + 2] * inv, ot[dt][r + 3] * inv) : 0u};
+      *reinterpret_cast<u32x2_t*>(p.o + at * D + d) = ov;
     }
-    const bool live = l > 0.f || l != l;
-    const float inv = live ? 1.f / l : 0.f;
-    const int64_t at = (int64_t(u.seq.first + token) * p.Hk + head) * p.G + (row - token * p.G);
-    const uint32_t packed = live ? pack2<BF16>(o0 * inv, o1 * inv) : 0u;
-    if (lane < D) p.o[at * D + d] = uint16_t(packed);
-    if constexpr (D == 128) p.o[at * D + d + 1] = uint16_t(packed >> 16);
-    if (p.lse != nullptr && lane == 0) p.lse[at] = live ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+  });
+  if (g != 0) return;
+  if (u.part) {
+    p.stats[part_at * 2] = m_run;
+    p.stats[part_at * 2 + 1] = l;
+  } else if (p.lse != nullptr) {
+    p.lse[at] = live ? (m_run + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
   }
 }
 // The rows of a wave whose O holds something that is no number (or infinite), bit by row.
@@ -737,26 +818,8 @@ __device__ __forceinline__ void few_rows(const ServeParams& p, const Unit& u, in
       const int stop = limit < to - 1 ? limit : to - 1;
       mask_scores<NTL>(st, stop - key0, g);
     }
-    const float m_new = fmaxf(m_run, max_of<NTL>(st, p.sl2));
-    if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
-      const float m_old = m_run == -INFINITY ? (m_new == -INFINITY ? 0.f : m_new) : m_run;
-      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_old - m_new);
-      l_run *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ot[dt][r] *= alpha;
-      m_run = m_new;
-    }
-    const float m_ref = m_run == -INFINITY ? 0.f : m_run;
     u32x4_t pb[NTL][2];
-    static_for<8 * NTL>([&](auto ic) {
-      constexpr int i = decltype(ic)::value, t = i / 8, r = 2 * (i % 8);
-      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], p.sl2, -m_ref));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r + 1], p.sl2, -m_ref));
-      l_run += p0 + p1;
-      pb[t][r >> 3][(r & 7) >> 1] = pack2<BF16>(p0, p1);
-    });
+    weigh_step<BF16, NTL>(st, p.sl2, m_run, l_run, ot, pb);
     if (more) {
       wait_loads_but<NCH>();  // the next K may be under way
     } else {
@@ -789,7 +852,7 @@ __device__ __forceinline__ void few_rows(const ServeParams& p, const Unit& u, in
 }
 
 template <bool BF16, int D, Keys KEYS, int KG>
-__global__ void __launch_bounds__(64 * KG) serve_few_kernel(const ServeParams p) {
+__global__ void __launch_bounds__(64 * KG, 2) serve_few_kernel(const ServeParams p) {
   constexpr int M = 32;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
   const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;

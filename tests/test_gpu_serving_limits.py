@@ -1,8 +1,9 @@
-"""Calls of the packed-sequence operators at their limits: offsets that run backwards."""
+"""Calls of the packed-sequence operators at their limits: offsets that run backwards, values that are no numbers."""
 import pytest
 import torch
 
 import omni_attn_torch as oat
+from serving_helpers import attention, attention_bound, offsets
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,86 @@ def test_backward_offsets_of_many_sequences(gpu_device, B, D):
         want = oat.omni_attention_packed(q[a:b].contiguous(), k[a:b].contiguous(), v[a:b].contiguous(), one).float()
         # two roundings of weights and results each, of values of at most 5
         assert (got - want).abs().max().item() <= 4 * 5 * torch.finfo(dtype).eps / 2
+
+
+def _paged_of(gen, k, v, lens, page):
+    """Packed keys and values in pages of a shuffled cache: key_pages, value_pages, page_table."""
+    need = [-(-n // page) for n in lens]
+    order = torch.randperm(sum(need) + 2, generator=gen)
+    pools = [torch.full((sum(need) + 2, k.shape[1], page, k.shape[2]), float("nan"), dtype=k.dtype, device=k.device) for _ in range(2)]
+    table, at, row = torch.zeros(len(lens), max(need), dtype=torch.int32), 0, 0
+    for b, n in enumerate(lens):
+        own = order[at:at + need[b]]
+        table[b, :need[b]] = own.to(torch.int32)
+        at += need[b]
+        for pool, x in zip(pools, (k, v)):
+            for i, pg in enumerate(own.tolist()):
+                part = x[row + i * page:row + min(n, (i + 1) * page)]
+                pool[pg, :, :part.shape[0]] = part.transpose(0, 1)
+        row += n
+    return pools[0], pools[1], table.to(k.device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Hq,Hk,D,lens,softcap", [
+    (4, 4, 64, [200], 0.0), (8, 2, 128, [130, 77], 0.0), (8, 1, 32, [300, 5], 20.0),  # few rows, four waves
+    (16, 16, 128, [1300], 0.0), (16, 16, 64, [700, 90], 15.0),                        # tiles of 64 rows
+    (32, 8, 128, [1500, 300], 0.0), (24, 24, 32, [1600], 0.0),                        # of 128, whole
+    (8, 8, 64, [70] * 40, 0.0)])                                                      # few rows, one wave
+@pytest.mark.parametrize("page", [0, 16, 64])
+def test_no_numbers_by_right_and_behind_a_row(gpu_device, dtype, Hq, Hk, D, lens, softcap, page):
+    """Infinities and NaN in V, some attended by a row and some behind it: every element that a row's own keys make a number is
+    that number, every other is none."""
+    gen = torch.Generator().manual_seed(D + Hq)
+    T = sum(lens)
+    q, k, v = (torch.randn(T, h, D, generator=gen).to(device=gpu_device, dtype=dtype) for h in (Hq, Hk, Hk))
+    at = offsets(lens)
+    for b, n in enumerate(lens):
+        v[at[b] + n // 3, :, 1::4] = float("inf")       # rows from a third on
+        v[at[b] + n // 2, 0, 2::8] = float("nan")       # from the middle on
+        v[at[b] + n - 1, :, 3::4] = float("-inf")       # the last alone
+    cu = torch.tensor(at, dtype=torch.int32, device=gpu_device)
+    if page:
+        kp, vp, table = _paged_of(gen, k, v, lens, page)
+        o, lse = oat.omni_attention_paged(q, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device=gpu_device), cu,
+                                          softcap=softcap, return_lse=True)
+    else:
+        o, lse = oat.omni_attention_packed(q, k, v, cu, softcap=softcap, return_lse=True)
+    for a, e in list(zip(at, at[1:]))[:6]:
+        clean = torch.where(torch.isfinite(v[a:e]), v[a:e], torch.zeros((), dtype=dtype, device=gpu_device))
+        want, mean, rl = attention(q[a:e], k[a:e], clean, 0, True, softcap)
+        seen = torch.cumsum((~torch.isfinite(v[a:e])).to(torch.int32), 0) > 0  # [row, Hk, D]: a key up to the row's own spoils it
+        seen = seen.repeat_interleave(Hq // Hk, dim=1)
+        assert torch.equal(~torch.isfinite(o[a:e]), seen)
+        smax = (q[a:e].double().norm(dim=-1).max() * k[a:e].double().norm(dim=-1).max()).item() / D ** 0.5
+        bound = attention_bound(want, mean, clean.double().abs().sum(0).max().item(), dtype, softcap, D, smax)
+        assert bool(((o[a:e].double() - want).abs() <= bound)[~seen].all())
+        assert bool(((lse[a:e].double() - rl).abs() <= (D + 8) * 2.0 ** -24 * smax + 8 * 2.0 ** -23 * softcap + 2.0 ** -21 * (1 + rl.abs())).all())
+
+
+@pytest.mark.parametrize("T,Hq,Hk,D", [(4096, 8, 2, 128), (4096, 8, 8, 64), (512, 8, 8, 64), (1300, 16, 16, 128)])
+@pytest.mark.parametrize("spoilt", ["first", "last"])
+def test_no_numbers_do_not_stop_a_launch(gpu_device, T, Hq, Hk, D, spoilt):
+    """One value that is no number, in the first key (all rows) or the last (one row): a second, slower walk over the tile's keys,
+    not one for every row."""
+    gen = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(T, h, D, generator=gen).to(device=gpu_device, dtype=torch.bfloat16) for h in (Hq, Hk, Hk))
+    bad = v.clone()
+    bad[0 if spoilt == "first" else T - 1] = float("nan")
+    cu = torch.tensor([0, T], dtype=torch.int32, device=gpu_device)
+
+    def fastest(values):
+        oat.omni_attention_packed(q, k, values, cu)
+        times = []
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            oat.omni_attention_packed(q, k, values, cu)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    clean, dirty = fastest(v), fastest(bad)
+    # (a row at a time takes 220 - 330 times as long as the launch without; launches and clocks vary by less than 2)
+    assert dirty <= 60 * clean, (clean, dirty)
