@@ -60,7 +60,7 @@ int check_pages(int num_pages, int page_size, int max_pages) {
 template <int M>
 __global__ void __launch_bounds__(1024) serve_count_kernel(const ServeParams p) {
   __shared__ float steps[16];
-  __shared__ int units[16];
+  __shared__ int units[16], cuts[16];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   float all = 0.f;
   for (int b = tid; b < p.B; b += 1024) {
@@ -73,18 +73,29 @@ __global__ void __launch_bounds__(1024) serve_count_kernel(const ServeParams p) 
   all = 0.f;
   for (int i = 0; i < 16; ++i) all += steps[i];
   const int most = part_steps(p, all);
-  int before = 0;
+  int before = 0, cut_before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 1024) {
     const Sequence s = sequence_of(p, b0 + tid);
-    const int end = wave_scan(tiles_of<M>(p, s) * parts_of(s.kv, most).n);
-    if (lane == 63) units[w] = end;
-    __syncthreads();
-    int here = before;
-    for (int i = 0; i < 16; ++i) {
-      if (i < w) here += units[i];
-      before += units[i];
+    const int parts = parts_of(s.kv, most).n, mine = tiles_of<M>(p, s) * parts;
+    const int end = wave_scan(mine), cut_end = wave_scan(parts > 1 ? mine : 0);
+    if (lane == 63) {
+      units[w] = end;
+      cuts[w] = cut_end;
     }
-    if (b0 + tid < p.B) p.ends[b0 + tid] = here + end;
+    __syncthreads();
+    int here = before, cut_here = cut_before;
+    for (int i = 0; i < 16; ++i) {
+      if (i < w) {
+        here += units[i];
+        cut_here += cuts[i];
+      }
+      before += units[i];
+      cut_before += cuts[i];
+    }
+    if (b0 + tid < p.B) {
+      p.ends[b0 + tid] = here + end;
+      p.ends[p.B + 1 + b0 + tid] = cut_here + cut_end;
+    }
     __syncthreads();
   }
   if (tid == 0) p.ends[p.B] = most;
@@ -108,12 +119,13 @@ int serve(ServeParams& p, int Hq, int D, void* workspace, size_t workspace_bytes
   p.least_steps = plan.least_steps;
   p.units = int(plan.units);
   p.places = plan.places;
+  p.slots = int(plan.slots);
   if (plan.share != 0.f) {
     if (!workspace || workspace_bytes < plan.workspace_bytes(p.T, p.Hk, D)) return OMNI_ATTN_ERR_WORKSPACE;
     if (misaligned(workspace, 16)) return OMNI_ATTN_ERR_MISALIGNED;
     p.sums = static_cast<float*>(workspace);
-    p.stats = p.sums + plan.units * p.Hk * plan.rows * D;
-    p.joins = reinterpret_cast<int32_t*>(p.stats + plan.units * p.Hk * plan.rows * 2);
+    p.stats = p.sums + plan.slots * p.Hk * plan.rows * D;
+    p.joins = reinterpret_cast<int32_t*>(p.stats + plan.slots * p.Hk * plan.rows * 2);
     p.ends = plan.counted != 0 ? p.joins + int64_t(p.T) * 4 : nullptr;
   }
   p.softcap = softcap;

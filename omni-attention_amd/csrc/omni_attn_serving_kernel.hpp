@@ -46,10 +46,12 @@ struct ServeParams {
   int least_steps;     // ... and the steps that a part may have in any case
   int places;          // units per key head that run at once, where tiles are shared
   int units;           // units per key head that there is a place for
-  int32_t* ends;       // [B + 1] of batches that a kernel of its own counts: units up to and with each sequence; steps of a part
-  float* sums;         // [units, Hk, M, D] unscaled O of parts
-  float* stats;        // [units, Hk, M, 2] their reference points (log2 domain) and sums of weights
-  int32_t* joins;      // [T, 4] of a token: first token and number of parts of its sequence, number of its first unit
+  int slots;           // parts per key head that there is a place for
+  int32_t* ends;       // [2 B + 1] of batches that a kernel of its own counts: units up to and with each sequence; steps of a
+                       // part; places of parts up to and with each sequence
+  float* sums;         // [slots, Hk, M, D] unscaled O of parts
+  float* stats;        // [slots, Hk, M, 2] their reference points (log2 domain) and sums of weights
+  int32_t* joins;      // [T, 4] of a token: first token and number of parts of its sequence, place of its first part
   float sl2, softcap, cap_c2;
 };
 
@@ -162,8 +164,6 @@ constexpr int kAll = 0x7fffffff;
 // tokens: one after 60000 keys 63 us, 78 with the shares; 4 after 1000 - 8000 28 and 30.5; beyond the lines one after 4000
 // 15.6 and 14.9, 16 after 300 - 16000 50 and 48.5, 60 after 4000 125 and 103.)
 template <int M>
-constexpr int kWeighed = M == 128 ? 16 : 8;  // sequences
-template <int M>
 __device__ __forceinline__ int weighed_steps(const ServeParams& p, int tiles, int steps, int lane, int fallback) {
   constexpr int kEnds = 4;
   const int longest = wave_max(tiles > 0 ? steps : 0), all_tiles = wave_sum(tiles);
@@ -186,7 +186,8 @@ struct Unit {
   Sequence seq;
   int b, tile;
   int step0, steps;  // range of steps (all that the tile has may be fewer)
-  int base, parts;   // (shared by parts) number of the sequence's first unit, parts of each of its tiles
+  int base, slot;    // (shared by parts) place of the sequence's first part, and of this one
+  int parts;         // parts of each of its tiles
   bool part;         // one of several: its sums are joined later
   bool found;        // no: (whole tiles) step0 is the number behind the last unit's (kAll: this number is left out)
 };
@@ -198,31 +199,35 @@ struct Unit {
 template <int M, bool WEIGH>
 __device__ __forceinline__ Unit find_part(const ServeParams& p, int rank, int lane) {
   Sequence s;
-  int b, most, in;
+  int b, most, in, base;
   if (p.ends != nullptr) {
     most = load_uniform(p.ends + p.B);
     b = count_up_to(p.B, rank, lane, [&](int i) { return p.ends[i - 1]; });
-    if (b == p.B) return Unit{{}, 0, 0, 0, 0, 0, 0, false, false};
+    if (b == p.B) return Unit{{}, 0, 0, 0, 0, 0, 0, 0, false, false};
     s = pick(sequence_of(p, b), 0);
     in = rank - (b == 0 ? 0 : load_uniform(p.ends + b - 1));
+    base = b == 0 ? 0 : load_uniform(p.ends + p.B + b);
   } else {
     const Sequence own = sequence_of(p, lane);
     const int tiles = tiles_of<M>(p, own);
     const float all = wave_sum(float(tiles) * float(steps_of(own.kv)));
     most = part_steps(p, all);
-    if (WEIGH && p.B <= kWeighed<M> && all > 2.f * float(p.places)) most = weighed_steps<M>(p, tiles, steps_of(own.kv), lane, most);
-    const int mine = tiles * parts_of(own.kv, most).n, end = wave_scan(mine);
+    if (WEIGH && weighed(p.B, M, all, p.places)) most = weighed_steps<M>(p, tiles, steps_of(own.kv), lane, most);
+    const int parts = parts_of(own.kv, most).n, mine = tiles * parts, end = wave_scan(mine);
+    const int cut = parts > 1 ? mine : 0, cut_end = wave_scan(cut);
     const uint64_t beyond = __builtin_amdgcn_ballot_w64(end > rank);
-    if (beyond == 0) return Unit{{}, 0, 0, 0, 0, 0, 0, false, false};
+    if (beyond == 0) return Unit{{}, 0, 0, 0, 0, 0, 0, 0, false, false};
     b = __builtin_ctzll(beyond);
     s = pick(own, b);
     in = rank - (__builtin_amdgcn_readlane(end, b) - __builtin_amdgcn_readlane(mine, b));
+    base = __builtin_amdgcn_readlane(cut_end, b) - __builtin_amdgcn_readlane(cut, b);
   }
   const Parts parts = parts_of(s.kv, most);
   const int tile = int(uint32_t(in) / uint32_t(parts.n));
   // (counts of overlapping sequences, from offsets that run backwards, may pass 32 bits)
-  if (in < 0 || tile >= tiles_of<M>(p, s)) return Unit{{}, 0, 0, 0, 0, 0, 0, false, false};
-  return Unit{s, b, tile, (in - tile * parts.n) * parts.steps, parts.steps, rank - in, parts.n, parts.n > 1, true};
+  if (in < 0 || tile >= tiles_of<M>(p, s) || (parts.n > 1 && (base < 0 || uint32_t(base) + uint32_t(in) >= uint32_t(p.slots))))
+    return Unit{{}, 0, 0, 0, 0, 0, 0, 0, false, false};
+  return Unit{s, b, tile, (in - tile * parts.n) * parts.steps, parts.steps, base, base + in, parts.n, parts.n > 1, true};
 }
 
 // Unit number `rank` of whole tiles.  Of up to 64 sequences those with most steps come first, so that a launch ends with
@@ -240,10 +245,10 @@ __device__ __forceinline__ Unit find_tile(const ServeParams& p, int rank, int la
       return int(uint32_t(from) * uint32_t(p.G) >> kLog) + b;
     };
     const int b = count_up_to(p.B, rank, lane, start), first = __builtin_amdgcn_readfirstlane(start(b));
-    if (b == p.B) return Unit{{}, 0, 0, first, 0, 0, 1, false, false};
+    if (b == p.B) return Unit{{}, 0, 0, first, 0, 0, 0, 1, false, false};
     const Sequence s = pick(sequence_of(p, b), 0);
     const int tile = whole_tile(rank, first, tiles_of<M>(p, s));
-    return Unit{s, b, tile, tile < 0 ? kAll : 0, kAll, 0, 1, false, tile >= 0};
+    return Unit{s, b, tile, tile < 0 ? kAll : 0, kAll, 0, 0, 1, false, tile >= 0};
   }
   const Sequence s = sequence_of(p, lane);
   const int most = wave_max(s.n > 0 ? steps_of(s.kv) : 0);
@@ -259,7 +264,7 @@ __device__ __forceinline__ Unit find_tile(const ServeParams& p, int rank, int la
     return token >= s.n ? 0 : (token <= 0 ? tiles : tiles - (row >> kLog));
   };
   const int all = wave_sum(tiles);
-  if (all <= rank) return Unit{{}, 0, 0, all, 0, 0, 1, false, false};
+  if (all <= rank) return Unit{{}, 0, 0, all, 0, 0, 0, 1, false, false};
   int level = 0, longer = 0;  // (tiles above the level)
   for (int bit = 8; bit != 0; bit >>= 1) {
     const int n = wave_sum(long_tiles((level | bit) << unit));
@@ -276,7 +281,7 @@ __device__ __forceinline__ Unit find_tile(const ServeParams& p, int rank, int la
   const int at = beyond != 0 ? __builtin_ctzll(beyond) : 0;
   const int in = rank - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(mine, at));
   const int tile = __builtin_amdgcn_readlane(tiles - from + mine, at) - 1 - in;
-  return Unit{pick(s, at), at, tile, 0, kAll, 0, 1, false, true};
+  return Unit{pick(s, at), at, tile, 0, kAll, 0, 0, 1, false, true};
 }
 template <int M, bool WEIGH>
 __device__ __forceinline__ Unit find_unit(const ServeParams& p, int rank, int lane) {
@@ -389,7 +394,7 @@ template <bool BF16, int D, int M>
 __device__ __forceinline__ void store_rows(const ServeParams& p, const Unit& u, int head, int slot, int row0, int rows_all,
                                            f32x16_t (&ot)[D / 32], float m_run, float l_run, uint32_t skip, uint16_t* stage,
                                            int lane) {
-  // row0: first row of the wave in the sequence; slot: number of the unit; skip: rows that are left out, by bit
+  // row0: first row of the wave in the sequence; slot: the part's place; skip: rows that are left out, by bit
   const int c = lane & 31, g = lane >> 5;
   const float l = pair_sum(l_run);
   if (u.part) {
@@ -712,7 +717,7 @@ constexpr size_t kFewLdsBytes = kMergeBytes<D> > size_t(2) * kFewStep<D> * D * 2
 
 // The rows from row0 on of a unit, by one wave, or by KG of which this is number kg.  LDS: bytes of a wave from lds on.
 template <bool BF16, int D, Keys KEYS, int M, int KG, int STEP, size_t LDS>
-__device__ __forceinline__ void few_rows(const ServeParams& p, const Unit& u, int head, int rank, int row0, int kg, uint8_t* lds, int lane) {
+__device__ __forceinline__ void few_rows(const ServeParams& p, const Unit& u, int head, int slot, int row0, int kg, uint8_t* lds, int lane) {
   constexpr bool PAGED = KEYS != kPacked;
   constexpr int NTL = STEP / 32, KS = D / 16, DT = D / 32, CPR = D / 8;
   constexpr int RPC = 64 / CPR, NCH = STEP / RPC, TILE = STEP * D;  // rows per load, loads per tile
@@ -843,10 +848,10 @@ __device__ __forceinline__ void few_rows(const ServeParams& p, const Unit& u, in
   const bool several = p.causal && first_key < last_key;  // rows that attend different keys
   if constexpr (KG == 1) {
     const uint32_t odd = several ? odd_rows<DT>(ot) & live_rows(rows_all - row0) : 0u;
-    store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, odd, sK, lane);
-    if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
+    store_rows<BF16, D, M>(p, u, head, slot, row0, rows_all, ot, m_run, l_run, odd, sK, lane);
+    if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, slot, row0, odd, from, to, lane);
   } else {
-    merge_groups<BF16, D, M, KG, PAGED>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, several, lds,
+    merge_groups<BF16, D, M, KG, PAGED>(p, u, head, slot, row0, rows_all, ot, m_run, l_run, several, lds,
                                         LDS, 0, kg, from, to, lane);
   }
 }
@@ -865,7 +870,7 @@ __global__ void __launch_bounds__(64 * KG, 2) serve_few_kernel(const ServeParams
     return;
   }
   tell_joins<M>(p, u, head, u.seq.n * p.G, threadIdx.x);
-  few_rows<BF16, D, KEYS, M, KG, kFewStep<D>, kFewLdsBytes<D>>(p, u, head, rank, u.tile * M, kg, lds_raw, lane);
+  few_rows<BF16, D, KEYS, M, KG, kFewStep<D>, kFewLdsBytes<D>>(p, u, head, u.slot, u.tile * M, kg, lds_raw, lane);
 }
 
 // ---- many rows: four waves per unit -------------------------------------------------------------------------------
@@ -918,7 +923,7 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
     if (p.share == 0.f && u.seq.kv <= kShortKeys) {
       constexpr size_t kOwn = kTileLdsBytes<D, M> / 4;
       const int row0 = u.tile * M + 32 * w;
-      if (row0 < u.seq.n * p.G) few_rows<BF16, D, KEYS, M, 1, 32, kOwn>(p, u, head, rank, row0, 0, lds_raw + w * kOwn, lane);
+      if (row0 < u.seq.n * p.G) few_rows<BF16, D, KEYS, M, 1, 32, kOwn>(p, u, head, u.slot, row0, 0, lds_raw + w * kOwn, lane);
       return;
     }
   }
@@ -1217,14 +1222,14 @@ __global__ void __launch_bounds__(256, 2) serve_tile_kernel(const ServeParams p)
   if constexpr (KG > 1) {
     static_assert(W * kMergeBytes<D> <= kTileLdsBytes<D, M>, "merge layout");
     __syncthreads();  // (the group's other wave may still read V)
-    merge_groups<BF16, D, M, KG, PAGED>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, several, lds_raw,
+    merge_groups<BF16, D, M, KG, PAGED>(p, u, head, u.slot, row0, rows_all, ot, m_run, l_run, several, lds_raw,
                                         kTileLdsBytes<D, M>, w * kMergeBytes<D>, kg, from, to, lane);
     return;
   }
   // (the K tiles are read by nobody any more: a wave stages its rows in a quarter of them)
   const uint32_t odd = several ? odd_rows<DT>(ot) & live_rows(rows_all - row0) : 0u;
-  store_rows<BF16, D, M>(p, u, head, rank, row0, rows_all, ot, m_run, l_run, odd, sK + w * 32 * D, lane);
-  if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, rank, row0, odd, from, to, lane);
+  store_rows<BF16, D, M>(p, u, head, u.slot, row0, rows_all, ot, m_run, l_run, odd, sK + w * 32 * D, lane);
+  if (odd != 0) sum_rows_again<BF16, D, M, PAGED>(p, u, head, u.slot, row0, odd, from, to, lane);
 }
 
 // Joins the parts of a row.  A wave has one token and R of its heads, 16 bytes of a part's row per lane.  Clears the rows
@@ -1257,7 +1262,7 @@ __global__ void __launch_bounds__(256) serve_join_kernel(const ServeParams p) {
   const int head = int(divide(uint32_t(mine ? h : Hq - 1), p.group));
   const int row = (t - first) * p.G + ((mine ? h : Hq - 1) - head * p.G);
   // (a token that no sequence has, where the offsets run backwards, has been told nothing)
-  if (parts < 1 || first < 0 || first > t || before < 0 || before + (int64_t(row / M) + 1) * parts > p.units) return;
+  if (parts < 1 || first < 0 || first > t || before < 0 || before + (int64_t(row / M) + 1) * parts > p.slots) return;
   const int64_t at = ((before + int64_t(row / M) * parts) * p.Hk + head) * M + row % M, step = int64_t(p.Hk) * M;
   float m = -INFINITY;
   for (int i = lane & (LPR - 1); i < parts; i += LPR) m = fmaxf(m, p.stats[(at + i * step) * 2]);

@@ -14,13 +14,19 @@ struct ServePlan {
   int least_steps; // steps that a part may have in any case
   int places;      // units per key head that run at once, where tiles are shared (two workgroups to a compute unit)
   int64_t units;   // units per key head that there is a place for
+  int64_t slots;   // parts per key head that there is a place for in the workspace (whole tiles need none)
   int64_t counted; // sequences whose units a kernel of its own counts, or 0
-  // the parts' rows and statistics, four words per token, one per counted sequence and one more
+  // the parts' rows and statistics, four words per token, two per counted sequence and one more
   size_t workspace_bytes(int64_t T, int Hk, int D) const {
     if (share == 0.f) return 0;
-    return size_t(units) * size_t(Hk) * size_t(rows) * size_t(D + 2) * sizeof(float) + size_t(T) * 16 + size_t(counted) * 4 + 4;
+    return size_t(slots) * size_t(Hk) * size_t(rows) * size_t(D + 2) * sizeof(float) + size_t(T) * 16 + size_t(counted) * 8 + 4;
   }
 };
+
+// Few sequences whose parts are weighed on the device instead of sharing the steps evenly, over a cache alone: at most so many.
+constexpr int weighed_sequences(int rows) { return rows == 128 ? 16 : 8; }
+// ... with `steps` steps in all tiles of a key head, which take more than two rounds of the units that run at once.
+constexpr bool weighed(int64_t B, int rows, float steps, int places) { return B <= weighed_sequences(rows) && steps > 2.f * float(places); }
 
 // T tokens in B sequences, Hk key heads with G query heads each; capacity: keys that a page table has room for, 0:
 // packed; cus: compute units.  Lengths are not known here: a sequence is taken to have T / B tokens, and keys of a
@@ -69,6 +75,10 @@ inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, int64_t capacit
   s.places = 2 * cus >= Hk ? 2 * cus / Hk : 1;
   s.units = tiles + 1 + (parts ? int64_t(s.share) + 1 : 0);
   if (parts && s.rows == 128) s.units += 3 * s.places / 2;  // (three rounds of them)
+  // A tile is cut where it has more steps than a part, so it has less than twice its steps over a part's, and all parts
+  // together are less than twice the share: however many sequences there are.  (1024 single tokens, 32 / 8 heads, D=128: 34 MB for
+  // 153 with a place for every tile; 4096, 32 / 32 heads, 35 MB for 2.2 GB.)  Weighed parts are as many as there are units.
+  s.slots = !parts ? 0 : (B <= weighed_sequences(s.rows) || s.units < 2 * int64_t(s.share) + 2 ? s.units : 2 * int64_t(s.share) + 2);
   return s;
 }
 

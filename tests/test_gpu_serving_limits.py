@@ -1,4 +1,4 @@
-"""Calls of the packed-sequence operators at their limits: offsets that run backwards, values that are no numbers."""
+"""Calls of the packed-sequence operators at their limits: offsets that run backwards, values that are no numbers, scratch memory."""
 import pytest
 import torch
 
@@ -121,3 +121,56 @@ def test_no_numbers_do_not_stop_a_launch(gpu_device, T, Hq, Hk, D, spoilt):
     clean, dirty = fastest(v), fastest(bad)
     # (a row at a time takes 220 - 330 times as long as the launch without; launches and clocks vary by less than 2)
     assert dirty <= 60 * clean, (clean, dirty)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Hq,Hk,D,page", [(9, 8, 8, 64, 64), (40, 8, 2, 128, 64), (64, 4, 1, 32, 16), (300, 8, 1, 64, 128), (1100, 4, 4, 32, 64)])
+def test_cut_and_whole_sequences_side_by_side(gpu_device, dtype, B, Hq, Hk, D, page):
+    """Single tokens whose sequences are cut into many parts, into a few and not at all, in any order, empty ones among them."""
+    gen = torch.Generator().manual_seed(B)
+    lens = [[1, 0, 2][0 if b % 5 else b // 5 % 3] for b in range(B)]
+    kv = [(4000 + 37 * b % 1500 if b % max(B // 6, 4) == 2 else (700 if b % 7 == 1 else 60 + 11 * b % 90)) if b % 9 else 0 for b in range(B)]
+    need = [-(-n // page) for n in kv]
+    pool = [torch.randn(sum(need) + 1, Hk, page, D, generator=gen).to(device=gpu_device, dtype=dtype) for _ in range(2)]
+    table, at = torch.zeros(B, max(need), dtype=torch.int32), 0
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(at, at + n)
+        at += n
+    cu = offsets(lens)
+    q = torch.randn(cu[-1] + 3, Hq, D, generator=gen).to(device=gpu_device, dtype=dtype)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu_device)
+    o, lse = oat.omni_attention_paged(q, pool[0], pool[1], table.to(gpu_device), i32(kv), i32(cu), return_lse=True)
+    assert bool((o[cu[-1]:] == 0).all()) and bool((lse[cu[-1]:] == -float("inf")).all())
+    at = 0
+    for b, n in enumerate(need):
+        rows = slice(cu[b], cu[b + 1])
+        if lens[b]:
+            k, v = (p[at:at + n].transpose(1, 2).reshape(-1, Hk, D)[:kv[b]] for p in pool)
+            want, mean, rl = attention(q[rows], k, v, kv[b] - lens[b], True, 0.0)
+            if kv[b]:
+                smax = (q[rows].double().norm(dim=-1).max() * k.double().norm(dim=-1).max()).item() / D ** 0.5
+                bound = attention_bound(want, mean, 0.0 if dtype == torch.bfloat16 else v.double().abs().sum(0).max().item(), dtype, 0.0, D, smax)
+                assert bool(((o[rows].double() - want).abs() <= bound).all()), b
+                room = (D + 8) * 2.0 ** -24 * smax + 2.0 ** -21 * (1 + rl.abs())
+                live = torch.isfinite(rl)
+                assert torch.equal(torch.isfinite(lse[rows]), live) and bool(((lse[rows].double() - rl).abs() <= room)[live].all()), b
+            else:
+                assert bool((o[rows] == 0).all()) and bool((lse[rows] == -float("inf")).all())
+        at += n
+
+
+def test_scratch_memory_of_many_sequences(gpu_device):
+    """One call's scratch does not grow with the batch: 4096 single tokens of 32 heads."""
+    B, H, D, page, dtype = 4096, 32, 128, 64, torch.bfloat16
+    q = torch.zeros(B, H, D, dtype=dtype, device=gpu_device)
+    kp, vp = (torch.zeros(16, H, page, D, dtype=dtype, device=gpu_device) for _ in range(2))
+    table = torch.zeros(B, 16, dtype=torch.int32, device=gpu_device)
+    kv = torch.full((B,), 100, dtype=torch.int32, device=gpu_device)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=gpu_device)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    o = oat.omni_attention_paged(q, kp, vp, table, kv, cu)
+    torch.cuda.synchronize()
+    assert bool((o == 0).all())
+    assert torch.cuda.max_memory_allocated() - before - o.numel() * 2 <= 64 * 2 ** 20

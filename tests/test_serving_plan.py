@@ -74,3 +74,62 @@ def test_units_of_offsets_that_run_backwards(tmp_path):
         assert outside == 0
         if in_order:
             assert found == tiles
+
+
+# What a launch in parts needs: parts of cut tiles as the device numbers them, and the places that the plan has for them.
+PARTS = r"""
+#include "omni_attn_serving_plan.hpp"
+#include <cmath>
+#include <cstdio>
+#include <vector>
+int main() {
+  int B, Hk, G, D, capacity;
+  while (scanf("%d %d %d %d %d", &B, &Hk, &G, &D, &capacity) == 5) {
+    std::vector<long long> n(B), kv(B);
+    long long T = 0;
+    for (int b = 0; b < B; ++b) {
+      if (scanf("%lld %lld", &n[b], &kv[b]) != 2) return 1;
+      T += n[b];
+    }
+    const omni_attn::ServePlan s = omni_attn::plan_serve(T, B, Hk, G, capacity, 256);
+    const long long M = s.rows;
+    long long cut = 0, most = 0;
+    if (s.share > 0.f) {
+      float all = 0.f;
+      for (int b = 0; b < B; ++b) all += float((n[b] * G + M - 1) / M) * float((kv[b] + 63) / 64);
+      most = (long long)std::ceil(all / s.share);
+      if (most < s.least_steps) most = s.least_steps;
+      for (int b = 0; b < B; ++b) {
+        const long long steps = (kv[b] + 63) / 64;
+        if (steps <= most) continue;
+        const long long parts = (steps + most - 1) / most, each = (steps + parts - 1) / parts;
+        cut += (n[b] * G + M - 1) / M * ((steps + each - 1) / each);
+      }
+    }
+    printf("%d %lld %lld %zu\n", s.share > 0.f, cut, (long long)s.slots, s.workspace_bytes(T, Hk, D));
+  }
+}
+"""
+
+
+def test_workspace_holds_the_parts_and_not_the_batch(tmp_path):
+    """Every part has a place, and the workspace does not grow with the number of sequences, but for the words that each has."""
+    rng = random.Random(2)
+    cases = []
+    for _ in range(2000):
+        B, Hk, G = rng.choice([1, 5, 9, 17, 64, 65, 300, 2000]), rng.choice([1, 2, 8, 24, 32]), rng.choice([1, 2, 4, 8])
+        n = [1] * B if rng.random() < 0.7 else [rng.randint(0, rng.choice([3, 40, 400])) for _ in range(B)]
+        n[0] = max(n[0], 1)
+        long = rng.choice([1, 3, 10])
+        kv = [m + (rng.randint(2000, 60000) if rng.randrange(B) < long else rng.randint(0, rng.choice([10, 2000]))) for m in n]
+        cases.append((B, Hk, G, rng.choice([32, 64, 128]), max(kv) + rng.choice([0, 10 ** 5]), n, kv))
+    for B, Hk, G in ((1024, 8, 4), (4096, 8, 4), (4096, 32, 1), (20000, 1, 1)):
+        cases.append((B, Hk, G, 128, 1 << 17, [1] * B, [500 + b % 500 for b in range(B)]))
+    got = _run(tmp_path, PARTS, [f"{B} {Hk} {G} {D} {c} " + " ".join(f"{a} {b}" for a, b in zip(n, kv)) for B, Hk, G, D, c, n, kv in cases])
+    assert len(got) == len(cases)
+    seen = 0
+    for line, (B, _, _, _, _, n, _) in zip(got, cases):
+        parts, cut, slots, size = map(int, line.split())
+        seen += parts
+        assert cut <= slots and size <= 16 * sum(n) + 8 * B + 4 + 128 * 2 ** 20
+    assert seen > 500
