@@ -2,6 +2,7 @@
 // cache's append, and the attention of packed sequences over their own keys or a paged cache.  Host-only C++ over
 // include/omni_attn_gfx950.h; the reference has no counterpart of these operators.
 #include <torch/extension.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -50,6 +51,14 @@ void check_no_grad(std::initializer_list<Tensor> tensors, const char* op) {
   for (const Tensor& t : tensors)
     if (t.defined() && t.requires_grad())
       refuse(std::string(op) + " is not differentiable: call it under torch.no_grad()");
+}
+
+// A tangent of forward-mode differentiation would be dropped without a word, also under torch.no_grad().
+void check_no_tangent(std::initializer_list<Tensor> tensors, const char* op) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : tensors)
+    if (t.defined() && t._fw_grad(/*level=*/0).defined())
+      refuse(std::string(op) + " has no forward-mode derivative: its operands must not have tangents");
 }
 
 // Rows that the kernels read in place: whole pieces of `piece` elements, up to 2^24 apart ([B, H, S, D]: 2^31).  Others are
@@ -207,6 +216,7 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 
 pybind11::tuple omni_attn_qk_rotary(Tensor q, Tensor k, Tensor positions, Tensor table, OptTensor wq, OptTensor wk, double eps,
                                     bool interleaved) {
+  check_no_tangent({q, k, table, wq.value_or(Tensor()), wk.value_or(Tensor())}, "omni_qk_rotary");
   check_operand(q, "query", q);
   check_operand(k, "key", q);
   require((q.dim() == 3 || q.dim() == 4) && k.dim() == q.dim(), "query and key must be [tokens, heads, head_dim] or [B, H, S, D]");
@@ -275,6 +285,8 @@ int64_t check_batch(Tensor& table, Tensor& lens, Tensor& cu, const Tensor& like,
 pybind11::object omni_attn_cache_append(Tensor k, Tensor v, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor kv_lens,
                                         Tensor cu, OptTensor table, OptTensor positions, OptTensor query, OptTensor wq,
                                         OptTensor wk, double eps, bool interleaved) {
+  check_no_tangent({k, v, k_pages, v_pages, table.value_or(Tensor()), query.value_or(Tensor()), wq.value_or(Tensor()),
+                    wk.value_or(Tensor())}, "omni_cache_append");
   check_operand(k, "key", k);
   check_operand(v, "value", k);
   require(k.dim() == 3 && k.sizes() == v.sizes(), "key and value must be [tokens, kv_heads, head_dim]");
@@ -418,6 +430,7 @@ class PackedFunction : public torch::autograd::Function<PackedFunction> {
 };
 
 pybind11::object omni_attn_packed(Tensor q, Tensor k, Tensor v, Tensor cu, bool causal, double softcap, bool want_lse) {
+  check_no_tangent({q, k, v}, "omni_attention_packed");
   check_operand(q, "query", q);
   check_operand(k, "key", q);
   check_operand(v, "value", q);
@@ -442,6 +455,7 @@ pybind11::object omni_attn_packed(Tensor q, Tensor k, Tensor v, Tensor cu, bool 
 
 pybind11::object omni_attn_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor kv_lens, Tensor cu,
                                  bool causal, double softcap, bool want_lse) {
+  check_no_tangent({q, k_pages, v_pages}, "omni_attention_paged");
   check_operand(q, "query", q);
   require(q.dim() == 3, "query must be [tokens, heads, head_dim]");
   const Pages pages = check_pages(k_pages, v_pages, q);

@@ -839,7 +839,8 @@ def omni_qk_rotary(query: Tensor, key: Tensor, positions: Tensor, table: Tensor,
                    key_norm: Optional[Tensor] = None, eps: float = 1e-6,
                    interleaved: bool = False) -> Tuple[Tensor, Tensor]:
     """Query and key heads normed by their root mean square (with weights ``query_norm``, ``key_norm`` [head_dim], where
-    given) and rotated by their positions, in one pass; differentiable in query, key and the weights.
+    given) and rotated by their positions, in one pass; differentiable in query, key and the weights (tangents of
+    forward-mode differentiation are refused).
 
     query, key   [B, H, S, head_dim] or packed [tokens, H, head_dim], fp16 / bf16, each with its own number of heads; any
                  strides (rows that are not multiples of 4 elements apart are copied).  head_dim: multiples of 8 up to 256
@@ -890,7 +891,8 @@ def omni_attention_packed(query: Tensor, key: Tensor, value: Tensor, cu_seqlens:
     ``omni_cache_append``.  ``causal``: a token attends itself and those before it; else its whole sequence.  ``softcap``
     as in ``omni_attention``.  Returns [tokens, heads, head_dim], with ``return_lse`` also the fp32 logsumexp
     [tokens, heads].  Tokens behind the last sequence get zeros (-inf).  Differentiable in query, key and value (not
-    through the logsumexp); the gradients take the operands to be finite."""
+    through the logsumexp; tangents of forward-mode differentiation are refused); the gradients take the operands to be
+    finite."""
     return _load_extension().omni_attn_packed(query, key, value, cu_seqlens, bool(causal), float(softcap), bool(return_lse))
 
 
