@@ -127,6 +127,11 @@ void check_rotation(Rotation& r, const Tensor& q, int64_t D) {
   if (r.wq.defined()) r.wq = aligned(r.wq);
   if (r.wk.defined()) r.wk = aligned(r.wk);
 }
+// Learned frequencies have no gradient here: refused, where one would be missing.
+void check_table_grad(const Tensor& table) {
+  if (at::GradMode::is_enabled() && table.defined() && table.requires_grad())
+    refuse("table must not require a gradient: the operators have none for it");
+}
 void check_head_dim(int64_t D) {
   if (D < 8 || D > 256 || D % 8 != 0)
     refuse("Unsupported head_dim=" + std::to_string(D) + ". Supported values: multiples of 8 up to 256.");
@@ -217,6 +222,7 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 pybind11::tuple omni_attn_qk_rotary(Tensor q, Tensor k, Tensor positions, Tensor table, OptTensor wq, OptTensor wk, double eps,
                                     bool interleaved) {
   check_no_tangent({q, k, table, wq.value_or(Tensor()), wk.value_or(Tensor())}, "omni_qk_rotary");
+  check_table_grad(table);
   check_operand(q, "query", q);
   check_operand(k, "key", q);
   require((q.dim() == 3 || q.dim() == 4) && k.dim() == q.dim(), "query and key must be [tokens, heads, head_dim] or [B, H, S, D]");
@@ -287,6 +293,7 @@ pybind11::object omni_attn_cache_append(Tensor k, Tensor v, Tensor k_pages, Tens
                                         OptTensor wk, double eps, bool interleaved) {
   check_no_tangent({k, v, k_pages, v_pages, table.value_or(Tensor()), query.value_or(Tensor()), wq.value_or(Tensor()),
                     wk.value_or(Tensor())}, "omni_cache_append");
+  check_table_grad(table.value_or(Tensor()));
   check_operand(k, "key", k);
   check_operand(v, "value", k);
   require(k.dim() == 3 && k.sizes() == v.sizes(), "key and value must be [tokens, kv_heads, head_dim]");

@@ -847,7 +847,7 @@ def omni_qk_rotary(query: Tensor, key: Tensor, positions: Tensor, table: Tensor,
     positions    rows of ``table``: [S] or [B, S] (packed: [tokens]), int32 or int64; the tokens of an image may share
                  one.  Positions outside the table read its first or last row
     table        omni_rotary_table(rotary_dim, ...); rotary_dim a multiple of 8 up to head_dim, the dimensions behind
-                 it are normed and not rotated
+                 it are normed and not rotated.  It has no gradient, and is refused where it requires one
     interleaved  pairs are (2i, 2i + 1); else (i, i + rotary_dim / 2)
 
     The results lie in memory as the operands do, so a projection's [B, S, H, D] seen as [B, H, S, D] goes into

@@ -41,3 +41,12 @@ def test_tangents_are_refused(op, name):
             CALLS[op](**{name: dual})
         with pytest.raises(ValueError, match="GPU tensor"):  # (without tangents the next check speaks)
             CALLS[op]()
+
+
+@pytest.mark.parametrize("op", ["rotary", "append"])
+def test_tables_that_require_a_gradient_are_refused(op):
+    learned = TABLE.clone().requires_grad_()
+    with pytest.raises(ValueError, match="table must not require a gradient"):
+        CALLS[op](table=learned)
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU tensor"):  # (nothing is lost: the next check speaks)
+        CALLS[op](table=learned)
