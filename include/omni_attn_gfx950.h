@@ -367,7 +367,8 @@ int omni_attn_qk_rotary_bwd_gfx950(const void* dq_out, const void* dk_out, const
  *              through bit for bit.
  *   q, q_out   [tokens, Hq, D], or NULL with Hq = 0: the tokens' queries, normed and rotated beside them.
  *   positions  [tokens]: table rows to rotate by, or NULL: the token's position in its sequence.
- *   k_pages, v_pages  [num_pages, Hk, page_size, D] contiguous; page_size a power of two.
+ *   k_pages, v_pages  [num_pages, Hk, page_size, D] contiguous, apart from one another and from the operands; page_size a
+ *              power of two.
  *   page_table [sequences, max_pages] int32.
  * A token whose page number is outside [0, num_pages), or whose position is negative or behind the page table, is not
  * written; nor is anything but the new tokens' rows.  Two new tokens must not name one row.  q_out rows of tokens behind

@@ -301,6 +301,10 @@ pybind11::object omni_attn_cache_append(Tensor k, Tensor v, Tensor k_pages, Tens
   const int64_t T = k.size(0), D = k.size(2);
   check_head_dim(D);
   require(pages.Hk == k.size(1) && pages.D == D, "key_pages must have the heads and head_dim of key");
+  {
+    const char *a = static_cast<const char*>(k_pages.data_ptr()), *b = static_cast<const char*>(v_pages.data_ptr());
+    require((a > b ? a - b : b - a) >= int64_t(k_pages.nbytes()), "key_pages and value_pages must not overlap");
+  }
   require(k.size(1) <= 65536 && T <= 0x7fffffff, "key is too large");
   c10::DeviceGuard guard(k.device());
   const int64_t B = check_batch(page_table, kv_lens, cu, k, pages);

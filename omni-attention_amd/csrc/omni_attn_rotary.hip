@@ -745,6 +745,11 @@ extern "C" int omni_attn_cache_append_gfx950(
     if (const int rc = check_rows(ptrs[i], *ats[i])) return rc;
     wide = wide && wide_rows(ptrs[i], *ats[i]);
   }
+  {  // (a row would get the key and the value of a token, in any order)
+    const uintptr_t k0 = reinterpret_cast<uintptr_t>(k_pages), v0 = reinterpret_cast<uintptr_t>(v_pages);
+    const uint64_t bytes = uint64_t(num_pages) * uint64_t(Hk) * uint64_t(page_size) * uint64_t(D) * 2;
+    if ((k0 > v0 ? k0 - v0 : v0 - k0) < bytes) return OMNI_ATTN_ERR_BAD_SHAPE;
+  }
   AppendParams ap{};
   RotaryParams& p = ap.r;
   p.q = {static_cast<const uint16_t*>(q_or_null), static_cast<uint16_t*>(q_out_or_null), strides(q_at), strides(q_out_at), q_weight_or_null, Hq};

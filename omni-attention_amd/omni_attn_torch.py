@@ -866,8 +866,9 @@ def omni_cache_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages
     are normed and rotated in the same launch and returned.
 
     key, value   [tokens, kv_heads, head_dim], the sequences' new tokens one behind the other
-    key_pages, value_pages  [num_pages, kv_heads, page_size, head_dim] contiguous, written in place; page_size a power of
-                 two from 16 (from 64 on a step of the attention looks up one page)
+    key_pages, value_pages  [num_pages, kv_heads, page_size, head_dim] contiguous, written in place, two tensors that do not
+                 overlap, nor the operands; page_size a power of two from 16 (from 64 on a step of the attention looks up
+                 one page)
     page_table   [sequences, max_pages] int32: the pages of each sequence, in order
     kv_lens      [sequences] int32: keys of each sequence, the new ones included
     cu_seqlens   [sequences + 1] int32, 0 first and not decreasing: sequence b has the tokens cu_seqlens[b] ..
