@@ -1,7 +1,14 @@
-"""What the kernels of packed sequences count and number on the device, on the CPU: units of batches whose offsets may be anything."""
+"""What the kernels of packed sequences count and number on the device, on the CPU: units of batches whose offsets may be
+anything, places of parts, and which batches' parts are weighed."""
+import math
 import os
 import random
 import subprocess
+
+import pytest
+import torch
+
+from serving_weighed import CHUNKS, FEW, bound, make, reference
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "omni-attention_amd", "csrc")
 
@@ -133,3 +140,55 @@ def test_workspace_holds_the_parts_and_not_the_batch(tmp_path):
         seen += parts
         assert cut <= slots and size <= 16 * sum(n) + 8 * B + 4 + 128 * 2 ** 20
     assert seen > 500
+
+
+WEIGHED = r"""
+#include "omni_attn_serving_plan.hpp"
+#include <cstdio>
+int main() {
+  int B, Hk, G, capacity;
+  while (scanf("%d %d %d %d", &B, &Hk, &G, &capacity) == 4) {
+    long long T = 0, n[64], kv[64];
+    for (int b = 0; b < B; ++b) {
+      if (scanf("%lld %lld", n + b, kv + b) != 2) return 1;
+      T += n[b];
+    }
+    const omni_attn::ServePlan s = omni_attn::plan_serve(T, B, Hk, G, capacity, 256);
+    float all = 0.f;
+    for (int b = 0; b < B; ++b) all += float((n[b] * G + s.rows - 1) / s.rows) * float((kv[b] + 63) / 64);
+    printf("%d %d %d\n", s.rows, s.waves, int(s.share > 0.f && omni_attn::weighed(B, s.rows, all, s.places)));
+  }
+}
+"""
+
+
+def test_the_weighed_batches_are_weighed(tmp_path):
+    """The batches that stand for weighed parts take that path on a card of 256 compute units: the single tokens and a few in
+    tiles of 32 rows, the chunks in tiles of 128."""
+    lines = []
+    for lens, cached, Hq, Hk, _ in FEW + CHUNKS:
+        total = [n + c for n, c in zip(lens, cached)]
+        lines.append(f"{len(lens)} {Hk} {Hq // Hk} {max(total)} " + " ".join(f"{n} {m}" for n, m in zip(lens, total)))
+    got = [tuple(map(int, x.split())) for x in _run(tmp_path, WEIGHED, lines)]
+    assert got == [(32, 4, 1)] * len(FEW) + [(128, 4, 1)] * len(CHUNKS)
+
+
+@pytest.mark.parametrize("case", range(len(FEW) + len(CHUNKS)))
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_the_bound_of_the_weighed_batches_tells_results_from_none(case, dtype):
+    """An output of zeros, and one that leaves an eighth of the keys out, is beyond the bound in most elements."""
+    lens, cached, Hq, Hk, D = (FEW + CHUNKS)[case]
+    q, rows = make(torch.Generator().manual_seed(case), lens, cached, Hq, Hk, D, dtype)
+    b = max(range(len(lens)), key=lambda i: cached[i] * (lens[i] > 0))
+    at = sum(lens[:b])
+    k, v = rows[b]
+    q = q[at:at + lens[b]][-2:, :Hq // Hk]  # the sequence's last rows, one key head
+    k, v = k[:, :1], v[:, :1]
+    first = k.shape[0] - q.shape[0]
+    want, mean, _, spread = reference(q, k, v, first, True)
+    smax = (q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max()).item() / math.sqrt(D)
+    room = bound(want, mean, spread, dtype, D, smax)
+    assert (want.abs() > room).double().mean().item() > 0.9
+    cut = k.shape[0] // 8
+    fewer = reference(q, k[cut:], v[cut:], first - cut, True)[0]
+    assert ((fewer - want).abs() > room).double().mean().item() > 0.7  # (a fifth of the dimensions have no slope)
