@@ -1,4 +1,5 @@
-"""Calls of the packed-sequence operators at their limits: offsets that run backwards, values that are no numbers, scratch memory."""
+"""Calls of the packed-sequence operators at their limits: offsets that run backwards, values that are no numbers, scratch memory,
+large groups, operands beyond 2^31 elements, an append of many sequences."""
 import pytest
 import torch
 
@@ -174,3 +175,106 @@ def test_scratch_memory_of_many_sequences(gpu_device):
     torch.cuda.synchronize()
     assert bool((o == 0).all())
     assert torch.cuda.max_memory_allocated() - before - o.numel() * 2 <= 64 * 2 ** 20
+
+
+@pytest.mark.parametrize("Hq,Hk,D", [(200, 1, 64), (300, 2, 32), (130, 1, 128)])
+def test_more_heads_in_a_group_than_rows_in_a_tile(gpu_device, Hq, Hk, D):
+    """A token's heads fill more than a tile: prompts, single tokens in parts, and gradients as the sums over single heads."""
+    gen = torch.Generator().manual_seed(Hq)
+    dtype, lens = torch.bfloat16, [5, 1, 90]
+    T, at = sum(lens), offsets(lens)
+    q, k, v, do = (torch.randn(T, h, D, generator=gen).to(device=gpu_device, dtype=dtype) for h in (Hq, Hk, Hk, Hq))
+    cu = torch.tensor(at, dtype=torch.int32, device=gpu_device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o, lse = oat.omni_attention_packed(*leaves, cu, return_lse=True)
+    grads = torch.autograd.grad(o, leaves, do)
+    one_by_one = [torch.zeros(t.shape, dtype=torch.float64, device=gpu_device) for t in leaves]
+    size = torch.zeros(2, dtype=torch.float64)
+    for h in range(0, Hq, Hq // Hk):
+        for i in range(h, h + Hq // Hk, 10):
+            heads, y = slice(i, min(i + 10, h + Hq // Hk)), slice(h * Hk // Hq, h * Hk // Hq + 1)
+            part = [t.detach().clone().requires_grad_() for t in (q[:, heads], k[:, y], v[:, y])]
+            out = oat.omni_attention_packed(*part, cu)
+            # (the same products in another tile: as many keys, the same order)
+            assert (out.float() - o[:, heads].float()).abs().max().item() <= 4 * 4 * torch.finfo(dtype).eps / 2
+            g = torch.autograd.grad(out, part, do[:, heads])
+            one_by_one[0][:, heads] = g[0].double()
+            for n in (1, 2):
+                one_by_one[n][:, y] += g[n].double()
+                size[n - 1] += g[n].double().abs().max().item()
+    # each part is rounded once, and the whole once: half a step of the largest parts
+    eps = torch.finfo(dtype).eps / 2
+    assert (grads[0].double() - one_by_one[0]).abs().max().item() <= 8 * eps * one_by_one[0].abs().max().item()
+    for n in (1, 2):
+        assert (grads[n].double() - one_by_one[n]).abs().max().item() <= 2 * eps * size[n - 1].item() + eps * grads[n].double().abs().max().item()
+    kp, vp, table = _paged_of(gen, torch.randn(6000, Hk, D, generator=gen).to(device=gpu_device, dtype=dtype),
+                              torch.randn(6000, Hk, D, generator=gen).to(device=gpu_device, dtype=dtype), [5000, 1000], 64)
+    kv = torch.tensor([5000, 1000], dtype=torch.int32, device=gpu_device)
+    cu = torch.tensor([0, 1, 3], dtype=torch.int32, device=gpu_device)
+    o, lse = oat.omni_attention_paged(q[:3].detach(), kp, vp, table, kv, cu, return_lse=True)
+    for b, (a, e) in enumerate(((0, 1), (1, 3))):
+        n = int(kv[b])
+        keys, values = (p[table[b].long()].transpose(1, 2).reshape(-1, Hk, D)[:n] for p in (kp, vp))
+        want, mean, rl = attention(q[a:e].detach(), keys, values, n - (e - a), True, 0.0)
+        smax = (q[a:e].double().norm(dim=-1).max() * keys.double().norm(dim=-1).max()).item() / D ** 0.5
+        assert bool(((o[a:e].double() - want).abs() <= attention_bound(want, mean, 0.0, dtype, 0.0, D, smax)).all())
+        assert bool(((lse[a:e].double() - rl).abs() <= (D + 8) * 2.0 ** -24 * smax + 2.0 ** -21 * (1 + rl.abs())).all())
+
+
+def test_packed_rows_beyond_32_bits(gpu_device):
+    """More than 2^31 elements in every operand: the last sequences, their gradients and the rows behind them."""
+    gen = torch.Generator().manual_seed(3)
+    dtype, H, D, n = torch.bfloat16, 64, 128, 300
+    behind = 5
+    T = (1 << 31) // (H * D) + 2 * n + behind
+    tail = [torch.randn(2 * n, H, D, generator=gen).to(device=gpu_device, dtype=dtype) for _ in range(4)]
+    lens = [700] * ((T - behind - 2 * n) // 700)
+    lens += [T - behind - 2 * n - sum(lens), n, n]
+    cu = torch.tensor(offsets(lens), dtype=torch.int32, device=gpu_device)
+    q, k, v, do = (torch.zeros(T, H, D, dtype=dtype, device=gpu_device) for _ in range(4))
+    rows = slice(T - behind - 2 * n, T - behind)
+    for x, t in zip((q, k, v, do), tail):
+        x[rows] = t
+        x[T - behind:] = 1.0
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o, lse = oat.omni_attention_packed(*leaves, cu, return_lse=True)
+    grads = torch.autograd.grad(o, leaves, do)
+    assert bool((o[T - behind:] == 0).all()) and bool((lse[T - behind:] == -float("inf")).all())
+    assert all(bool((g[T - behind:] == 0).all()) for g in grads)
+    small = [t.clone().requires_grad_() for t in tail[:3]]
+    two = torch.tensor([0, n, 2 * n], dtype=torch.int32, device=gpu_device)
+    want, want_lse = oat.omni_attention_packed(*small, two, return_lse=True)
+    want_grads = torch.autograd.grad(want, small, tail[3])
+    # (another form may take the same rows: weights and results rounded to half a step of values of at most 6 each)
+    eps = torch.finfo(dtype).eps / 2
+    assert (o[rows].float() - want.float()).abs().max().item() <= 4 * 6 * eps
+    assert (lse[rows] - want_lse).abs().max().item() <= 1e-4
+    for g, w in zip(grads, want_grads):
+        assert (g[rows].float() - w.float()).abs().max().item() <= 16 * eps * w.float().abs().max().item()
+    assert bool((o[:rows.start] == 0).all())
+
+
+@pytest.mark.parametrize("B", [65, 128, 129, 5000])
+def test_append_of_many_sequences(gpu_device, B):
+    """More sequences than a wave has lanes, some without a new token: every token finds its own."""
+    gen = torch.Generator().manual_seed(B)
+    dtype, Hk, D, page = torch.float16, 2, 32, 16
+    lens = torch.randint(0, 4, (B,), generator=gen).tolist()
+    lens[0], lens[1], lens[B - 1] = 0, 3, 2
+    cached = torch.randint(0, 30, (B,), generator=gen).tolist()
+    T = sum(lens) + 2
+    k, v, q = (torch.randn(T, Hk, D, generator=gen).to(device=gpu_device, dtype=dtype) for _ in range(3))
+    kp, vp = (torch.zeros(3 * B, Hk, page, D, dtype=dtype, device=gpu_device) for _ in range(2))
+    table = torch.randperm(3 * B, generator=gen).to(torch.int32).view(B, 3)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu_device)
+    y = oat.omni_cache_append(k, v, kp, vp, table.to(gpu_device), i32([n + c for n, c in zip(lens, cached)]), i32(offsets(lens)), query=q)
+    want_k, want_v = torch.zeros_like(kp), torch.zeros_like(vp)
+    pages, at = [], []
+    for b, (n, c) in enumerate(zip(lens, cached)):
+        for i in range(c, c + n):
+            pages.append(int(table[b, i // page]))
+            at.append(i % page)
+    pages, at = torch.tensor(pages, device=gpu_device), torch.tensor(at, device=gpu_device)
+    want_k[pages, :, at], want_v[pages, :, at] = k[:T - 2], v[:T - 2]
+    assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+    assert torch.equal(y[:T - 2], q[:T - 2]) and bool((y[T - 2:] == 0).all())
