@@ -42,10 +42,10 @@ inline ServePlan plan_serve(int64_t T, int64_t B, int Hk, int G, int64_t capacit
   s.least_steps = 2;
   if (all <= 64 * B) {
     // Single tokens, a few.  One wave per tile where keys are few and tiles more than the card holds at a time: D=128, 32 / 8
-    // heads, 512 sequences of 30 - 100 keys 34 us, 58 with four waves, 110 with four and parts; 256 of 100 - 300 keys 41, 47
-    // and 61; 200 prompts of 60 tokens 24 and 41.  Else four waves and parts: 8 tokens after 2000 keys 22 us, 34 with whole
-    // tiles, 106 with one wave; after 60000 keys 345, 900 and 3232; 64 tokens after 500 - 1500 keys 50 us, 44 with whole tiles
-    // (lengths are not known here).  Twice as many units or half as many: within 3 %.
+    // heads, 512 sequences of 30 - 100 keys 28 us, 46 with four waves, 52 with four waves and parts; 256 of 100 - 300 keys 37, 39
+    // and 45; 200 prompts of 60 tokens, as many key heads, 24 and 41.  Else four waves and parts: 8 tokens after 60000 keys 343,
+    // 616 with whole tiles, 2160 with one wave (8 after 2000 keys 26 us, 23 and 65, 64 after 500 - 1500 keys 51, 44 and 58: what
+    // this loses by, lengths are not known here).  Twice as many units or half as many: within 3 %.
     if ((keys <= 512 && tiles_of(32) * Hk > 4 * cus) || (capacity == 0 && keys <= 128)) s.waves = 1;
     if (s.waves == 4 && keys > 512) wanted = 4 * cus;
     s.least_steps = 4;
