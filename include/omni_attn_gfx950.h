@@ -398,7 +398,7 @@ int omni_attn_cache_append_gfx950(const void* q_or_null, const void* k, const vo
  *              Rows without a key, and rows of tokens behind the last sequence, are zeros (lse -inf).
  *   workspace  omni_attn_packed_workspace_bytes, omni_attn_paged_workspace_bytes of the current device (may be 0),
  *              16-byte aligned; its contents before and after the call are meaningless.  It holds the parts that long caches are
- *              cut into, up to about 100 MiB, and 16 bytes per token and 8 per sequence.
+ *              cut into, up to about 140 MiB for 128 key heads or fewer, and 16 bytes per token and 8 per sequence.
  * D is 32, 64 or 128; softcap as in omni_attn_fwd_gfx950.  Two calls that may run at the same time need two workspaces.
  */
 size_t omni_attn_packed_workspace_bytes(int tokens, int sequences, int Hq, int Hk, int D);

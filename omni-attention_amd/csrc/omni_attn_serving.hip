@@ -56,7 +56,7 @@ int check_pages(int num_pages, int page_size, int max_pages) {
   return (long long)max_pages * page_size > 0x3fffffffLL ? OMNI_ATTN_ERR_TOO_LARGE : OMNI_ATTN_OK;
 }
 
-// Counts the units of more sequences than a wave has lanes, in one workgroup.
+// Counts the units, and the places of parts, of more sequences than a wave has lanes, in one workgroup.
 template <int M>
 __global__ void __launch_bounds__(1024) serve_count_kernel(const ServeParams p) {
   __shared__ float steps[16];
